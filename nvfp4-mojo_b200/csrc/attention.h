@@ -1,0 +1,18 @@
+// attention.h -- internals shared by the attention translation units
+// (include/nvfp4_attention.h).
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/nvfp4_attention.h"
+
+namespace nvfp4 {
+
+// Checks of the structs that both entry points take: NVFP4_OK, or an error
+// with its message recorded.
+int check_kv_cache(const nvfp4_kv_cache *c);
+int check_attention_batch(const nvfp4_attention_batch *b, int page_size);
+
+}  // namespace nvfp4

@@ -1,0 +1,13 @@
+// attention_launch.h -- host launchers of the attention kernels.
+#pragma once
+
+#include "attention.cuh"
+
+namespace nvfp4 {
+
+// attention_rows.cu: items of R = 16 or 32 rows (16 above head size 128), and
+// the launch that joins what its blocks cut.
+cudaError_t launch_attn_rows(const CUtensorMap &tk, const CUtensorMap &tv, const AttnArgs &a, int R,
+                             int grid, cudaStream_t st);
+
+}  // namespace nvfp4

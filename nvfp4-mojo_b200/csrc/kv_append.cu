@@ -1,0 +1,367 @@
+// kv_append.cu -- appending keys and values to the paged cache, with the
+// heads' norm and the position rotation on the way (include/nvfp4_attention.h).
+//
+// A row (one head of one token) belongs to a group of lanes of one warp, each
+// holding 4 rotation pairs in registers; the group sums the squares for the
+// norm by shuffles, turns its pairs and stores them.  A warp keeps its token's
+// sines and cosines in registers and walks over that token's heads, so the
+// angles (the only 64-bit arithmetic) are computed once per token and warp.
+// HBM-bound for many tokens, latency-bound for a few: then a token's heads are
+// spread over more warps.
+#include <cuda_bf16.h>
+
+#include "../../include/nvfp4.h"
+#include "abi_util.h"
+#include "attention.h"
+#include "kernels.h"
+
+namespace nvfp4 {
+
+int check_kv_cache(const nvfp4_kv_cache *c) {
+  if (!c) return fail(NVFP4_ERR_INVALID_ARG, "null cache");
+  if (c->head_dim <= 0 || c->head_dim > 256 || c->head_dim % 8)
+    return fail(NVFP4_ERR_UNSUPPORTED, "head_dim %d: multiples of 8 up to 256", c->head_dim);
+  if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)))
+    return fail(NVFP4_ERR_UNSUPPORTED, "page_size %d: powers of two from 16 to 256", c->page_size);
+  if (c->num_kv_heads <= 0 || c->num_kv_heads > 65535 || c->num_pages < 0 || c->num_pages > INT32_MAX)
+    return fail(NVFP4_ERR_INVALID_ARG, "bad cache shape: %lld pages, %d heads", (long long)c->num_pages,
+                c->num_kv_heads);
+  for (int i = 0; i < 3; ++i)
+    if (c->k_strides[i] <= 0 || c->v_strides[i] <= 0 || c->k_strides[i] % 8 || c->v_strides[i] % 8 ||
+        c->k_strides[i] >= (1ll << 38) || c->v_strides[i] >= (1ll << 38))
+      return fail(NVFP4_ERR_INVALID_ARG, "cache strides must be positive multiples of 8 elements");
+  if (c->num_pages > 0 && (!c->k || !c->v)) return fail(NVFP4_ERR_INVALID_ARG, "null cache pointer");
+  if (!aligned(c->k, 16) || !aligned(c->v, 16))
+    return fail(NVFP4_ERR_INVALID_ARG, "cache must be 16-byte aligned");
+  return NVFP4_OK;
+}
+
+int check_attention_batch(const nvfp4_attention_batch *b, int page_size) {
+  if (!b) return fail(NVFP4_ERR_INVALID_ARG, "null batch");
+  if (b->num_seqs < 0 || b->num_seqs > (1 << 20) || b->num_tokens < 0 || b->num_tokens > (1 << 24) ||
+      b->max_q_len < 0)
+    return fail(NVFP4_ERR_INVALID_ARG, "bad batch: %d sequences, %lld tokens, max_q_len %d", b->num_seqs,
+                (long long)b->num_tokens, b->max_q_len);
+  if (!b->q_start && b->num_seqs != b->num_tokens)
+    return fail(NVFP4_ERR_INVALID_ARG, "without q_start every sequence has one token: %d sequences, %lld tokens",
+                b->num_seqs, (long long)b->num_tokens);
+  if (b->num_tokens > 0 && b->num_seqs > 0 && b->max_q_len < 1)
+    return fail(NVFP4_ERR_INVALID_ARG, "max_q_len %d with %lld tokens", b->max_q_len, (long long)b->num_tokens);
+  if (b->prefix_len < 0 || b->max_pages < 0 ||
+      (int64_t)b->max_pages * page_size + b->prefix_len + b->num_tokens > (1ll << 30))
+    return fail(NVFP4_ERR_INVALID_ARG, "bad lengths: max_pages %d, prefix_len %d", b->max_pages, b->prefix_len);
+  if (b->prefix_len > 0 && !b->prefix_pages) return fail(NVFP4_ERR_INVALID_ARG, "null prefix_pages");
+  if (b->num_seqs > 0 && !b->kv_len) return fail(NVFP4_ERR_INVALID_ARG, "null kv_len");
+  if (b->num_seqs > 0 && b->max_pages > 0 && (!b->page_table || b->page_table_stride < b->max_pages))
+    return fail(NVFP4_ERR_INVALID_ARG, "null page_table or stride below max_pages");
+  return NVFP4_OK;
+}
+
+namespace {
+
+constexpr int kAppendWarps = 8;
+
+struct AppendArgs {
+  nvfp4_kv_cache c;
+  nvfp4_attention_batch b;
+  nvfp4_rotary rot;  // rotary_dim 0: none
+  nvfp4_qk_norm norm;
+  nvfp4_head_rows q, k, v, qo;
+  const int32_t *pos;
+  int64_t pos_stride;
+  int num_axes, num_heads, page_shift;
+  int chunks;       // warps per token
+  int chunk_rows;   // rows (heads of q, k, v in that order) per warp
+};
+
+__device__ __forceinline__ float bf(uint32_t w, int hi) {
+  return __uint_as_float(hi ? (w & 0xffff0000u) : (w << 16));
+}
+
+// Pairs p0 .. p0+3 of a row: first members at i0, second at i1 (VEC: both
+// runs of 4 consecutive elements; interleaved: one run of 8 at i0).
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_pairs(const T *row, const int (&ei)[4], const int (&ej)[4],
+                                           bool inter, float (&a)[4], float (&b)[4]) {
+  if constexpr (VEC && sizeof(T) == 2) {
+    uint32_t w[4];
+    if (inter) {
+      const uint4 q = *reinterpret_cast<const uint4 *>(row + ei[0]);
+      w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = bf(w[i], 0), b[i] = bf(w[i], 1);
+    } else {
+      const uint2 x = *reinterpret_cast<const uint2 *>(row + ei[0]);
+      const uint2 y = *reinterpret_cast<const uint2 *>(row + ej[0]);
+      a[0] = bf(x.x, 0), a[1] = bf(x.x, 1), a[2] = bf(x.y, 0), a[3] = bf(x.y, 1);
+      b[0] = bf(y.x, 0), b[1] = bf(y.x, 1), b[2] = bf(y.y, 0), b[3] = bf(y.y, 1);
+    }
+  } else if constexpr (VEC) {
+    if (inter) {
+      const float4 x = *reinterpret_cast<const float4 *>(row + ei[0]);
+      const float4 y = *reinterpret_cast<const float4 *>(row + ei[0] + 4);
+      a[0] = x.x, b[0] = x.y, a[1] = x.z, b[1] = x.w;
+      a[2] = y.x, b[2] = y.y, a[3] = y.z, b[3] = y.w;
+    } else {
+      const float4 x = *reinterpret_cast<const float4 *>(row + ei[0]);
+      const float4 y = *reinterpret_cast<const float4 *>(row + ej[0]);
+      a[0] = x.x, a[1] = x.y, a[2] = x.z, a[3] = x.w;
+      b[0] = y.x, b[1] = y.y, b[2] = y.z, b[3] = y.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = ei[i] < 0 ? 0.0f : (float)row[ei[i]];
+      b[i] = ej[i] < 0 ? 0.0f : (float)row[ej[i]];
+    }
+  }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store_pairs(__nv_bfloat16 *row, const int (&ei)[4], const int (&ej)[4],
+                                            bool inter, const float (&a)[4], const float (&b)[4]) {
+  if constexpr (VEC) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = inter ? __floats2bfloat162_rn(a[i], b[i])
+                               : i < 2 ? __floats2bfloat162_rn(a[2 * i], a[2 * i + 1])
+                                       : __floats2bfloat162_rn(b[2 * i - 4], b[2 * i - 3]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    if (inter) {
+      *reinterpret_cast<uint4 *>(row + ei[0]) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+      *reinterpret_cast<uint2 *>(row + ei[0]) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2 *>(row + ej[0]) = make_uint2(w[2], w[3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (ei[i] >= 0) row[ei[i]] = __float2bfloat16(a[i]);
+      if (ej[i] >= 0) row[ej[i]] = __float2bfloat16(b[i]);
+    }
+  }
+}
+
+// LPR lanes per row (4 pairs each), 32 / LPR rows per warp step.
+template <typename T, int LPR, bool VEC>
+__global__ void __launch_bounds__(kAppendWarps * 32) kv_append_kernel(AppendArgs a) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  constexpr int RPW = 32 / LPR;
+  const int lane = threadIdx.x & 31, sub = lane / LPR, l = lane % LPR;
+  const int64_t unit = (int64_t)blockIdx.x * kAppendWarps + (threadIdx.x >> 5);
+  const int64_t t = unit / a.chunks;
+  if (t >= a.b.num_tokens) return;
+  const int chunk = (int)(unit % a.chunks);
+
+  // The token's sequence: token t itself in a step of single tokens (checked
+  // first), else by bisection of q_start.
+  int b = (int)t, qs = (int)t, qe = (int)t + 1;
+  if (a.b.q_start) {
+    const int B = a.b.num_seqs;
+    b = min(b, B - 1);
+    if (!(a.b.q_start[b] <= t && t < a.b.q_start[b + 1])) {
+      int lo = 0, hi = B;  // the first b with q_start[b + 1] > t
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (a.b.q_start[mid + 1] > t) hi = mid;
+        else lo = mid + 1;
+      }
+      b = lo;
+      if (b >= B || a.b.q_start[b] > t) return;  // in no sequence
+    }
+    qs = a.b.q_start[b];
+    qe = a.b.q_start[b + 1];
+  }
+  const int64_t key = (int64_t)a.b.kv_len[b] - qe + t;  // own key index
+  const int64_t at = key >> a.page_shift;
+  int64_t page = -1;
+  if (key >= 0 && at < a.b.max_pages) page = a.b.page_table[b * a.b.page_table_stride + at];
+  const bool cached = page >= 0 && page < a.c.num_pages;
+  const int slot = (int)(key & (a.c.page_size - 1));
+
+  // This lane's pairs: p < rotary_dim / 2 are turned; the rest of the head is
+  // paired half against half and only normed.
+  const int D = a.c.head_dim, R = a.rot.rotary_dim, half = R / 2;
+  const bool inter = a.rot.interleaved;
+  const bool active = l * 8 < D;
+  int ei[4], ej[4];
+  float cs[4], sn[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int p = 4 * l + i;
+    ei[i] = ej[i] = -1;
+    cs[i] = 1.0f, sn[i] = 0.0f;
+    if (2 * p < D) {
+      if (inter) ei[i] = 2 * p, ej[i] = 2 * p + 1;
+      else if (p < half) ei[i] = p, ej[i] = p + half;
+      else ei[i] = R + (p - half), ej[i] = R + (p - half) + (D - R) / 2;
+      if (p < half) {
+        int axis = a.rot.axis ? a.rot.axis[p] : 0;
+        axis = axis < 0 ? 0 : axis >= a.num_axes ? a.num_axes - 1 : axis;
+        const int64_t pos = a.pos ? a.pos[axis * a.pos_stride + t] : key + a.b.prefix_len;
+        // Whole turns are taken off in 64 bits: pos * inv_freq / (2 pi) keeps
+        // 2^-53 of up to 2^31 turns, far below fp32's step of the remainder.
+        const double turns = (double)pos * (double)a.rot.inv_freq[p] * 0.15915494309189533577;
+        sincospif(2.0f * (float)(turns - rint(turns)), &sn[i], &cs[i]);
+        cs[i] *= a.rot.scale;
+        sn[i] *= a.rot.scale;
+      }
+    }
+  }
+  float wq[2][4], wk[2][4];  // norm weights of the pairs' members
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(a.norm.q_weight);
+    const __nv_bfloat16 *k = static_cast<const __nv_bfloat16 *>(a.norm.k_weight);
+    wq[0][i] = q && ei[i] >= 0 ? __bfloat162float(q[ei[i]]) + a.norm.weight_offset : 1.0f;
+    wq[1][i] = q && ej[i] >= 0 ? __bfloat162float(q[ej[i]]) + a.norm.weight_offset : 1.0f;
+    wk[0][i] = k && ei[i] >= 0 ? __bfloat162float(k[ei[i]]) + a.norm.weight_offset : 1.0f;
+    wk[1][i] = k && ej[i] >= 0 ? __bfloat162float(k[ej[i]]) + a.norm.weight_offset : 1.0f;
+  }
+
+  const int HQ = a.num_heads, KV = a.c.num_kv_heads, rows = HQ + 2 * KV;
+  const int r0 = chunk * a.chunk_rows, r1 = min(rows, r0 + a.chunk_rows);
+  const float inv_d = 1.0f / (float)D;
+#pragma unroll 2
+  for (int rr = r0; rr < r1; rr += RPW) {
+    const int r = rr + sub;
+    const bool isq = r < HQ, isk = !isq && r < HQ + KV;
+    const int h = isq ? r : isk ? r - HQ : r - HQ - KV;
+    const bool on = r < r1 && active && (isq || cached);
+    float x[4] = {0, 0, 0, 0}, y[4] = {0, 0, 0, 0};
+    if (on) {
+      const nvfp4_head_rows &in = isq ? a.q : isk ? a.k : a.v;
+      load_pairs<T, VEC>(static_cast<const T *>(in.data) + t * in.token_stride + h * in.head_stride, ei,
+                         ej, inter, x, y);
+    }
+    const bool normed = isq ? a.norm.q_weight != nullptr : isk && a.norm.k_weight != nullptr;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s = fmaf(x[i], x[i], fmaf(y[i], y[i], s));
+#pragma unroll
+    for (int o = LPR / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (normed) {
+      const float inv = rsqrtf(s * inv_d + a.norm.eps);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] *= inv * (isq ? wq[0][i] : wk[0][i]);
+        y[i] *= inv * (isq ? wq[1][i] : wk[1][i]);
+      }
+    }
+    if (isq || isk) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float u = x[i] * cs[i] - y[i] * sn[i], w = y[i] * cs[i] + x[i] * sn[i];
+        x[i] = u, y[i] = w;
+      }
+    }
+    if (on) {
+      __nv_bfloat16 *dst;
+      if (isq)
+        dst = static_cast<__nv_bfloat16 *>(a.qo.data) + t * a.qo.token_stride + h * a.qo.head_stride;
+      else if (isk)
+        dst = static_cast<__nv_bfloat16 *>(a.c.k) + page * a.c.k_strides[0] + slot * a.c.k_strides[1] +
+              h * a.c.k_strides[2];
+      else
+        dst = static_cast<__nv_bfloat16 *>(a.c.v) + page * a.c.v_strides[0] + slot * a.c.v_strides[1] +
+              h * a.c.v_strides[2];
+      store_pairs<VEC>(dst, ei, ej, inter, x, y);
+    }
+  }
+}
+
+template <typename T, int LPR>
+cudaError_t launch_append(AppendArgs &a, bool vec, cudaStream_t st) {
+  constexpr int RPW = 32 / LPR;
+  const int rows = a.num_heads + 2 * a.c.num_kv_heads;
+  // A warp takes a whole token where there are tokens enough for 16 warps on
+  // every SM; fewer tokens are split over up to one warp per step of rows.
+  const int64_t want = 148 * 16;
+  int64_t chunks = a.b.num_tokens >= want ? 1 : (want + a.b.num_tokens - 1) / a.b.num_tokens;
+  const int steps = (rows + RPW - 1) / RPW;
+  if (chunks > steps) chunks = steps;
+  a.chunk_rows = (int)((steps + chunks - 1) / chunks) * RPW;
+  a.chunks = (rows + a.chunk_rows - 1) / a.chunk_rows;
+  const int64_t warps = a.b.num_tokens * a.chunks;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((warps + kAppendWarps - 1) / kAppendWarps), 1, 1);
+  cfg.blockDim = dim3(kAppendWarps * 32, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return vec ? cudaLaunchKernelEx(&cfg, kv_append_kernel<T, LPR, true>, a)
+             : cudaLaunchKernelEx(&cfg, kv_append_kernel<T, LPR, false>, a);
+}
+
+}  // namespace
+}  // namespace nvfp4
+
+using namespace nvfp4;
+
+extern "C" int nvfp4_kv_append(const nvfp4_kv_cache *cache, const nvfp4_attention_batch *batch,
+                               const nvfp4_rotary *rotary, const nvfp4_qk_norm *norm,
+                               const nvfp4_head_rows *q, const nvfp4_head_rows *k,
+                               const nvfp4_head_rows *v, int in_dtype, int32_t num_heads,
+                               const int32_t *positions, int64_t position_stride, int32_t num_axes,
+                               const nvfp4_head_rows *q_out, void *stream) {
+  NVFP4_ABI_RANGE();
+  int rc = check_kv_cache(cache);
+  if (rc) return rc;
+  if ((rc = check_attention_batch(batch, cache->page_size))) return rc;
+  if (in_dtype != NVFP4_DTYPE_F32 && in_dtype != NVFP4_DTYPE_BF16)
+    return fail(NVFP4_ERR_INVALID_ARG, "bad dtype");
+  if (num_heads <= 0 || num_heads > 65535) return fail(NVFP4_ERR_INVALID_ARG, "bad num_heads %d", num_heads);
+  if (!q || !k || !v || !q_out) return fail(NVFP4_ERR_INVALID_ARG, "null row descriptor");
+  const int R = rotary ? rotary->rotary_dim : 0;
+  if (rotary && (R <= 0 || R % 2 || R > cache->head_dim || !rotary->inv_freq))
+    return fail(NVFP4_ERR_INVALID_ARG, "rotary_dim %d: even, 2 .. head_dim, with inv_freq", R);
+  if (positions && (num_axes < 1 || (num_axes > 1 && position_stride < batch->num_tokens)))
+    return fail(NVFP4_ERR_INVALID_ARG, "positions need num_axes >= 1 rows of num_tokens");
+  if (norm && !(norm->eps >= 0.0f)) return fail(NVFP4_ERR_INVALID_ARG, "eps must not be negative");
+  if (batch->num_tokens == 0 || batch->num_seqs == 0) return NVFP4_OK;
+  if (!q->data || !k->data || !v->data || !q_out->data) return fail(NVFP4_ERR_INVALID_ARG, "null row pointer");
+  const int esize = in_dtype == NVFP4_DTYPE_BF16 ? 2 : 4;
+  auto overlaps = [](const nvfp4_head_rows *a, const nvfp4_head_rows *b) { return a->data == b->data; };
+  if (overlaps(q, q_out) && (esize != 2 || q->token_stride != q_out->token_stride ||
+                             q->head_stride != q_out->head_stride))
+    return fail(NVFP4_ERR_INVALID_ARG, "q_out is q with another dtype or stride");
+  AppendArgs a = {};
+  a.c = *cache;
+  a.b = *batch;
+  if (rotary) a.rot = *rotary;
+  if (norm) a.norm = *norm;
+  a.q = *q;
+  a.k = *k;
+  a.v = *v;
+  a.qo = *q_out;
+  a.pos = positions;
+  a.pos_stride = position_stride;
+  a.num_axes = positions ? num_axes : 1;
+  a.num_heads = num_heads;
+  for (a.page_shift = 4; (1 << a.page_shift) < cache->page_size;) ++a.page_shift;
+  // Runs of 4 pairs as 8- or 16-byte accesses: the halves of the turned and
+  // of the plain part must hold whole runs, on aligned rows.
+  const int D = cache->head_dim;
+  auto fits = [&](const nvfp4_head_rows *r, int es) {
+    return aligned(r->data, 16) && (r->token_stride * es) % 16 == 0 && (r->head_stride * es) % 16 == 0;
+  };
+  const bool vec = fits(q, esize) && fits(k, esize) && fits(v, esize) && fits(q_out, 2) &&
+                   (a.rot.interleaved || (R % 8 == 0 && (D - R) % 8 == 0));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (in_dtype == NVFP4_DTYPE_BF16)
+    e = D <= 64 ? launch_append<__nv_bfloat16, 8>(a, vec, st)
+        : D <= 128 ? launch_append<__nv_bfloat16, 16>(a, vec, st)
+                   : launch_append<__nv_bfloat16, 32>(a, vec, st);
+  else
+    e = D <= 64 ? launch_append<float, 8>(a, vec, st)
+        : D <= 128 ? launch_append<float, 16>(a, vec, st)
+                   : launch_append<float, 32>(a, vec, st);
+  return check_launch(e, "cache append launch");
+}

@@ -4,6 +4,15 @@ Python mirror of the reference package's public names (nvfp4/__init__.mojo:
 1-59) over libnvfp4.so (include/nvfp4.h).  Compute entry points run CUDA
 kernels for sm_100a; there is no CPU fallback.
 """
+from .attention import (
+    AttentionBatch,
+    AttentionConfig,
+    PagedKVCache,
+    Rotary,
+    attention_workspace,
+    kv_append,
+    paged_attention,
+)
 from .config import (
     FP4_E2M1_LUT,
     NVFP4_GROUP_SIZE,
@@ -17,6 +26,7 @@ from .config import (
     unpack_fp4_pair,
 )
 from .deltanet import nvfp4_matvec, sigmoid, silu
+from .norm import norm_residual
 from .nvfp4_gemm_gpu import (
     BK,
     BM,
@@ -53,5 +63,6 @@ __all__ = [
     "nvfp4_linear", "nvfp4_linear_forward", "nvfp4_linear_w4a4", "quantize_act", "LIB_PATH",
     "Nvfp4Error", "LoadedWeight", "SafetensorsFile", "TensorInfo", "discover_safetensor_shards",
     "load_linear_safetensors", "load_moe_experts", "load_qwen35_layer", "open_model_shards",
-    "open_safetensors",
+    "open_safetensors", "AttentionBatch", "AttentionConfig", "PagedKVCache", "Rotary",
+    "attention_workspace", "kv_append", "paged_attention", "norm_residual",
 ]

@@ -146,6 +146,73 @@ class EpPeers(ctypes.Structure):
                 ("timeout_ms", ctypes.c_int32), ("windows", ctypes.c_void_p * EP_MAX_WORLD)]
 
 
+class HeadRows(ctypes.Structure):
+    """struct nvfp4_head_rows (include/nvfp4_attention.h)."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64)]
+
+
+class KvCache(ctypes.Structure):
+    """struct nvfp4_kv_cache."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_strides", ctypes.c_int64 * 3),
+                ("v_strides", ctypes.c_int64 * 3), ("num_pages", ctypes.c_int64),
+                ("page_size", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32)]
+
+
+class AttnBatch(ctypes.Structure):
+    """struct nvfp4_attention_batch."""
+
+    _fields_ = [("num_seqs", ctypes.c_int32), ("max_q_len", ctypes.c_int32),
+                ("num_tokens", ctypes.c_int64), ("q_start", ctypes.c_void_p),
+                ("kv_len", ctypes.c_void_p), ("page_table", ctypes.c_void_p),
+                ("page_table_stride", ctypes.c_int64), ("max_pages", ctypes.c_int32),
+                ("prefix_len", ctypes.c_int32), ("prefix_pages", ctypes.c_void_p),
+                ("visible_len", ctypes.c_void_p)]
+
+
+class RotaryDesc(ctypes.Structure):
+    """struct nvfp4_rotary."""
+
+    _fields_ = [("inv_freq", ctypes.c_void_p), ("axis", ctypes.c_void_p),
+                ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("scale", ctypes.c_float)]
+
+
+class QkNorm(ctypes.Structure):
+    """struct nvfp4_qk_norm."""
+
+    _fields_ = [("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p),
+                ("eps", ctypes.c_float), ("weight_offset", ctypes.c_float)]
+
+
+class AttnDesc(ctypes.Structure):
+    """struct nvfp4_attention_desc."""
+
+    _fields_ = [("num_heads", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("causal", ctypes.c_int32),
+                ("window", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("softcap", ctypes.c_float)]
+
+
+class NormDesc(ctypes.Structure):
+    """struct nvfp4_norm_desc (include/nvfp4_norm.h)."""
+
+    _fields_ = [("rows", ctypes.c_int64), ("hidden", ctypes.c_int32), ("x_dtype", ctypes.c_int32),
+                ("residual_dtype", ctypes.c_int32), ("y_dtype", ctypes.c_int32),
+                ("gate_act", ctypes.c_int32), ("residual_scale", ctypes.c_float),
+                ("eps", ctypes.c_float), ("weight_offset", ctypes.c_float),
+                ("x_stride", ctypes.c_int64), ("residual_stride", ctypes.c_int64),
+                ("residual_out_stride", ctypes.c_int64), ("y_stride", ctypes.c_int64),
+                ("gate_row_stride", ctypes.c_int64), ("gate_col_stride", ctypes.c_int64)]
+
+
+GATE_LINEAR = 0
+GATE_SIGMOID = 1
+
+
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
@@ -212,6 +279,21 @@ SIGNATURES = {
                                       ctypes.POINTER(DeltaNetWeightPtrs), _vp, _int, _vp, _int,
                                       _i64, ctypes.POINTER(DeltaNetStatePtrs), _int, _vp,
                                       ctypes.c_size_t, _vp]),
+    # include/nvfp4_attention.h
+    "nvfp4_kv_append": (_int, [ctypes.POINTER(KvCache), ctypes.POINTER(AttnBatch),
+                               ctypes.POINTER(RotaryDesc), ctypes.POINTER(QkNorm),
+                               ctypes.POINTER(HeadRows), ctypes.POINTER(HeadRows),
+                               ctypes.POINTER(HeadRows), _int, ctypes.c_int32, _vp, _i64,
+                               ctypes.c_int32, ctypes.POINTER(HeadRows), _vp]),
+    "nvfp4_attention_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(AttnDesc),
+                                                         ctypes.POINTER(AttnBatch)]),
+    "nvfp4_paged_attention": (_int, [ctypes.POINTER(AttnDesc), ctypes.POINTER(HeadRows),
+                                     ctypes.POINTER(KvCache), ctypes.POINTER(AttnBatch), _vp,
+                                     ctypes.POINTER(HeadRows), ctypes.POINTER(HeadRows), _vp, _vp,
+                                     ctypes.c_size_t, _vp]),
+    # include/nvfp4_norm.h
+    "nvfp4_norm_residual": (_int, [ctypes.POINTER(NormDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                   _vp]),
     # include/nvfp4_loader.h
     "nvfp4_st_open": (_int, [ctypes.c_char_p, ctypes.POINTER(_vp)]),
     "nvfp4_st_close": (None, [_vp]),
