@@ -232,7 +232,7 @@ def prepare(case, seed):
             s["visible"] = torch.minimum(s["kv_len"], torch.tensor(c["visible"], dtype=torch.int32, device="cuda")) if c["visible"] else None
     s["c"] = c
     if own:  # the handles and workspace that a serving loop keeps over its layers
-        A, _ = _package()
+        A, N = s["package"] = _package()
         if c["kind"] != "norm":
             s["cache"] = A.PagedKVCache(s["k"], s["v"])
             s["batch"] = A.AttentionBatch(
@@ -251,7 +251,7 @@ def prepare(case, seed):
 
 
 def _run_own(s):
-    A, N = _package()
+    A, N = s["package"]
     c = s["c"]
     if c["kind"] == "norm":
         r, y = N.norm_residual(s["x"], s["residual"], pre_weight=s["pre"], post_weight=s["post_w"],
