@@ -115,7 +115,7 @@ int nvfp4_kv_append(const nvfp4_kv_cache *cache, const nvfp4_attention_batch *ba
 
 /*
  * Attention of query position p over key positions j in [lo, hi):
- *   s = scale * q.k;  softcap > 0: s = softcap * tanh(s / softcap);
+ *   s = scale * q.k (scale > 0);  softcap > 0: s = softcap * tanh(s / softcap);
  *   slopes: s -= slopes[head] * |p - j|;
  *   hi = causal ? max(p + 1, visible_len) : all;  lo = window ? p - window + 1 : 0.
  * Query head h reads key/value head h / (num_heads / num_kv_heads); at most

@@ -61,14 +61,20 @@ int check_desc(const nvfp4_attention_desc *d) {
     return fail(NVFP4_ERR_UNSUPPORTED, "more than 128 query heads per key/value head");
   if (d->head_dim <= 0 || d->head_dim > 256 || d->head_dim % 8)
     return fail(NVFP4_ERR_UNSUPPORTED, "head_dim %d: multiples of 8 up to 256", d->head_dim);
-  if (!std::isfinite(d->scale) || !std::isfinite(d->softcap) || d->softcap < 0.0f)
-    return fail(NVFP4_ERR_INVALID_ARG, "scale must be finite, softcap finite and not negative");
+  if (!std::isfinite(d->scale) || !(d->scale > 0.0f) || !std::isfinite(d->softcap) || d->softcap < 0.0f)
+    return fail(NVFP4_ERR_INVALID_ARG, "scale must be positive, softcap not negative, both finite");
   if (d->window < 0) return fail(NVFP4_ERR_INVALID_ARG, "window must not be negative");
   return NVFP4_OK;
 }
 
-// Query rows of an item: 16 or 32.
-int rows_of(const nvfp4_attention_desc &d, int64_t rows) { return rows <= 16 || d.head_dim > 128 ? 16 : 32; }
+// Query rows of an item, which also names the kernel: 16 or 32 rows on
+// attention_rows.cu while a sequence's rows per key/value head fit one item
+// (keys are read once), else attention_tc.cu.
+int rows_of(const nvfp4_attention_desc &d, int64_t rows) {
+  if (rows <= 16) return 16;
+  if (d.head_dim > 128) return 128;
+  return rows <= 32 ? 32 : 256;
+}
 
 struct AttnLayout {
   size_t part_o, part_ml, meta, prev_o, prev_lse, total;
@@ -150,12 +156,6 @@ extern "C" int nvfp4_paged_attention(const nvfp4_attention_desc *desc, const nvf
   if (ws_bytes < L.total)
     return fail(NVFP4_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", ws_bytes, L.total);
 
-  CUtensorMap tk, tv;
-  const int box = cache->page_size < 64 ? cache->page_size : 64;
-  if (!make_cache_map(&tk, cache->k, cache->k_strides, *cache, box) ||
-      !make_cache_map(&tv, cache->v, cache->v_strides, *cache, box))
-    return fail(NVFP4_ERR_CUDA, "tensor map of the cache");
-
   AttnArgs a = {};
   a.B = batch->num_seqs;
   a.T = (int)batch->num_tokens;
@@ -192,6 +192,16 @@ extern "C" int nvfp4_paged_attention(const nvfp4_attention_desc *desc, const nvf
   a.part_ml = reinterpret_cast<float2 *>(w + L.part_ml);
   a.meta = reinterpret_cast<int4 *>(w + L.meta);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto pass = [&](int R, const char *what) -> int {
+    // A box of the cache map: a page, or as much of it as a key tile takes.
+    const int tile = R == 256 ? 128 : 64, box = cache->page_size < tile ? cache->page_size : tile;
+    CUtensorMap tk, tv;
+    if (!make_cache_map(&tk, cache->k, cache->k_strides, *cache, box) ||
+        !make_cache_map(&tv, cache->v, cache->v_strides, *cache, box))
+      return fail(NVFP4_ERR_CUDA, "tensor map of the cache");
+    return check_launch(R <= 32 ? launch_attn_rows(tk, tv, a, R, grid, st) : launch_attn_tc(tk, tv, a, grid, st),
+                        what);
+  };
   if (batch->prefix_len > 0) {
     // All tokens against the shared prefix first: its keys are read once for
     // the whole batch; the own pass joins the result in its last step.
@@ -200,11 +210,10 @@ extern "C" int nvfp4_paged_attention(const nvfp4_attention_desc *desc, const nvf
     a.prefix_pass = 1;
     a.page_table = batch->prefix_pages;
     a.max_blocks = (int)(((int64_t)a.T * a.G + L.R0 - 1) / L.R0);
-    rc = check_launch(launch_attn_rows(tk, tv, a, L.R0, grid, st), "attention launch (prefix)");
-    if (rc) return rc;
+    if ((rc = pass(L.R0, "attention launch (prefix)"))) return rc;
     a.prefix_pass = 0;
     a.page_table = batch->page_table;
   }
   a.max_blocks = (int)(((int64_t)batch->max_q_len * a.G + L.R1 - 1) / L.R1);
-  return check_launch(launch_attn_rows(tk, tv, a, L.R1, grid, st), "attention launch");
+  return pass(L.R1, "attention launch");
 }

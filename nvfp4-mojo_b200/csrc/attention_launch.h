@@ -10,4 +10,8 @@ namespace nvfp4 {
 cudaError_t launch_attn_rows(const CUtensorMap &tk, const CUtensorMap &tv, const AttnArgs &a, int R,
                              int grid, cudaStream_t st);
 
+// attention_tc.cu: items of 256 rows (128 above head size 128).
+cudaError_t launch_attn_tc(const CUtensorMap &tk, const CUtensorMap &tv, const AttnArgs &a, int grid,
+                           cudaStream_t st);
+
 }  // namespace nvfp4

@@ -1,0 +1,549 @@
+// attention_tc.cu -- attention of many query rows per key/value head (prompts,
+// a shared prefix) over the paged cache, on the 5th-generation tensor cores.
+//
+// An item is QT tiles of 128 query rows (attention.cuh: the heads of a group
+// share their keys, so 8 heads make a tile of 16 tokens).  Per key tile j and
+// query tile t: S = Q K_j^T into TMEM, a softmax thread per row, P as bf16
+// back into TMEM over S, O += P V_j with P as the TMEM operand and V in its
+// natural token-major layout (MN-major operand).  O stays in TMEM for all of
+// an item.  Up to head size 128 QT = 2 and the two tiles alternate: while one
+// is in its softmax the other has the tensor cores.  Above, O takes half of
+// TMEM: QT = 1 and two S buffers, the next S running under the softmax.
+//   warps 0-3 (and 4-7, QT = 2)  softmax of tile 0 (1), Q into shared memory,
+//                                the rare rescaling of O, the epilogue;
+//   then one warp each           MMA issue (one thread), TMA producer, and the
+//                                zeroing of values that no row sees.
+// O is rescaled only when a row's maximum has grown by more than 2^8 since
+// the last time (weights then stay below 2^8, exact in the sums' fp32); the
+// reference is the same for sum and product, so the result is not changed.
+// Bound by the tensor cores and, nearly as much, by the exponentials: 2 x 128
+// x 128 of them per 2048 tensor cycles are 2048 cycles of the MUFU.
+#include <cuda_bf16.h>
+
+#include "../../include/nvfp4.h"
+#include "abi_util.h"
+#include "attention.cuh"
+#include "attention_launch.h"
+#include "kernels.h"
+#include "tc_common.cuh"
+
+namespace nvfp4 {
+
+static __device__ int g_attn_tc_status;
+
+namespace {
+
+template <int DP>
+struct TcCfg {
+  static constexpr int QT = DP <= 128 ? 2 : 1;
+  static constexpr int R = 128 * QT;
+  static constexpr int KT = DP <= 128 ? 128 : 64;   // keys per tile
+  static constexpr int kTile = KT * DP * 2;         // bytes of a key or value tile
+  static constexpr int kQ = 128 * DP * 2;           // bytes of a query tile
+  static constexpr int kSlots = DP == 64 ? 8 : 4;
+  static constexpr int kSoftWarps = 4 * QT;
+  static constexpr int kThreads = (kSoftWarps + 4) * 32;
+  static constexpr int offKV = QT * kQ;
+  static constexpr int bytes = offKV + kSlots * kTile + 1024;
+  // TMEM columns: S tiles (tile t, or buffer t when QT = 1), then O.
+  static constexpr int colO = 2 * KT;
+  static constexpr int cols = 512;
+};
+
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D[tmem] (+)= A[tmem] * B[smem].
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Values [token][d], 64 columns of 128 swizzled bytes per token, as the
+// MN-major B operand: 64-column blocks `block` bytes apart (leading offset),
+// groups of 8 tokens 1024 bytes apart (stride offset).
+__device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t saddr, uint32_t block) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(block >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+constexpr uint32_t kTransposeB = 1u << 16;
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int h, int row,
+                                            int page, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(h), "r"(row), "r"(page), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+template <int DP, bool MOD>
+__global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
+    attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                   const __grid_constant__ AttnArgs a) {
+  using C = TcCfg<DP>;
+  constexpr int QT = C::QT, R = C::R, KT = C::KT, kSlots = C::kSlots;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                              ~static_cast<uintptr_t>(1023));
+  __shared__ AttnPlanSmem plan;
+  __shared__ uint64_t bars[3 * kSlots + 9];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t full = smem_u32(bars);
+  const uint32_t empty = full + 8 * kSlots;   // the slot's MMAs are done
+  const uint32_t edge = empty + 8 * kSlots;   // a value tile landed that needs zeroing
+  const uint32_t bar_q = edge + 8 * kSlots;   // [2] queries of tile t in shared memory
+  const uint32_t bar_s = bar_q + 16;          // [2] S ready
+  const uint32_t bar_p = bar_s + 16;          // [2] P written (and O rescaled)
+  const uint32_t bar_o = bar_p + 16;          // [2] P V done (tile t; QT = 1: even and odd products)
+  const uint32_t bar_end = bar_o + 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 1);
+      mbar_init(edge + 8 * i, 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(bar_q + 8 * t, 4);
+      mbar_init(bar_s + 8 * t, 1);
+      mbar_init(bar_p + 8 * t, 4);
+      mbar_init(bar_o + 8 * t, 1);
+    }
+    mbar_init(bar_end, 1);
+    mbar_fence_init();
+    prefetch_tmap(&tmK);
+    prefetch_tmap(&tmV);
+  }
+  // TMEM is taken after the launches before have ended and before a launch
+  // behind this one may start: neither can hold what this block waits for.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (warp == C::kSoftWarps) {
+    tmem_alloc(smem_u32(&tmem_slot), C::cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  AttnCursor cur = attn_plan<R, KT>(a, 2, &plan);  // ends with __syncthreads
+  tc_fence_after();
+  asm volatile("griddepcontrol.launch_dependents;");
+  const uint32_t tmem = tmem_slot;
+  if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, -1);
+  volatile int *abort = &abort_flag;
+  int *status = &g_attn_tc_status;
+  AttnSegment g;
+  // Tiles of an item in use: the second one only with rows beyond 128.
+  auto tiles = [&](const AttnSegment &x) { return QT == 2 && x.s.ql * a.G - x.rb * R > 128 ? 2 : 1; };
+
+  if (warp < C::kSoftWarps) {
+    if constexpr (QT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int t = warp >> 2, wq = warp & 3;            // tile, lane quarter
+    const int my = t * 128 + wq * 32 + lane;           // row within the item
+    const uint32_t lanes = static_cast<uint32_t>(32 * wq) << 16;
+    const uint32_t tO = tmem + lanes + C::colO + (QT == 2 ? t * DP : 0);
+    uint8_t *Q = smem + t * C::kQ;
+    const float sl2 = a.scale * kLog2e;
+
+    // This warp's 32 rows of Q, 16-byte chunks swizzled as the MMA reads them;
+    // rows and columns beyond the item's or the head's are zeros.
+    auto load_q = [&](const AttnSegment &x) {
+      const int row = x.rb * R + my;
+      const __nv_bfloat16 *src = nullptr;
+      if (row < x.s.ql * a.G) {
+        const int i = row / a.G;
+        src = a.q + (int64_t)(x.s.tok0 + i) * a.q_ts + (int64_t)(x.h * a.G + row - i * a.G) * a.q_hs;
+      }
+      constexpr int CH = DP / 8, RPI = 32 / CH;  // chunks per row, rows per warp step
+      const int c = lane % CH;
+#pragma unroll 8
+      for (int r0 = 0; r0 < 32; r0 += RPI) {
+        const int r = r0 + lane / CH;
+        const uint64_t p = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(src), r);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (p && 8 * c < a.D) v = *(reinterpret_cast<const uint4 *>(p) + c);
+        const int rr = wq * 32 + r;
+        *reinterpret_cast<uint4 *>(Q + (c >> 3) * (128 * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_q + 8 * t);
+    };
+
+    // Product i of this query tile is in.  With QT = 1 the S that is ready
+    // may be ahead of the last two products, so these alternate between two
+    // barriers: each then has at most one phase outstanding.
+    auto o_wait = [&](uint32_t i) {
+      return QT == 2 ? mbar_wait(bar_o + 8 * t, i & 1, status, kDevTimeoutAcc, abort)
+                     : mbar_wait(bar_o + 8 * (i & 1), (i >> 1) & 1, status, kDevTimeoutAcc, abort);
+    };
+    uint32_t n = 0;  // key tiles of this query tile so far
+    bool have = attn_segment<R, KT>(a, cur, g), ok = true;
+    if (have && g.take > 0 && t < tiles(g)) load_q(g);
+    while (have && ok) {
+      const bool mine = t < tiles(g);
+      const int row = g.rb * R + my;
+      const bool in = row < g.s.ql * a.G;
+      AttnRow ar = {};
+      float m = -INFINITY, l = 0.0f;
+      if (mine) {
+        ar = attn_row(a, g.s, g.h, in ? row : 0);
+        if (!in) ar.lo = ar.hi = 0;
+        const float slope = MOD && a.slopes ? a.slopes[ar.head] * kLog2e : 0.0f;
+        const int pos = ar.pos - (a.prefix_pass ? 0 : a.prefix_len);
+        for (int u = 0; u < g.take; ++u, ++n) {
+          const int j0 = (g.it.u0 + g.off + u) * KT;
+          const int b = QT == 2 ? t : (n & 1);
+          const uint32_t ph = QT == 2 ? n & 1 : (n >> 1) & 1;
+          const uint32_t tS = tmem + lanes + b * KT;
+          if (!__all_sync(0xffffffffu, mbar_wait(bar_s + 8 * b, ph, status, kDevTimeoutAcc, abort))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          uint32_t raw[KT / 32][32];
+#pragma unroll
+          for (int c = 0; c < KT / 32; ++c) tmem_ld_32x32b_x32(tS + 32 * c, raw[c]);
+          tmem_ld_wait();
+          float s[KT];
+#pragma unroll
+          for (int c = 0; c < KT; ++c) s[c] = __uint_as_float(raw[c / 32][c % 32]);
+          if constexpr (MOD) {
+#pragma unroll
+            for (int c = 0; c < KT; ++c) {
+              float v = s[c] * a.scale;
+              if (a.softcap > 0.0f)  // cap tanh(v / cap)
+                v = a.softcap - __fdividef(2.0f * a.softcap, 1.0f + ex2(v * (2.0f * kLog2e / a.softcap)));
+              s[c] = fmaf(v, kLog2e, -slope * fabsf((float)(pos - j0 - c)));
+            }
+          }
+          const float c2 = MOD ? 1.0f : sl2;
+          if (__any_sync(0xffffffffu, j0 < ar.lo || j0 + KT > ar.hi)) {
+            const int lo = ar.lo - j0, hi = ar.hi - j0;
+#pragma unroll
+            for (int c = 0; c < KT; ++c) s[c] = c >= lo && c < hi ? s[c] : -INFINITY;
+          }
+          float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int c = 4; c < KT; c += 4)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], s[c + i]);
+          const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c2;
+          const bool grow = mx > m + 8.0f;
+          if (__any_sync(0xffffffffu, grow)) {
+            const float mn = grow ? mx : m;
+            if (u > 0) {  // O of the tiles before, once they are all in
+              if (!__all_sync(0xffffffffu, o_wait(n - 1))) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              const float f = grow ? ex2(m - mn) : 1.0f;
+              l *= f;
+#pragma unroll 1
+              for (int c = 0; c < DP; c += 32) {
+                uint32_t o[32];
+                tmem_ld_32x32b_x32(tO + c, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_st_x32(tO + c, o);
+              }
+            }
+            m = mn;
+          }
+          const float mu = m == -INFINITY ? 0.0f : m;
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int c = 0; c < KT; c += 64) {
+            uint32_t p[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float x = ex2(fmaf(s[c + 2 * i], c2, -mu)), y = ex2(fmaf(s[c + 2 * i + 1], c2, -mu));
+              sum[(2 * i) & 3] += x;
+              sum[(2 * i + 1) & 3] += y;
+              // Rounded to bf16 for the second product only; the sum keeps
+              // the unrounded weights.
+              p[i] = pack_bf16(x, y);
+            }
+            tmem_st_x32(tS + c / 2, p);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_p + 8 * b);
+        }
+      }
+      if (!ok) break;
+      // The next item's queries first (this item's S are all done), so that
+      // its first S runs under this epilogue.
+      const AttnSegment e = g;
+      have = attn_segment<R, KT>(a, cur, g);
+      if (have && g.take > 0 && t < tiles(g)) load_q(g);
+      if (!mine) continue;
+      if (e.take > 0) {
+        if (!__all_sync(0xffffffffu, o_wait(n - 1))) break;
+        tc_fence_after();
+      }
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t o[32];
+        if (e.take > 0) {
+          tmem_ld_32x32b_x32(tO + c, o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
+        }
+        if (!in) continue;
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 v = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]),
+                                       __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+          if (e.whole)
+            attn_finish4(a, ar, c + i, DP, v, m, l);
+          else
+            *reinterpret_cast<float4 *>(a.part_o + ((int64_t)e.slot * R + my) * DP + c + i) = v;
+        }
+      }
+      if (in && !e.whole) a.part_ml[(int64_t)e.slot * R + my] = make_float2(m, l);
+      if (e.leads && threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(e.b, e.h, e.rb, e.last_part);
+      tc_fence_before();
+    }
+  } else {
+    if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    const int role = warp - C::kSoftWarps;
+    if (role == 0) {
+      // ---------------- MMA issue ----------------
+      if (lane == 0) {
+        constexpr uint32_t idS = idesc_bf16_f32(128, KT);
+        constexpr uint32_t idO = idesc_bf16_f32(128, DP) | kTransposeB;
+        bool ok = true;
+        uint32_t tile = 0;             // key tiles so far: K in slot 2 tile, V in 2 tile + 1
+        uint32_t ns[2] = {0, 0};       // S issued per query tile
+        uint32_t nq[2] = {0, 0};       // queries awaited per query tile
+        bool pend = false, pfirst = false;
+        int pnt = 0;                   // the pending P V: query tiles, first of its item
+        auto wait = [&](uint32_t bar, uint32_t ph, int code) {
+          ok = ok && mbar_wait(bar, ph, status, code, abort);
+          return ok;
+        };
+        auto full_wait = [&](uint32_t pos) {
+          return wait(full + 8 * (pos % kSlots), (pos / kSlots) & 1, kDevTimeoutFull);
+        };
+        auto do_s = [&](int t, bool first) {
+          if (first && !wait(bar_q + 8 * t, nq[t]++ & 1, kDevTimeoutDec)) return;
+          tc_fence_after();
+          const int b = QT == 2 ? t : (ns[0] & 1);
+          const uint32_t k0 = sbase + C::offKV + ((2 * tile) % kSlots) * C::kTile;
+          const uint32_t q0 = sbase + t * C::kQ;
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k)
+            tc_mma_f16(tmem + b * KT, sw128_kmajor_desc(q0 + (k >> 2) * (128 * 128) + 32 * (k & 3)),
+                       sw128_kmajor_desc(k0 + (k >> 2) * (KT * 128) + 32 * (k & 3)), idS, k != 0);
+          tc_commit(bar_s + 8 * b);
+          ++ns[t];
+        };
+        auto do_pv = [&](int t, uint32_t vtile) {
+          // P of the tile before the S issued last (QT = 1: one S is ahead).
+          const uint32_t np = QT == 2 ? ns[t] - 1 : vtile;
+          const int b = QT == 2 ? t : (np & 1);
+          if (!wait(bar_p + 8 * b, (QT == 2 ? np : np >> 1) & 1, kDevTimeoutDec)) return;
+          tc_fence_after();
+          const uint32_t v0 = sbase + C::offKV + ((2 * vtile + 1) % kSlots) * C::kTile;
+          const uint32_t d = tmem + C::colO + (QT == 2 ? t * DP : 0);
+#pragma unroll
+          for (int k = 0; k < KT / 16; ++k)
+            tc_mma_f16_ts(d, tmem + b * KT + 8 * k, sw128_mnmajor_desc(v0 + k * 2048, KT * 128), idO,
+                          !(pfirst && k == 0));
+          tc_commit(bar_o + 8 * (QT == 2 ? t : (np & 1)));
+        };
+        auto pv_all = [&](uint32_t vtile) {
+          if (!full_wait(2 * vtile + 1)) return;
+          for (int t = 0; t < pnt && ok; ++t) do_pv(t, vtile);
+          tc_commit(empty + 8 * ((2 * vtile + 1) % kSlots));
+          pend = false;
+        };
+        while (ok && attn_segment<R, KT>(a, cur, g)) {
+          const int nt = tiles(g);
+          for (int u = 0; u < g.take && ok; ++u, ++tile) {
+            if (u == 0 && pend) pv_all(tile - 1);  // the item before is finished first
+            if (!ok || !full_wait(2 * tile)) break;
+            if (QT == 2 && pend) {
+              if (!full_wait(2 * tile - 1)) break;
+              for (int t = 0; t < nt && ok; ++t) {
+                do_pv(t, tile - 1);
+                if (ok) do_s(t, false);
+              }
+              tc_commit(empty + 8 * ((2 * tile - 1) % kSlots));
+            } else {
+              for (int t = 0; t < nt && ok; ++t) do_s(t, u == 0);
+            }
+            tc_commit(empty + 8 * ((2 * tile) % kSlots));
+            if (QT == 1 && pend && ok) pv_all(tile - 1);
+            pend = ok;
+            pfirst = u == 0;
+            pnt = nt;
+          }
+        }
+        if (ok && pend) pv_all(tile - 1);
+        // TMEM is given back only when every MMA has finished.
+        tc_commit(bar_end);
+        volatile int no_abort = 0;
+        mbar_wait(bar_end, 0, status, kDevTimeoutAcc, &no_abort);
+      }
+      __syncwarp();
+    } else if (role == 1) {
+      // ---------------- TMA producer ----------------
+      const int box = a.page_size < KT ? a.page_size : KT;
+      const int per = KT / box;
+      constexpr int halves = DP / 64;
+      uint32_t at = 0;
+      bool ok = true;
+      while (ok && attn_segment<R, KT>(a, cur, g)) {
+        const int *pages = a.page_table + (a.prefix_pass ? 0 : (int64_t)g.b * a.pt_stride);
+        int ids = 0, ids_at = -64;
+        for (int u = 0; u < g.take && ok; ++u) {
+          const int j0 = (g.it.u0 + g.off + u) * KT;
+          const int i = lane % per, hf = lane / per;
+          const int tok = j0 + i * box;
+          const bool mine = hf < halves && tok < g.it.hi && tok + box > g.it.lo;
+          const int p0 = j0 >> a.page_shift, p1 = (j0 + KT - 1) >> a.page_shift;
+          if (p1 >= ids_at + 32 || p0 < ids_at) {
+            ids_at = p0;
+            ids = pages[min(p0 + lane, (g.it.hi - 1) >> a.page_shift)];
+          }
+          const int page = __shfl_sync(0xffffffffu, ids, ((tok >> a.page_shift) - ids_at) & 31);
+          const int row = tok & (a.page_size - 1);
+          const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * box * 128;
+          const bool ragged = j0 < g.it.lo || j0 + KT > g.it.hi;
+          for (int kv = 0; kv < 2; ++kv, ++at) {
+            const uint32_t slot = at % kSlots, round = at / kSlots;
+            if (round > 0 && !__all_sync(0xffffffffu, mbar_wait(empty + 8 * slot, (round - 1) & 1, status,
+                                                                kDevTimeoutEmpty, abort))) {
+              ok = false;
+              break;
+            }
+            const uint32_t bar = (kv && ragged ? edge : full) + 8 * slot;
+            if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+            __syncwarp();
+            if (mine)
+              tma_load_4d(sbase + C::offKV + slot * C::kTile + hf * (KT * 128) + i * box * 128,
+                          kv ? &tmV : &tmK, 64 * hf, g.h, row, page, bar);
+          }
+        }
+      }
+      // Drain: the block never exits with a copy still writing its memory.
+      for (uint32_t q = at > kSlots ? at - kSlots : 0; q < at; ++q) {
+        volatile int no_abort = 0;
+        mbar_wait(full + 8 * (q % kSlots), (q / kSlots) & 1, status, kDevTimeoutFull, &no_abort);
+      }
+    } else if (role == 2) {
+      // ---------------- values that no row sees ----------------
+      // Rows of a value tile before the first or from the last key on (never
+      // loaded, or the rest of a page) are zeroed: their weights are zero,
+      // but what lies there may not be finite.
+      uint32_t at = 0, phase = 0;
+      bool ok = true;
+      while (ok && attn_segment<R, KT>(a, cur, g)) {
+        for (int u = 0; u < g.take; ++u, at += 2) {
+          const int j0 = (g.it.u0 + g.off + u) * KT;
+          if (j0 >= g.it.lo && j0 + KT <= g.it.hi) continue;
+          const uint32_t slot = (at + 1) % kSlots;
+          if (!__all_sync(0xffffffffu, mbar_wait(edge + 8 * slot, (phase >> slot) & 1, status,
+                                                 kDevTimeoutFull, abort))) {
+            ok = false;
+            break;
+          }
+          phase ^= 1u << slot;
+          uint8_t *V = smem + C::offKV + slot * C::kTile;
+          for (int x = lane; x < KT * (DP / 8); x += 32) {
+            const int r = x / (DP / 8), c = x % (DP / 8), j = j0 + r;
+            if (j < g.it.lo || j >= g.it.hi)
+              *reinterpret_cast<uint4 *>(V + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+                  make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full + 8 * slot);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == C::kSoftWarps) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::cols);
+  }
+}
+
+template <int DP>
+cudaError_t launch_tc(const CUtensorMap &tk, const CUtensorMap &tv, const AttnArgs &a, int grid,
+                      cudaStream_t st) {
+  using C = TcCfg<DP>;
+  auto k = a.softcap > 0.0f || a.slopes ? attn_tc_kernel<DP, true> : attn_tc_kernel<DP, false>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::bytes);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid, 1, 1);
+  cfg.blockDim = dim3(C::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = C::bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if ((e = cudaLaunchKernelEx(&cfg, k, tk, tv, a)) != cudaSuccess) return e;
+  cfg.gridDim = dim3((unsigned)grid, C::R / 4, 1);
+  cfg.blockDim = dim3(128, 1, 1);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, attn_join_kernel<C::R, C::KT, DP>, a);
+}
+
+}  // namespace
+
+cudaError_t launch_attn_tc(const CUtensorMap &tk, const CUtensorMap &tv, const AttnArgs &a, int grid,
+                           cudaStream_t st) {
+  if (a.D <= 64) return launch_tc<64>(tk, tv, a, grid, st);
+  if (a.D <= 128) return launch_tc<128>(tk, tv, a, grid, st);
+  return launch_tc<256>(tk, tv, a, grid, st);
+}
+
+int read_attn_tc_device_status() {
+  int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_attn_tc_status, sizeof(int)) != cudaSuccess) return -1;
+  if (v) cudaMemcpyToSymbol(g_attn_tc_status, &zero, sizeof(int));
+  return v;
+}
+
+}  // namespace nvfp4

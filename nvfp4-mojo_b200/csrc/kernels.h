@@ -150,6 +150,7 @@ cudaError_t launch_w4a16_tc(const WeightSpec &ws, const AlphaSpec &al, const uin
 // (-1: not readable).
 int read_gemm_device_status();
 int read_attn_rows_device_status();
+int read_attn_tc_device_status();
 int read_gemv_device_status();
 int read_moe_tc_device_status();
 int read_w4a4_device_status();

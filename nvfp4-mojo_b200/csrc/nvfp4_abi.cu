@@ -287,10 +287,10 @@ extern "C" int nvfp4_dequant_tile(const uint8_t *w, const uint8_t *sf, float *ou
 }
 
 extern "C" int nvfp4_device_status(void) {
-  const int words[7] = {read_gemm_device_status(), read_gemv_device_status(),
+  const int words[8] = {read_gemm_device_status(), read_gemv_device_status(),
                         read_moe_tc_device_status(), read_w4a4_device_status(),
                         read_gemv_ts_device_status(), read_gemv_dg_device_status(),
-                        read_attn_rows_device_status()};
+                        read_attn_rows_device_status(), read_attn_tc_device_status()};
   int v = 0;
   for (int w : words) {
     if (w < 0) return fail(NVFP4_ERR_CUDA, "could not read the device status word");

@@ -130,6 +130,19 @@ def test_prompts(H, KV, D, causal):
     run_and_check(make(9, [1, 90, 200, 65], [1, 90, 33, 17], KV, D, H, 32), causal=causal)
 
 
+@pytest.mark.parametrize("H,KV,D", [(8, 1, 128), (8, 1, 256), (2, 2, 64)])
+def test_prompts_over_many_key_tiles(H, KV, D):
+    """Many key tiles per item and several items per block, repeated: the
+    hand-over between the roles of a block, tile after tile."""
+    import nvfp4
+
+    s = make(27, [2900, 700, 1500], [300, 700, 40], KV, D, H, 16)
+    first, _ = run_and_check(s)
+    cfg, b, q = nvfp4.AttentionConfig(H, KV, D), batch_of(s), s["q"].cuda()
+    for _ in range(20):
+        assert torch.equal(nvfp4.paged_attention(q, s["cache"], b, cfg), first)
+
+
 @pytest.mark.parametrize("qlens", [[2, 3, 1], [4, 4, 4], [1, 9, 40], [129, 1, 128], [1, 1, 300]])
 def test_query_lengths(qlens):
     """Around every row count at which another kernel or tile is taken."""
