@@ -162,11 +162,11 @@ __device__ __forceinline__ int attn_blocks(const AttnArgs &a, const AttnSeq &s) 
   return (int)(((int64_t)s.ql * a.G + R - 1) / R);
 }
 
-// An item that sees nothing still takes one unit of the line: its rows are
-// written too.
-template <int R, int KT>
+// An item takes E more units of the line than it has, for what it costs to
+// begin and end it (also where its rows see nothing: they are written too).
+template <int R, int KT, int E>
 __device__ __forceinline__ int attn_item_units(const AttnArgs &a, const AttnSeq &s, int rb) {
-  return max(attn_item<R, KT>(a, s, rb).units, 1);
+  return attn_item<R, KT>(a, s, rb).units + E;
 }
 
 // Where a block starts on the line, and how far it goes.
@@ -185,7 +185,7 @@ struct AttnPlanSmem {
 
 // Plans this block's share; every thread of the block calls it.  parts: at
 // most gridDim.x and one per `min_units` units.
-template <int R, int KT>
+template <int R, int KT, int E>
 __device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units, AttnPlanSmem *sm) {
   const int nt = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = nt >> 5;
   const int NS = attn_num_seqs(a);
@@ -196,7 +196,7 @@ __device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units
     const AttnSeq s = attn_seq(a, b);
     const int nb = attn_blocks<R>(a, s);
     int u = 0;
-    for (int rb = by_warp ? lane : 0; rb < nb; rb += by_warp ? 32 : 1) u += attn_item_units<R, KT>(a, s, rb);
+    for (int rb = by_warp ? lane : 0; rb < nb; rb += by_warp ? 32 : 1) u += attn_item_units<R, KT, E>(a, s, rb);
     return u;
   };
   auto warp_units = [&](int b) -> int {  // every lane gets sequence b's units
@@ -273,7 +273,7 @@ __device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units
       const int nb = attn_blocks<R>(a, s);
       for (int base = 0; base < nb; base += 32) {  // the item within the sequence and head
         const int rb = base + lane;
-        int inc = rb < nb ? attn_item_units<R, KT>(a, s, rb) : 0;
+        int inc = rb < nb ? attn_item_units<R, KT, E>(a, s, rb) : 0;
         const int u = inc;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -310,80 +310,128 @@ __device__ __forceinline__ void attn_next(const AttnArgs &a, AttnCursor &c, int 
   } while (c.b < NS && attn_seq(a, c.b).ql == 0);
 }
 
-// One stretch of a block's share: units [off, off + take) of an item.
+// One stretch of a block's share: key units [off, off + take) of an item.
 struct AttnSegment {
   AttnSeq s;
   AttnItem it;
   int b, h, rb, off, take;
-  bool whole;      // the block has all of the item
-  int slot;        // workspace part otherwise
-  bool leads;      // the item starts here and goes on in later blocks ...
-  int last_part;   // ... up to this one
+  int slot;        // workspace part; -1: the block has all of the item
+  int last_part;   // >= 0: the item starts here and goes on up to this block
 };
 
-template <int R, int KT>
+template <int R, int KT, int E>
 __device__ __forceinline__ bool attn_segment(const AttnArgs &a, AttnCursor &c, AttnSegment &g) {
-  if (c.at >= c.end) return false;
-  g.s = attn_seq(a, c.b);
-  g.it = attn_item<R, KT>(a, g.s, c.rb);
-  g.b = c.b;
-  g.h = c.h;
-  g.rb = c.rb;
-  g.off = c.off;
-  const int n = max(g.it.units, 1);
-  const long long left = c.end - c.at;
-  g.take = (int)(left < (long long)(n - c.off) ? left : (long long)(n - c.off));
-  const bool ends = c.off + g.take == n;
-  g.whole = c.off == 0 && ends;
-  g.leads = c.off == 0 && !ends;
-  g.slot = 2 * blockIdx.x + (g.leads ? 1 : 0);
-  g.last_part = g.leads ? (int)(((c.at + n) * c.parts - 1) / c.total) : 0;
-  c.at += g.take;
-  c.off += g.take;
-  if (ends) attn_next<R>(a, c, attn_blocks<R>(a, g.s));
-  if (g.it.units == 0) g.take = 0;
-  return true;
+  while (c.at < c.end) {
+    g.s = attn_seq(a, c.b);
+    g.it = attn_item<R, KT>(a, g.s, c.rb);
+    g.b = c.b;
+    g.h = c.h;
+    g.rb = c.rb;
+    const int n = g.it.units + E, off = c.off;
+    const long long left = c.end - c.at;
+    const int take = (int)(left < (long long)(n - off) ? left : (long long)(n - off));
+    g.off = off;
+    g.take = min(off + take, g.it.units) - min(off, g.it.units);
+    const bool real = g.take > 0 || (g.it.units == 0 && off == 0);
+    const bool first = off == 0, last = off + take >= g.it.units;
+    g.slot = first && last ? -1 : 2 * (int)blockIdx.x + (first ? 1 : 0);
+    g.last_part = -1;
+    if (first && !last)
+      g.last_part = (int)(((c.at + g.it.units) * c.parts - 1) / c.total);
+    c.at += take;
+    c.off += take;
+    if (c.off == n) attn_next<R>(a, c, attn_blocks<R>(a, g.s));
+    if (real) return true;
+  }
+  return false;
 }
 
-// The last step for 4 values of a row: o unnormalised against 2^m, l its sum.
-// Joins the prefix pass's part, normalises, gates and stores (or, in the
-// prefix pass, keeps the normalised row in fp32).
-__device__ __forceinline__ void attn_finish4(const AttnArgs &a, const AttnRow &r, int d, int DP,
-                                             float4 o, float m, float l) {
-  if (d >= a.D) return;
-  const int64_t rid = (int64_t)r.token * a.Hq + r.head;
-  if (a.prefix_pass) {
-    const float inv = l > 0.0f ? 1.0f / l : l != l ? l : 0.0f;
-    *reinterpret_cast<float4 *>(a.prev_o + rid * DP + d) =
-        make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-    if (d == 0) a.prev_lse[rid] = l == 0.0f ? -INFINITY : m + log2f(l);
-    return;
-  }
-  if (a.prev_o) {
-    const float pl = a.prev_lse[rid];
+// The last step of a row: its output is o * so + prefix part * sp, gated.
+struct AttnFinish {
+  float so, sp, lse2;
+  int64_t id;  // (token, head) of the row
+};
+
+// m, l: the row's maximum (base 2) and sum.
+__device__ __forceinline__ AttnFinish attn_finish(const AttnArgs &a, const AttnRow &r, float m, float l) {
+  AttnFinish f;
+  f.id = (int64_t)r.token * a.Hq + r.head;
+  f.sp = 0.0f;
+  float w = 1.0f;
+  if (a.prev_o && !a.prefix_pass) {
+    const float pl = a.prev_lse[f.id];
     if (pl != -INFINITY) {
       const float top = fmaxf(m, pl);
-      const float wo = m == -INFINITY ? 0.0f : exp2f(m - top), wp = exp2f(pl - top);
-      const float4 p = *reinterpret_cast<const float4 *>(a.prev_o + rid * DP + d);
-      o = make_float4(o.x * wo + p.x * wp, o.y * wo + p.y * wp, o.z * wo + p.z * wp, o.w * wo + p.w * wp);
-      l = l * wo + wp;
+      w = m == -INFINITY ? 0.0f : exp2f(m - top);
+      f.sp = exp2f(pl - top);
+      l = l * w + f.sp;
       m = top;
     }
   }
-  const float inv = l > 0.0f ? 1.0f / l : l != l ? l : 0.0f;
-  float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-  if (l == 0.0f) v[0] = v[1] = v[2] = v[3] = 0.0f;
-  if (a.gate) {
-    const uint2 g = *reinterpret_cast<const uint2 *>(a.gate + r.token * a.g_ts + r.head * a.g_hs + d);
-    const float gv[4] = {__uint_as_float(g.x << 16), __uint_as_float(g.x & 0xffff0000u),
-                         __uint_as_float(g.y << 16), __uint_as_float(g.y & 0xffff0000u)};
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a row that sees nothing is 0
+  f.so = w * inv;
+  f.sp *= inv;
+  f.lse2 = l == 0.0f ? -INFINITY : m + log2f(l);
+  return f;
+}
+
+__device__ __forceinline__ void attn_store_lse(const AttnArgs &a, const AttnFinish &f) {
+  if (a.prefix_pass) a.prev_lse[f.id] = f.lse2;
+  else if (a.lse) a.lse[f.id] = f.lse2 * kLn2;
+}
+
+__device__ __forceinline__ float sigmoidf(float x) { return __fdividef(1.0f, 1.0f + ex2(-x * kLog2e)); }
+
+// N = 4 or 8 values of the row from column d on (the prefix pass keeps the
+// normalised row in fp32).
+template <int N>
+__device__ __forceinline__ void attn_store(const AttnArgs &a, const AttnRow &r, const AttnFinish &f, int d,
+                                           int DP, float (&v)[N]) {
+  if (d >= a.D) return;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = v[i] / (1.0f + ex2(-gv[i] * kLog2e));
+  for (int i = 0; i < N; ++i) v[i] = f.so == 0.0f ? 0.0f : v[i] * f.so;
+  if (a.prefix_pass) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      *reinterpret_cast<float4 *>(a.prev_o + f.id * DP + d + i) =
+          make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    return;
   }
-  const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
-  *reinterpret_cast<uint2 *>(a.out + r.token * a.o_ts + r.head * a.o_hs + d) =
-      make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
-  if (d == 0 && a.lse) a.lse[rid] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+  if (f.sp != 0.0f) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 p = *reinterpret_cast<const float4 *>(a.prev_o + f.id * DP + d + i);
+      v[i] = fmaf(p.x, f.sp, v[i]);
+      v[i + 1] = fmaf(p.y, f.sp, v[i + 1]);
+      v[i + 2] = fmaf(p.z, f.sp, v[i + 2]);
+      v[i + 3] = fmaf(p.w, f.sp, v[i + 3]);
+    }
+  }
+  if (a.gate) {
+    const __nv_bfloat16 *gp = a.gate + r.token * a.g_ts + r.head * a.g_hs + d;
+    uint32_t g[N / 2];
+    if constexpr (N == 8) {
+      const uint4 x = *reinterpret_cast<const uint4 *>(gp);
+      g[0] = x.x, g[1] = x.y, g[2] = x.z, g[3] = x.w;
+    } else {
+      const uint2 x = *reinterpret_cast<const uint2 *>(gp);
+      g[0] = x.x, g[1] = x.y;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      v[i] *= sigmoidf(__uint_as_float(g[i / 2] << 16));
+      v[i + 1] *= sigmoidf(__uint_as_float(g[i / 2] & 0xffff0000u));
+    }
+  }
+  uint32_t w[N / 2];
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[i], v[i + 1]);
+    w[i / 2] = *reinterpret_cast<const uint32_t *>(&h);
+  }
+  __nv_bfloat16 *op = a.out + r.token * a.o_ts + r.head * a.o_hs + d;
+  if constexpr (N == 8) *reinterpret_cast<uint4 *>(op) = make_uint4(w[0], w[1], w[2], w[3]);
+  else *reinterpret_cast<uint2 *>(op) = make_uint2(w[0], w[1]);
 }
 
 // Joins the parts of the items that blocks cut: blockIdx.x is the block that
@@ -430,8 +478,13 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
     }
   }
   const AttnRow ar = attn_row(a, s, w.y, row);
+  const AttnFinish f = attn_finish(a, ar, m, l);
 #pragma unroll
-  for (int v = 0; v < V; ++v) attn_finish4(a, ar, 4 * lane + 128 * v, DP, acc[v], m, l);
+  for (int v = 0; v < V; ++v) {
+    float x[4] = {acc[v].x, acc[v].y, acc[v].z, acc[v].w};
+    attn_store<4>(a, ar, f, 4 * lane + 128 * v, DP, x);
+  }
+  if (lane == 0) attn_store_lse(a, f);
 }
 
 }  // namespace nvfp4

@@ -27,6 +27,7 @@ constexpr int kKT = 64;      // tokens per tile
 constexpr int kWarps = 4;    // consumer warps, 16 tokens of a tile each
 constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kMergeBytes = 32768;
+constexpr int kItemCost = 1;  // of an item's beginning and end, in tiles
 
 template <int MT, int DP>
 struct RowsCfg {
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tmap(&tmV);
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  AttnCursor cur = attn_plan<R, kKT>(a, 1, &plan);
+  AttnCursor cur = attn_plan<R, kKT, kItemCost>(a, 1 + kItemCost, &plan);
   if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, -1);
   volatile int *abort = &abort_flag;
   AttnSegment g;
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int halves = DP / 64;
     int slot = 0, round = 0;
     bool ok = true;
-    while (ok && attn_segment<R, kKT>(a, cur, g)) {
+    while (ok && attn_segment<R, kKT, kItemCost>(a, cur, g)) {
       const int *pages = a.page_table + (a.prefix_pass ? 0 : (int64_t)g.b * a.pt_stride);
       int ids = 0, ids_at = -64;
       for (int u = g.it.u0 + g.off; u < g.it.u0 + g.off + g.take && ok; ++u) {
@@ -169,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float sl2 = a.scale * kLog2e;
     int slot = 0, round = 0;
     bool ok = true;
-    while (ok && attn_segment<R, kKT>(a, cur, g)) {
+    while (ok && attn_segment<R, kKT, kItemCost>(a, cur, g)) {
       // Q fragments and the rows' key intervals.
       uint32_t qf[MT][DP / 16][4];
       int lo[MT][2], hi[MT][2], pos[MT][2];
@@ -375,8 +376,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             acc.z = fmaf(v.z, f, acc.z);
             acc.w = fmaf(v.w, f, acc.w);
           }
-          if (g.whole) {
-            attn_finish4(a, attn_row(a, g.s, g.h, row), c0 + d, DP, acc, mm, ll);
+          if (g.slot < 0) {
+            const AttnRow ar = attn_row(a, g.s, g.h, row);
+            const AttnFinish f = attn_finish(a, ar, mm, ll);
+            float x[4] = {acc.x, acc.y, acc.z, acc.w};
+            attn_store<4>(a, ar, f, c0 + d, DP, x);
+            if (c0 + d == 0) attn_store_lse(a, f);
           } else {
             *reinterpret_cast<float4 *>(a.part_o + ((int64_t)g.slot * R + r) * DP + c0 + d) = acc;
             if (c0 + d == 0) a.part_ml[(int64_t)g.slot * R + r] = make_float2(mm, ll);
@@ -384,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         consumers_sync();
       }
-      if (g.leads && threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(g.b, g.h, g.rb, g.last_part);
+      if (g.last_part >= 0 && threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(g.b, g.h, g.rb, g.last_part);
     }
   }
 }

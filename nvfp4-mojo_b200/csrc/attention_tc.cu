@@ -11,8 +11,9 @@
 // TMEM: QT = 1 and two S buffers, the next S running under the softmax.
 //   warps 0-3 (and 4-7, QT = 2)  softmax of tile 0 (1), Q into shared memory,
 //                                the rare rescaling of O, the epilogue;
-//   then one warp each           MMA issue (one thread), TMA producer, and the
-//                                zeroing of values that no row sees.
+//   then one warp each           MMA issue (one thread), TMA producer, zeroing
+//                                of values that no row sees, and the block's
+//                                list of items.
 // O is rescaled only when a row's maximum has grown by more than 2^8 since
 // the last time (weights then stay below 2^8, exact in the sums' fp32); the
 // reference is the same for sum and product, so the result is not changed.
@@ -33,6 +34,9 @@ static __device__ int g_attn_tc_status;
 
 namespace {
 
+constexpr int kItemCost = 1;  // of an item's beginning and end, in key tiles
+constexpr int kSegs = 4;      // items that the scheduling warp may be ahead
+
 template <int DP>
 struct TcCfg {
   static constexpr int QT = DP <= 128 ? 2 : 1;
@@ -44,7 +48,8 @@ struct TcCfg {
   static constexpr int kSoftWarps = 4 * QT;
   static constexpr int kThreads = (kSoftWarps + 4) * 32;
   static constexpr int offKV = QT * kQ;
-  static constexpr int bytes = offKV + kSlots * kTile + 1024;
+  static constexpr int offStage = offKV + kSlots * kTile;  // 2 KB per softmax warp
+  static constexpr int bytes = offStage + kSoftWarps * 2048 + 1024;
   // TMEM columns: S tiles (tile t, or buffer t when QT = 1), then O.
   static constexpr int colO = 2 * KT;
   static constexpr int cols = 512;
@@ -59,6 +64,15 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
       "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
       "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -112,7 +126,8 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                               ~static_cast<uintptr_t>(1023));
   __shared__ AttnPlanSmem plan;
-  __shared__ uint64_t bars[3 * kSlots + 9];
+  __shared__ uint64_t bars[3 * kSlots + 9 + 2 * kSegs];
+  __shared__ AttnSegment segs[kSegs];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   const uint32_t sbase = smem_u32(smem);
@@ -124,6 +139,8 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
   const uint32_t bar_p = bar_s + 16;          // [2] P written (and O rescaled)
   const uint32_t bar_o = bar_p + 16;          // [2] P V done (tile t; QT = 1: even and odd products)
   const uint32_t bar_end = bar_o + 16;
+  const uint32_t seg_full = bar_end + 8;      // [kSegs] the block's next items
+  const uint32_t seg_empty = seg_full + 8 * kSegs;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -140,6 +157,10 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       mbar_init(bar_o + 8 * t, 1);
     }
     mbar_init(bar_end, 1);
+    for (int i = 0; i < kSegs; ++i) {
+      mbar_init(seg_full + 8 * i, 1);
+      mbar_init(seg_empty + 8 * i, C::kSoftWarps + 3);
+    }
     mbar_fence_init();
     prefetch_tmap(&tmK);
     prefetch_tmap(&tmV);
@@ -152,7 +173,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
     tmem_relinquish();
   }
   tc_fence_before();
-  AttnCursor cur = attn_plan<R, KT>(a, 2, &plan);  // ends with __syncthreads
+  AttnCursor cur = attn_plan<R, KT, kItemCost>(a, 2 + kItemCost, &plan);  // ends with __syncthreads
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;");
   const uint32_t tmem = tmem_slot;
@@ -160,6 +181,19 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
   volatile int *abort = &abort_flag;
   int *status = &g_attn_tc_status;
   AttnSegment g;
+  // The next item of the block from the scheduling warp's ring (every lane
+  // of the warp calls it; take < 0: no more).
+  uint32_t nseg = 0;
+  auto next_seg = [&]() -> bool {
+    const uint32_t i = nseg % kSegs;
+    if (!__all_sync(0xffffffffu, mbar_wait(seg_full + 8 * i, (nseg / kSegs) & 1, status, kDevTimeoutDec, abort)))
+      return false;
+    g = segs[i];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(seg_empty + 8 * i);
+    ++nseg;
+    return g.take >= 0;
+  };
   // Tiles of an item in use: the second one only with rows beyond 128.
   auto tiles = [&](const AttnSegment &x) { return QT == 2 && x.s.ql * a.G - x.rb * R > 128 ? 2 : 1; };
 
@@ -174,7 +208,8 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
 
     // This warp's 32 rows of Q, 16-byte chunks swizzled as the MMA reads them;
     // rows and columns beyond the item's or the head's are zeros.
-    auto load_q = [&](const AttnSegment &x) {
+    auto load_q = [&]() {
+      const AttnSegment &x = g;
       const int row = x.rb * R + my;
       const __nv_bfloat16 *src = nullptr;
       if (row < x.s.ql * a.G) {
@@ -183,15 +218,18 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       }
       constexpr int CH = DP / 8, RPI = 32 / CH;  // chunks per row, rows per warp step
       const int c = lane % CH;
-#pragma unroll 8
+#pragma unroll
       for (int r0 = 0; r0 < 32; r0 += RPI) {
         const int r = r0 + lane / CH;
         const uint64_t p = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(src), r);
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (p && 8 * c < a.D) v = *(reinterpret_cast<const uint4 *>(p) + c);
         const int rr = wq * 32 + r;
-        *reinterpret_cast<uint4 *>(Q + (c >> 3) * (128 * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
+        const bool on = p != 0 && 8 * c < a.D;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                         smem_u32(Q + (c >> 3) * (128 * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4))),
+                     "l"(on ? p + 16 * c : reinterpret_cast<uint64_t>(a.q)), "r"(on ? 16 : 0)
+                     : "memory");
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_q + 8 * t);
@@ -205,8 +243,8 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
                      : mbar_wait(bar_o + 8 * (i & 1), (i >> 1) & 1, status, kDevTimeoutAcc, abort);
     };
     uint32_t n = 0;  // key tiles of this query tile so far
-    bool have = attn_segment<R, KT>(a, cur, g), ok = true;
-    if (have && g.take > 0 && t < tiles(g)) load_q(g);
+    bool have = next_seg(), ok = true;
+    if (have && g.take > 0 && t < tiles(g)) load_q();
     while (have && ok) {
       const bool mine = t < tiles(g);
       const int row = g.rb * R + my;
@@ -305,37 +343,71 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       if (!ok) break;
       // The next item's queries first (this item's S are all done), so that
       // its first S runs under this epilogue.
-      const AttnSegment e = g;
-      have = attn_segment<R, KT>(a, cur, g);
-      if (have && g.take > 0 && t < tiles(g)) load_q(g);
+      const int e_take = g.take, e_slot = g.slot, e_rb = g.rb;
+      if (g.last_part >= 0 && threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(g.b, g.h, g.rb, g.last_part);
+      const int left = min(g.s.ql * a.G - e_rb * R - t * 128 - wq * 32, 32);  // this warp's rows in use
+      have = next_seg();
+      if (have && g.take > 0 && t < tiles(g)) load_q();
       if (!mine) continue;
-      if (e.take > 0) {
+      if (e_take > 0) {
         if (!__all_sync(0xffffffffu, o_wait(n - 1))) break;
         tc_fence_after();
       }
+      // O by way of shared memory, 16 columns at a time, so that 4 lanes
+      // store 16 columns of a row side by side.
+      AttnFinish f = {};
+      if (in && e_slot < 0) {
+        f = attn_finish(a, ar, m, l);
+        attn_store_lse(a, f);
+      }
+      if (in && e_slot >= 0) a.part_ml[(int64_t)e_slot * R + my] = make_float2(m, l);
+      AttnRow rows4[4];   // of this lane's 4 rows of a step
+      AttnFinish fin4[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int src = 8 * i + (lane >> 2);
+        rows4[i].token = __shfl_sync(0xffffffffu, ar.token, src);
+        rows4[i].head = __shfl_sync(0xffffffffu, ar.head, src);
+        fin4[i].sp = __shfl_sync(0xffffffffu, f.sp, src);
+        fin4[i].so = 1.0f;  // applied by the row's own thread
+        fin4[i].id = (int64_t)rows4[i].token * a.Hq + rows4[i].head;
+      }
+      uint8_t *stage = smem + C::offStage + warp * 2048;
 #pragma unroll 1
-      for (int c = 0; c < DP; c += 32) {
-        uint32_t o[32];
-        if (e.take > 0) {
-          tmem_ld_32x32b_x32(tO + c, o);
+      for (int c = 0; c < DP; c += 16) {
+        uint32_t o[16];
+        if (e_take > 0) {
+          tmem_ld_x16(tO + c, o);
           tmem_ld_wait();
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0u;
+          for (int i = 0; i < 16; ++i) o[i] = 0u;
         }
-        if (!in) continue;
+        if (e_slot < 0) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          const float4 v = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]),
-                                       __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
-          if (e.whole)
-            attn_finish4(a, ar, c + i, DP, v, m, l);
-          else
-            *reinterpret_cast<float4 *>(a.part_o + ((int64_t)e.slot * R + my) * DP + c + i) = v;
+          for (int i = 0; i < 16; ++i)
+            o[i] = f.so == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[i]) * f.so);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<uint4 *>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
+              make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 8 * i + (lane >> 2), d = c + 4 * (lane & 3);
+          const float4 x = *reinterpret_cast<const float4 *>(stage + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
+          if (r < left) {
+            if (e_slot < 0) {
+              float v[4] = {x.x, x.y, x.z, x.w};
+              attn_store<4>(a, rows4[i], fin4[i], d, DP, v);
+            } else {
+              *reinterpret_cast<float4 *>(a.part_o + ((int64_t)e_slot * R + t * 128 + wq * 32 + r) * DP + d) = x;
+            }
+          }
+        }
+        __syncwarp();
       }
-      if (in && !e.whole) a.part_ml[(int64_t)e.slot * R + my] = make_float2(m, l);
-      if (e.leads && threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(e.b, e.h, e.rb, e.last_part);
       tc_fence_before();
     }
   } else {
@@ -350,6 +422,15 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
         uint32_t tile = 0;             // key tiles so far: K in slot 2 tile, V in 2 tile + 1
         uint32_t ns[2] = {0, 0};       // S issued per query tile
         uint32_t nq[2] = {0, 0};       // queries awaited per query tile
+        // next_seg for this thread alone.
+        auto next_one = [&]() -> bool {
+          const uint32_t i = nseg % kSegs;
+          if (!mbar_wait(seg_full + 8 * i, (nseg / kSegs) & 1, status, kDevTimeoutDec, abort)) return false;
+          g = segs[i];
+          mbar_arrive(seg_empty + 8 * i);
+          ++nseg;
+          return g.take >= 0;
+        };
         bool pend = false, pfirst = false;
         int pnt = 0;                   // the pending P V: query tiles, first of its item
         auto wait = [&](uint32_t bar, uint32_t ph, int code) {
@@ -392,7 +473,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
           tc_commit(empty + 8 * ((2 * vtile + 1) % kSlots));
           pend = false;
         };
-        while (ok && attn_segment<R, KT>(a, cur, g)) {
+        while (ok && next_one()) {
           const int nt = tiles(g);
           for (int u = 0; u < g.take && ok; ++u, ++tile) {
             if (u == 0 && pend) pv_all(tile - 1);  // the item before is finished first
@@ -428,7 +509,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       constexpr int halves = DP / 64;
       uint32_t at = 0;
       bool ok = true;
-      while (ok && attn_segment<R, KT>(a, cur, g)) {
+      while (ok && next_seg()) {
         const int *pages = a.page_table + (a.prefix_pass ? 0 : (int64_t)g.b * a.pt_stride);
         int ids = 0, ids_at = -64;
         for (int u = 0; u < g.take && ok; ++u) {
@@ -473,7 +554,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       // but what lies there may not be finite.
       uint32_t at = 0, phase = 0;
       bool ok = true;
-      while (ok && attn_segment<R, KT>(a, cur, g)) {
+      while (ok && next_seg()) {
         for (int u = 0; u < g.take; ++u, at += 2) {
           const int j0 = (g.it.u0 + g.off + u) * KT;
           if (j0 >= g.it.lo && j0 + KT <= g.it.hi) continue;
@@ -495,6 +576,17 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(full + 8 * slot);
         }
+      }
+    } else if (lane == 0) {
+      // ---------------- the block's items, ahead of the other warps --------
+      for (uint32_t n = 0;; ++n) {
+        const uint32_t i = n % kSegs;
+        if (n >= kSegs && !mbar_wait(seg_empty + 8 * i, (n / kSegs - 1) & 1, status, kDevTimeoutEmpty, abort)) break;
+        const bool more = attn_segment<R, KT, kItemCost>(a, cur, g);
+        if (!more) g.take = -1;
+        segs[i] = g;
+        mbar_arrive(seg_full + 8 * i);
+        if (!more) break;
       }
     }
   }
