@@ -7,7 +7,8 @@
 // item is (sequence, key/value head, R consecutive rows); its keys, the union
 // of what its rows see, are walked in units of KT.  All items' units, in the
 // order sequence, head, rows, form one line of W units that the launch's
-// blocks divide evenly: block c takes [c W / parts, (c + 1) W / parts).  An
+// blocks divide evenly: block c takes [c W / parts, (c + 1) W / parts).  W is
+// below 2^31 (checked by the caller from the bounds of the call).  An
 // item cut by a block boundary leaves unnormalised parts in the workspace, at
 // most two per block, which a second launch joins in the order of the blocks.
 // The division depends on the lengths alone, so results repeat bit for bit.
@@ -16,6 +17,7 @@
 #include <cuda_bf16.h>
 
 #include "attention.h"
+#include "tc_common.cuh"
 
 namespace nvfp4 {
 
@@ -169,17 +171,44 @@ __device__ __forceinline__ int attn_item_units(const AttnArgs &a, const AttnSeq 
   return attn_item<R, KT>(a, s, rb).units + E;
 }
 
+// Bounded wait on an mbarrier phase, as mbar_wait (tc_common.cuh) in fewer
+// instructions: the attention kernels wait in many places, and their code must
+// stay in the instruction cache.
+__device__ __forceinline__ bool attn_wait(uint32_t bar, uint32_t parity, int *status, int code,
+                                          volatile int *abort) {
+  bool ok = mbar_try_wait(bar, parity);
+  if (!ok) {
+    uint32_t t0, t;
+    asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t0));
+    do {
+      ok = mbar_try_wait(bar, parity);
+      asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
+      if (!ok && t - t0 > (uint32_t)kWaitLimitNs) {
+        *status = code;
+        *abort = 1;
+      }
+    } while (!ok && !*abort);
+  }
+  return ok;
+}
+
 // Where a block starts on the line, and how far it goes.
 struct AttnCursor {
-  int b, h, rb, off;    // item and unit within it
-  long long at, end;    // on the line
-  long long total;      // W
-  int parts;
+  int b, h, rb, off;  // item and unit within it
+  int at, end;        // on the line
+  int total, parts;   // W and the blocks that have a share
 };
+
+// The first unit of part c: floor(c total / parts).  The quotient's fraction
+// is a multiple of 1 / parts, so a quarter unit before the division keeps the
+// rounded product on the right side.
+__device__ __forceinline__ int attn_line_at(int c, int total, int parts, double inv) {
+  return (int)(((double)c * (double)total + 0.25) * inv);
+}
 
 struct AttnPlanSmem {
   int units[kPlanCache];  // per sequence and head
-  long long sum[32];
+  int sum[32];
   AttnCursor cur;
 };
 
@@ -187,127 +216,90 @@ struct AttnPlanSmem {
 // most gridDim.x and one per `min_units` units.
 template <int R, int KT, int E>
 __device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units, AttnPlanSmem *sm) {
-  const int nt = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = nt >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
   const int NS = attn_num_seqs(a);
-  long long sum = 0;
-  // Sequences of few items: a thread each; of many: a warp each.
-  const bool by_warp = a.max_blocks > 4;
-  auto lane_units = [&](int b) -> int {  // by_warp: this lane's share
+  // Units of the items start, start + step, ... of sequence b and one head.
+  auto seq_units = [&](int b, int start, int step) -> int {
     const AttnSeq s = attn_seq(a, b);
     const int nb = attn_blocks<R>(a, s);
     int u = 0;
-    for (int rb = by_warp ? lane : 0; rb < nb; rb += by_warp ? 32 : 1) u += attn_item_units<R, KT, E>(a, s, rb);
+#pragma unroll 1
+    for (int rb = start; rb < nb; rb += step) u += attn_item_units<R, KT, E>(a, s, rb);
     return u;
   };
-  auto warp_units = [&](int b) -> int {  // every lane gets sequence b's units
-    int u = lane_units(b);
-    if (by_warp)
-      for (int o = 16; o; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-    return u;
-  };
-  if (by_warp) {
-    for (int b = warp; b < NS; b += nw) {
-      const int u = warp_units(b);
-      if (lane == 0) {
-        if (b < kPlanCache) sm->units[b] = u;
-        sum += u;
-      }
-    }
-  } else {
-    for (int b = tid; b < NS; b += nt) {
-      const int u = lane_units(b);
+  // Sequences of few items: a thread each; of many: a warp each.
+  const bool by_warp = a.max_blocks > 4;
+  int sum = 0;
+#pragma unroll 1
+  for (int b = by_warp ? warp : tid; b < NS; b += by_warp ? nw : (int)blockDim.x) {
+    int u = seq_units(b, by_warp ? lane : 0, by_warp ? 32 : 1);
+    if (by_warp) u = __reduce_add_sync(0xffffffffu, u);
+    if (!by_warp || lane == 0) {
       if (b < kPlanCache) sm->units[b] = u;
       sum += u;
     }
   }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  sum = __reduce_add_sync(0xffffffffu, sum);
   if (lane == 0) sm->sum[warp] = sum;
   __syncthreads();
   if (warp == 0) {
-    long long total = 0;
-    for (int i = 0; i < nw; ++i) total += sm->sum[i];
-    total *= a.Hkv;
-    AttnCursor c;
-    c.total = total;
-    const long long most = (total + min_units - 1) / min_units;
-    c.parts = (int)(most < (long long)gridDim.x ? most : (long long)gridDim.x);
-    c.b = c.h = c.rb = c.off = 0;
-    c.at = c.end = 0;
+    AttnCursor c = {};
+    c.total = a.Hkv * __reduce_add_sync(0xffffffffu, lane < nw ? sm->sum[lane] : 0);
+    c.parts = min((c.total + min_units - 1) / min_units, (int)gridDim.x);
     if ((int)blockIdx.x < c.parts) {
-      c.at = (long long)blockIdx.x * total / c.parts;
-      c.end = (long long)(blockIdx.x + 1) * total / c.parts;
-      long long before = 0;
-      long long o = c.at;
-      int ub = 0;
-      for (int base = 0; base < NS; base += 32) {  // the sequence that holds unit c.at
-        long long u = 0;
-        if (base + 32 <= kPlanCache || !by_warp) {
-          const int b = base + lane;
-          if (b < NS) u = b < kPlanCache ? sm->units[b] : lane_units(b);
-        } else {
-          for (int i = 0; i < 32 && base + i < NS; ++i) {
-            const int w = warp_units(base + i);
-            if (i == lane) u = w;
-          }
-        }
-        long long inc = u * a.Hkv;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const long long v = __shfl_up_sync(0xffffffffu, inc, d);
-          if (lane >= d) inc += v;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, before + inc > c.at);
-        if (hit) {
-          const int f = __ffs(hit) - 1;
-          c.b = base + f;
-          ub = (int)__shfl_sync(0xffffffffu, u, f);
-          o = c.at - before - (__shfl_sync(0xffffffffu, inc, f) - (long long)ub * a.Hkv);
-          break;
-        }
-        before += __shfl_sync(0xffffffffu, inc, 31);
-      }
-      c.h = (int)(o / ub);
-      int r = (int)(o % ub);
-      const AttnSeq s = attn_seq(a, c.b);
-      const int nb = attn_blocks<R>(a, s);
-      for (int base = 0; base < nb; base += 32) {  // the item within the sequence and head
-        const int rb = base + lane;
-        int inc = rb < nb ? attn_item_units<R, KT, E>(a, s, rb) : 0;
-        const int u = inc;
+      const double inv = 1.0 / (double)c.parts;
+      c.at = attn_line_at(blockIdx.x, c.total, c.parts, inv);
+      c.end = attn_line_at(blockIdx.x + 1, c.total, c.parts, inv);
+      // The sequence that holds unit c.at, 32 sequences at a time; then, with
+      // its units per head, the item in the same way.
+      int o = c.at, ub = 0;
+#pragma unroll 1
+      for (int base = 0; base < NS; base += 32) {
+        const int b = base + lane;
+        const int u = b >= NS ? 0 : b < kPlanCache ? sm->units[b] : seq_units(b, 0, 1);
+        int inc = u * a.Hkv;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
           const int v = __shfl_up_sync(0xffffffffu, inc, d);
           if (lane >= d) inc += v;
         }
-        const unsigned hit = __ballot_sync(0xffffffffu, inc > r);
+        const unsigned hit = __ballot_sync(0xffffffffu, inc > o);
+        if (hit) {
+          const int f = __ffs(hit) - 1;
+          c.b = base + f;
+          ub = __shfl_sync(0xffffffffu, u, f);
+          o -= __shfl_sync(0xffffffffu, inc, f) - ub * a.Hkv;
+          break;
+        }
+        o -= __shfl_sync(0xffffffffu, inc, 31);
+      }
+      c.h = o / ub;
+      o -= c.h * ub;
+      const AttnSeq s = attn_seq(a, c.b);
+      const int nb = attn_blocks<R>(a, s);
+#pragma unroll 1
+      for (int base = 0; base < nb; base += 32) {
+        const int u = base + lane < nb ? attn_item_units<R, KT, E>(a, s, base + lane) : 0;
+        int inc = u;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, inc, d);
+          if (lane >= d) inc += v;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, inc > o);
         if (hit) {
           const int f = __ffs(hit) - 1;
           c.rb = base + f;
-          c.off = r - (__shfl_sync(0xffffffffu, inc, f) - __shfl_sync(0xffffffffu, u, f));
+          c.off = o - (__shfl_sync(0xffffffffu, inc, f) - __shfl_sync(0xffffffffu, u, f));
           break;
         }
-        r -= __shfl_sync(0xffffffffu, inc, 31);
+        o -= __shfl_sync(0xffffffffu, inc, 31);
       }
     }
     if (lane == 0) sm->cur = c;
   }
   __syncthreads();
   return sm->cur;
-}
-
-// The next item on the line after (b, h, rb).
-template <int R>
-__device__ __forceinline__ void attn_next(const AttnArgs &a, AttnCursor &c, int nb) {
-  c.off = 0;
-  if (++c.rb < nb) return;
-  c.rb = 0;
-  if (++c.h < a.Hkv) return;
-  c.h = 0;
-  const int NS = attn_num_seqs(a);
-  do {
-    ++c.b;
-  } while (c.b < NS && attn_seq(a, c.b).ql == 0);
 }
 
 // One stretch of a block's share: key units [off, off + take) of an item.
@@ -321,26 +313,41 @@ struct AttnSegment {
 
 template <int R, int KT, int E>
 __device__ __forceinline__ bool attn_segment(const AttnArgs &a, AttnCursor &c, AttnSegment &g) {
+#pragma unroll 1
   while (c.at < c.end) {
     g.s = attn_seq(a, c.b);
+    const int nb = attn_blocks<R>(a, g.s);
+    if (c.rb >= nb) {  // on to the next head or sequence
+      c.rb = 0;
+      if (nb == 0 || ++c.h == a.Hkv) {
+        c.h = 0;
+        ++c.b;
+      }
+      continue;
+    }
     g.it = attn_item<R, KT>(a, g.s, c.rb);
     g.b = c.b;
     g.h = c.h;
     g.rb = c.rb;
     const int n = g.it.units + E, off = c.off;
-    const long long left = c.end - c.at;
-    const int take = (int)(left < (long long)(n - off) ? left : (long long)(n - off));
+    const int take = min(c.end - c.at, n - off);
     g.off = off;
     g.take = min(off + take, g.it.units) - min(off, g.it.units);
     const bool real = g.take > 0 || (g.it.units == 0 && off == 0);
     const bool first = off == 0, last = off + take >= g.it.units;
     g.slot = first && last ? -1 : 2 * (int)blockIdx.x + (first ? 1 : 0);
     g.last_part = -1;
-    if (first && !last)
-      g.last_part = (int)(((c.at + g.it.units) * c.parts - 1) / c.total);
+    if (first && !last) {
+      const int x = c.at + g.it.units - 1;  // the item's last unit
+      const double inv = 1.0 / (double)c.parts;
+      int p = min((int)((double)x * (double)c.parts / (double)c.total), c.parts - 1);
+      while (p + 1 < c.parts && attn_line_at(p + 1, c.total, c.parts, inv) <= x) ++p;
+      while (attn_line_at(p, c.total, c.parts, inv) > x) --p;
+      g.last_part = p;
+    }
     c.at += take;
     c.off += take;
-    if (c.off == n) attn_next<R>(a, c, attn_blocks<R>(a, g.s));
+    if (c.off == n) c.off = 0, ++c.rb;
     if (real) return true;
   }
   return false;

@@ -104,13 +104,18 @@ AttnLayout attn_layout(const nvfp4_attention_desc &d, const nvfp4_attention_batc
   return L;
 }
 
-// The line's units are counted in 31 bits per sequence and head.
+// The line of units (attention.cuh) is counted in 31 bits.
 int check_size(const nvfp4_attention_desc &d, const nvfp4_attention_batch &b, int page_size) {
   const int64_t G = d.num_heads / d.num_kv_heads;
-  const int64_t keys = (int64_t)b.max_pages * page_size + b.prefix_len;
-  if (b.num_tokens * G >= (1ll << 30) || (b.num_tokens * G / 16 + 1) * (keys / 64 + 2) >= (1ll << 31))
-    return fail(NVFP4_ERR_UNSUPPORTED, "%lld tokens against %lld keys in one call", (long long)b.num_tokens,
-                (long long)keys);
+  const double keys = (double)b.max_pages * page_size, rows = (double)b.num_tokens * G;
+  const AttnLayout L = attn_layout(d, b, 1);
+  auto line = [&](int R, double n, double seqs) {
+    return d.num_kv_heads * (rows / R + seqs) * (n / (R == 256 ? 128 : 64) + 3);
+  };
+  if (rows >= (double)(1ll << 30) || line(L.R1, keys, b.num_seqs) >= 2147483648.0 ||
+      (b.prefix_len > 0 && line(L.R0, b.prefix_len, 1) >= 2147483648.0))
+    return fail(NVFP4_ERR_UNSUPPORTED, "%lld tokens against up to %.0f keys in one call",
+                (long long)b.num_tokens, keys + b.prefix_len);
   return NVFP4_OK;
 }
 

@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           if (round > 0) {
-            const bool w = mbar_wait(empty + 8 * slot, (round - 1) & 1, &g_attn_rows_status,
+            const bool w = attn_wait(empty + 8 * slot, (round - 1) & 1, &g_attn_rows_status,
                                      kDevTimeoutEmpty, abort);
             if (!__all_sync(0xffffffffu, w)) {
               ok = false;
@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int issued = round * kSlots + slot;
     for (int q = issued > kSlots ? issued - kSlots : 0; q < issued; ++q) {
       volatile int no_abort = 0;
-      mbar_wait(full + 8 * (q % kSlots), (q / kSlots) & 1, &g_attn_rows_status, kDevTimeoutFull, &no_abort);
+      attn_wait(full + 8 * (q % kSlots), (q / kSlots) & 1, &g_attn_rows_status, kDevTimeoutFull, &no_abort);
     }
   } else {
     // ---------------- consumers ----------------
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool any = j0 < g.it.hi && j0 + 16 > g.it.lo;
         float s[MT][2][4];
         // ---- S = Q K^T
-        bool w = mbar_wait(full + 8 * slot, round & 1, &g_attn_rows_status, kDevTimeoutFull, abort);
+        bool w = attn_wait(full + 8 * slot, round & 1, &g_attn_rows_status, kDevTimeoutFull, abort);
         if (!__all_sync(0xffffffffu, w)) {
           ok = false;
           break;
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         // ---- O += P V
-        w = mbar_wait(full + 8 * slot, round & 1, &g_attn_rows_status, kDevTimeoutFull, abort);
+        w = attn_wait(full + 8 * slot, round & 1, &g_attn_rows_status, kDevTimeoutFull, abort);
         if (!__all_sync(0xffffffffu, w)) {
           ok = false;
           break;

@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
   uint32_t nseg = 0;
   auto next_seg = [&]() -> bool {
     const uint32_t i = nseg % kSegs;
-    if (!__all_sync(0xffffffffu, mbar_wait(seg_full + 8 * i, (nseg / kSegs) & 1, status, kDevTimeoutDec, abort)))
+    if (!__all_sync(0xffffffffu, attn_wait(seg_full + 8 * i, (nseg / kSegs) & 1, status, kDevTimeoutDec, abort)))
       return false;
     g = segs[i];
     __syncwarp();
@@ -239,8 +239,8 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
     // may be ahead of the last two products, so these alternate between two
     // barriers: each then has at most one phase outstanding.
     auto o_wait = [&](uint32_t i) {
-      return QT == 2 ? mbar_wait(bar_o + 8 * t, i & 1, status, kDevTimeoutAcc, abort)
-                     : mbar_wait(bar_o + 8 * (i & 1), (i >> 1) & 1, status, kDevTimeoutAcc, abort);
+      return QT == 2 ? attn_wait(bar_o + 8 * t, i & 1, status, kDevTimeoutAcc, abort)
+                     : attn_wait(bar_o + 8 * (i & 1), (i >> 1) & 1, status, kDevTimeoutAcc, abort);
     };
     uint32_t n = 0;  // key tiles of this query tile so far
     bool have = next_seg(), ok = true;
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
           const int b = QT == 2 ? t : (n & 1);
           const uint32_t ph = QT == 2 ? n & 1 : (n >> 1) & 1;
           const uint32_t tS = tmem + lanes + b * KT;
-          if (!__all_sync(0xffffffffu, mbar_wait(bar_s + 8 * b, ph, status, kDevTimeoutAcc, abort))) {
+          if (!__all_sync(0xffffffffu, attn_wait(bar_s + 8 * b, ph, status, kDevTimeoutAcc, abort))) {
             ok = false;
             break;
           }
@@ -361,52 +361,100 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
         attn_store_lse(a, f);
       }
       if (in && e_slot >= 0) a.part_ml[(int64_t)e_slot * R + my] = make_float2(m, l);
-      AttnRow rows4[4];   // of this lane's 4 rows of a step
-      AttnFinish fin4[4];
+      // This lane's 4 rows of a step, at its 4 columns.
+      const int64_t id = in ? (int64_t)ar.token * a.Hq + ar.head : 0;
+      const float so = e_slot < 0 ? f.so : 1.0f;
+      int64_t at[4], gat[4], pat[4];
+      float sp[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int src = 8 * i + (lane >> 2);
-        rows4[i].token = __shfl_sync(0xffffffffu, ar.token, src);
-        rows4[i].head = __shfl_sync(0xffffffffu, ar.head, src);
-        fin4[i].sp = __shfl_sync(0xffffffffu, f.sp, src);
-        fin4[i].so = 1.0f;  // applied by the row's own thread
-        fin4[i].id = (int64_t)rows4[i].token * a.Hq + rows4[i].head;
+        const int tok = __shfl_sync(0xffffffffu, ar.token, src), head = __shfl_sync(0xffffffffu, ar.head, src);
+        pat[i] = __shfl_sync(0xffffffffu, id, src) * DP;
+        if (e_slot >= 0) at[i] = ((int64_t)e_slot * R + t * 128 + wq * 32 + src) * DP;
+        else if (a.prefix_pass) at[i] = pat[i];
+        else at[i] = tok * a.o_ts + head * a.o_hs;
+        gat[i] = tok * a.g_ts + head * a.g_hs;
+        sp[i] = __shfl_sync(0xffffffffu, f.sp, src);
       }
-      uint8_t *stage = smem + C::offStage + warp * 2048;
+      const bool to_f32 = e_slot >= 0 || a.prefix_pass, joins = !to_f32 && a.prev_o, gates = !to_f32 && a.gate;
+      float *f32 = e_slot >= 0 ? a.part_o : a.prev_o;
+      const uint32_t stage = sbase + C::offStage + warp * 2048;
+      const uint32_t st_w = stage + lane * 64, x_w = (lane >> 1) & 3;
+      // The gates come a step ahead of their use.
+      auto load_gates = [&](uint2 (&v)[4], int d) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (gates && 8 * i + (lane >> 2) < left && d < a.D)
+            v[i] = *reinterpret_cast<const uint2 *>(a.gate + gat[i] + d);
+      };
+      uint2 gv[4] = {}, gn[4] = {};
+      load_gates(gn, 4 * (lane & 3));
 #pragma unroll 1
       for (int c = 0; c < DP; c += 16) {
-        uint32_t o[16];
-        if (e_take > 0) {
-          tmem_ld_x16(tO + c, o);
-          tmem_ld_wait();
-        } else {
+        const int d = c + 4 * (lane & 3);
+        uint32_t o[16] = {};
+        if (e_take > 0) tmem_ld_x16(tO + c, o);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = 0u;
+        for (int i = 0; i < 4; ++i) gv[i] = gn[i];
+        if (c + 16 < DP) load_gates(gn, d + 16);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) v[x] = so == 0.0f ? 0.0f : __uint_as_float(o[4 * i + x]) * so;
+          asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(st_w + ((i ^ x_w) << 4)), "f"(v[0]),
+                       "f"(v[1]), "f"(v[2]), "f"(v[3])
+                       : "memory");
         }
-        if (e_slot < 0) {
+        __syncwarp();
+        float4 x[4];
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            o[i] = f.so == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[i]) * f.so);
+        for (int i = 0; i < 4; ++i) {
+          const int r = 8 * i + (lane >> 2);
+          asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
+                       : "=f"(x[i].x), "=f"(x[i].y), "=f"(x[i].z), "=f"(x[i].w)
+                       : "r"(stage + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4))
+                       : "memory");
+        }
+        __syncwarp();
+        if (d >= a.D) continue;
+        if (to_f32) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (8 * i + (lane >> 2) < left) *reinterpret_cast<float4 *>(f32 + at[i] + d) = x[i];
+          continue;
+        }
+        if (joins) {
+          float4 p[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            p[i] = make_float4(0, 0, 0, 0);
+            if (sp[i] != 0.0f) p[i] = *reinterpret_cast<const float4 *>(a.prev_o + pat[i] + d);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[i].x = fmaf(p[i].x, sp[i], x[i].x);
+            x[i].y = fmaf(p[i].y, sp[i], x[i].y);
+            x[i].z = fmaf(p[i].z, sp[i], x[i].z);
+            x[i].w = fmaf(p[i].w, sp[i], x[i].w);
+          }
+        }
+        if (gates) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[i].x *= sigmoidf(__uint_as_float(gv[i].x << 16));
+            x[i].y *= sigmoidf(__uint_as_float(gv[i].x & 0xffff0000u));
+            x[i].z *= sigmoidf(__uint_as_float(gv[i].y << 16));
+            x[i].w *= sigmoidf(__uint_as_float(gv[i].y & 0xffff0000u));
+          }
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<uint4 *>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
-              make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 8 * i + (lane >> 2), d = c + 4 * (lane & 3);
-          const float4 x = *reinterpret_cast<const float4 *>(stage + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
-          if (r < left) {
-            if (e_slot < 0) {
-              float v[4] = {x.x, x.y, x.z, x.w};
-              attn_store<4>(a, rows4[i], fin4[i], d, DP, v);
-            } else {
-              *reinterpret_cast<float4 *>(a.part_o + ((int64_t)e_slot * R + t * 128 + wq * 32 + r) * DP + d) = x;
-            }
-          }
-        }
-        __syncwarp();
+          if (8 * i + (lane >> 2) < left)
+            *reinterpret_cast<uint2 *>(a.out + at[i] + d) =
+                make_uint2(pack_bf16(x[i].x, x[i].y), pack_bf16(x[i].z, x[i].w));
       }
       tc_fence_before();
     }
@@ -419,87 +467,94 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
         constexpr uint32_t idS = idesc_bf16_f32(128, KT);
         constexpr uint32_t idO = idesc_bf16_f32(128, DP) | kTransposeB;
         bool ok = true;
-        uint32_t tile = 0;             // key tiles so far: K in slot 2 tile, V in 2 tile + 1
-        uint32_t ns[2] = {0, 0};       // S issued per query tile
-        uint32_t nq[2] = {0, 0};       // queries awaited per query tile
-        // next_seg for this thread alone.
-        auto next_one = [&]() -> bool {
-          const uint32_t i = nseg % kSegs;
-          if (!mbar_wait(seg_full + 8 * i, (nseg / kSegs) & 1, status, kDevTimeoutDec, abort)) return false;
-          g = segs[i];
-          mbar_arrive(seg_empty + 8 * i);
-          ++nseg;
-          return g.take >= 0;
-        };
-        bool pend = false, pfirst = false;
-        int pnt = 0;                   // the pending P V: query tiles, first of its item
+        uint32_t tile = 0;       // key tiles so far: K in slot 2 tile, V in 2 tile + 1
+        uint32_t ns[2] = {0, 0}; // S issued per query tile
+        uint32_t nq[2] = {0, 0}; // queries awaited per query tile
+        bool pend = false, pfirst = false, more = true;
+        int pnt = 0, u = 0, nt = 0;  // pnt, pfirst: of the pending P V
+        g.take = 0;
         auto wait = [&](uint32_t bar, uint32_t ph, int code) {
-          ok = ok && mbar_wait(bar, ph, status, code, abort);
-          return ok;
+          ok = ok && attn_wait(bar, ph, status, code, abort);
         };
-        auto full_wait = [&](uint32_t pos) {
-          return wait(full + 8 * (pos % kSlots), (pos / kSlots) & 1, kDevTimeoutFull);
-        };
-        auto do_s = [&](int t, bool first) {
-          if (first && !wait(bar_q + 8 * t, nq[t]++ & 1, kDevTimeoutDec)) return;
-          tc_fence_after();
-          const int b = QT == 2 ? t : (ns[0] & 1);
-          const uint32_t k0 = sbase + C::offKV + ((2 * tile) % kSlots) * C::kTile;
-          const uint32_t q0 = sbase + t * C::kQ;
+        while (ok && (more || pend)) {
+          // The next key tile, if any; P V of the tile before it is pending.
+          if (more && u == g.take) {
+            do {
+              const uint32_t i = nseg % kSegs;
+              wait(seg_full + 8 * i, (nseg / kSegs) & 1, kDevTimeoutDec);
+              if (!ok) break;
+              g = segs[i];
+              mbar_arrive(seg_empty + 8 * i);
+              ++nseg;
+            } while (g.take == 0);
+            if (!ok) break;
+            more = g.take > 0;
+            u = 0;
+            nt = tiles(g);
+          }
+          // In which order: bits 0, 1 the query tile, bit 2 a P V, bit 3 none.
+          // Within an item QT = 2 alternates P V and S of the two tiles and
+          // QT = 1 keeps one S ahead; an item's last P V come before the next
+          // item's S, which may wait for its queries.
+          uint32_t ops;
+          const bool inner = more && pend && u > 0;
+          if (QT == 2) ops = inner ? 0x1504 : 0x1054;
+          else ops = inner ? 0x8840 : 0x8804;
+          if (!pend || pnt < 2) ops |= QT == 2 ? (inner ? 0x0800 : 0x0080) : 0;
+          if (!pend) ops |= QT == 2 ? 0x0008 : (inner ? 0x0080 : 0x0008);
+          if (!more) ops |= QT == 2 ? 0x8800 : 0x0080;
+          if (more && nt < 2 && QT == 2) ops |= 0x8000;
+          bool v_in = false, k_in = false;
+#pragma unroll 1
+          for (; ops != 0x8888 && ok; ops = (ops >> 4) | 0x8000) {
+            const int op = ops & 15, t = op & 3;
+            if (op & 8) continue;
+            if (op & 4) {
+              if (!v_in) wait(full + 8 * ((2 * tile - 1) % kSlots), ((2 * tile - 1) / kSlots) & 1, kDevTimeoutFull);
+              v_in = true;
+              const uint32_t np = QT == 2 ? ns[t] - 1 : tile - 1;  // this P V's count
+              const int b = QT == 2 ? t : (np & 1);
+              wait(bar_p + 8 * b, (QT == 2 ? np : np >> 1) & 1, kDevTimeoutDec);
+              if (!ok) break;
+              tc_fence_after();
+              const uint64_t v0 =
+                  sw128_mnmajor_desc(sbase + C::offKV + ((2 * tile - 1) % kSlots) * C::kTile, KT * 128);
+              const uint32_t d = tmem + C::colO + (QT == 2 ? t * DP : 0), p = tmem + b * KT;
 #pragma unroll
-          for (int k = 0; k < DP / 16; ++k)
-            tc_mma_f16(tmem + b * KT, sw128_kmajor_desc(q0 + (k >> 2) * (128 * 128) + 32 * (k & 3)),
-                       sw128_kmajor_desc(k0 + (k >> 2) * (KT * 128) + 32 * (k & 3)), idS, k != 0);
-          tc_commit(bar_s + 8 * b);
-          ++ns[t];
-        };
-        auto do_pv = [&](int t, uint32_t vtile) {
-          // P of the tile before the S issued last (QT = 1: one S is ahead).
-          const uint32_t np = QT == 2 ? ns[t] - 1 : vtile;
-          const int b = QT == 2 ? t : (np & 1);
-          if (!wait(bar_p + 8 * b, (QT == 2 ? np : np >> 1) & 1, kDevTimeoutDec)) return;
-          tc_fence_after();
-          const uint32_t v0 = sbase + C::offKV + ((2 * vtile + 1) % kSlots) * C::kTile;
-          const uint32_t d = tmem + C::colO + (QT == 2 ? t * DP : 0);
-#pragma unroll
-          for (int k = 0; k < KT / 16; ++k)
-            tc_mma_f16_ts(d, tmem + b * KT + 8 * k, sw128_mnmajor_desc(v0 + k * 2048, KT * 128), idO,
-                          !(pfirst && k == 0));
-          tc_commit(bar_o + 8 * (QT == 2 ? t : (np & 1)));
-        };
-        auto pv_all = [&](uint32_t vtile) {
-          if (!full_wait(2 * vtile + 1)) return;
-          for (int t = 0; t < pnt && ok; ++t) do_pv(t, vtile);
-          tc_commit(empty + 8 * ((2 * vtile + 1) % kSlots));
-          pend = false;
-        };
-        while (ok && next_one()) {
-          const int nt = tiles(g);
-          for (int u = 0; u < g.take && ok; ++u, ++tile) {
-            if (u == 0 && pend) pv_all(tile - 1);  // the item before is finished first
-            if (!ok || !full_wait(2 * tile)) break;
-            if (QT == 2 && pend) {
-              if (!full_wait(2 * tile - 1)) break;
-              for (int t = 0; t < nt && ok; ++t) {
-                do_pv(t, tile - 1);
-                if (ok) do_s(t, false);
-              }
-              tc_commit(empty + 8 * ((2 * tile - 1) % kSlots));
+              for (int k = 0; k < KT / 16; ++k)
+                tc_mma_f16_ts(d, p + 8 * k, v0 + k * (2048 >> 4), idO, !(pfirst && k == 0));
+              tc_commit(bar_o + 8 * (QT == 2 ? t : (np & 1)));
             } else {
-              for (int t = 0; t < nt && ok; ++t) do_s(t, u == 0);
+              if (!k_in) wait(full + 8 * ((2 * tile) % kSlots), ((2 * tile) / kSlots) & 1, kDevTimeoutFull);
+              k_in = true;
+              if (u == 0) wait(bar_q + 8 * t, nq[t]++ & 1, kDevTimeoutDec);
+              if (!ok) break;
+              tc_fence_after();
+              const int b = QT == 2 ? t : (ns[0] & 1);
+              const uint64_t k0 = sw128_kmajor_desc(sbase + C::offKV + ((2 * tile) % kSlots) * C::kTile);
+              const uint64_t q0 = sw128_kmajor_desc(sbase + t * C::kQ);
+#pragma unroll
+              for (int k = 0; k < DP / 16; ++k)
+                tc_mma_f16(tmem + b * KT, q0 + (((k >> 2) * (128 * 128) + 32 * (k & 3)) >> 4),
+                           k0 + (((k >> 2) * (KT * 128) + 32 * (k & 3)) >> 4), idS, k != 0);
+              tc_commit(bar_s + 8 * b);
+              ++ns[t];
             }
+          }
+          if (pend) tc_commit(empty + 8 * ((2 * tile - 1) % kSlots));
+          if (more) {
             tc_commit(empty + 8 * ((2 * tile) % kSlots));
-            if (QT == 1 && pend && ok) pv_all(tile - 1);
-            pend = ok;
             pfirst = u == 0;
             pnt = nt;
+            ++u;
+            ++tile;
           }
+          pend = more;
         }
-        if (ok && pend) pv_all(tile - 1);
         // TMEM is given back only when every MMA has finished.
         tc_commit(bar_end);
         volatile int no_abort = 0;
-        mbar_wait(bar_end, 0, status, kDevTimeoutAcc, &no_abort);
+        attn_wait(bar_end, 0, status, kDevTimeoutAcc, &no_abort);
       }
       __syncwarp();
     } else if (role == 1) {
@@ -528,7 +583,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
           const bool ragged = j0 < g.it.lo || j0 + KT > g.it.hi;
           for (int kv = 0; kv < 2; ++kv, ++at) {
             const uint32_t slot = at % kSlots, round = at / kSlots;
-            if (round > 0 && !__all_sync(0xffffffffu, mbar_wait(empty + 8 * slot, (round - 1) & 1, status,
+            if (round > 0 && !__all_sync(0xffffffffu, attn_wait(empty + 8 * slot, (round - 1) & 1, status,
                                                                 kDevTimeoutEmpty, abort))) {
               ok = false;
               break;
@@ -545,7 +600,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       // Drain: the block never exits with a copy still writing its memory.
       for (uint32_t q = at > kSlots ? at - kSlots : 0; q < at; ++q) {
         volatile int no_abort = 0;
-        mbar_wait(full + 8 * (q % kSlots), (q / kSlots) & 1, status, kDevTimeoutFull, &no_abort);
+        attn_wait(full + 8 * (q % kSlots), (q / kSlots) & 1, status, kDevTimeoutFull, &no_abort);
       }
     } else if (role == 2) {
       // ---------------- values that no row sees ----------------
@@ -559,7 +614,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
           const int j0 = (g.it.u0 + g.off + u) * KT;
           if (j0 >= g.it.lo && j0 + KT <= g.it.hi) continue;
           const uint32_t slot = (at + 1) % kSlots;
-          if (!__all_sync(0xffffffffu, mbar_wait(edge + 8 * slot, (phase >> slot) & 1, status,
+          if (!__all_sync(0xffffffffu, attn_wait(edge + 8 * slot, (phase >> slot) & 1, status,
                                                  kDevTimeoutFull, abort))) {
             ok = false;
             break;
@@ -581,7 +636,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       // ---------------- the block's items, ahead of the other warps --------
       for (uint32_t n = 0;; ++n) {
         const uint32_t i = n % kSegs;
-        if (n >= kSegs && !mbar_wait(seg_empty + 8 * i, (n / kSegs - 1) & 1, status, kDevTimeoutEmpty, abort)) break;
+        if (n >= kSegs && !attn_wait(seg_empty + 8 * i, (n / kSegs - 1) & 1, status, kDevTimeoutEmpty, abort)) break;
         const bool more = attn_segment<R, KT, kItemCost>(a, cur, g);
         if (!more) g.take = -1;
         segs[i] = g;
