@@ -110,7 +110,7 @@ int check_size(const nvfp4_attention_desc &d, const nvfp4_attention_batch &b, in
   const double keys = (double)b.max_pages * page_size, rows = (double)b.num_tokens * G;
   const AttnLayout L = attn_layout(d, b, 1);
   auto line = [&](int R, double n, double seqs) {
-    return d.num_kv_heads * (rows / R + seqs) * (n / (R == 256 ? 128 : 64) + 3);
+    return d.num_kv_heads * (rows / R + seqs) * (n / 64 + 3);
   };
   if (rows >= (double)(1ll << 30) || line(L.R1, keys, b.num_seqs) >= 2147483648.0 ||
       (b.prefix_len > 0 && line(L.R0, b.prefix_len, 1) >= 2147483648.0))
@@ -199,7 +199,7 @@ extern "C" int nvfp4_paged_attention(const nvfp4_attention_desc *desc, const nvf
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto pass = [&](int R, const char *what) -> int {
     // A box of the cache map: a page, or as much of it as a key tile takes.
-    const int tile = R == 256 ? 128 : 64, box = cache->page_size < tile ? cache->page_size : tile;
+    const int box = cache->page_size < 64 ? cache->page_size : 64;
     CUtensorMap tk, tv;
     if (!make_cache_map(&tk, cache->k, cache->k_strides, *cache, box) ||
         !make_cache_map(&tv, cache->v, cache->v_strides, *cache, box))

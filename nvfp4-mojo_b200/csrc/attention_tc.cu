@@ -2,13 +2,13 @@
 // a shared prefix) over the paged cache, on the 5th-generation tensor cores.
 //
 // An item is QT tiles of 128 query rows (attention.cuh: the heads of a group
-// share their keys, so 8 heads make a tile of 16 tokens).  Per key tile j and
-// query tile t: S = Q K_j^T into TMEM, a softmax thread per row, P as bf16
-// back into TMEM over S, O += P V_j with P as the TMEM operand and V in its
-// natural token-major layout (MN-major operand).  O stays in TMEM for all of
-// an item.  Up to head size 128 QT = 2 and the two tiles alternate: while one
-// is in its softmax the other has the tensor cores.  Above, O takes half of
-// TMEM: QT = 1 and two S buffers, the next S running under the softmax.
+// share their keys, so 8 heads make a tile of 16 tokens); QT = 2, or 1 above
+// head size 128, where O takes half of TMEM.  Per tile of 64 keys and query
+// tile: S = Q K^T into one of two S buffers in TMEM, a softmax thread per row,
+// P as bf16 back over S, O += P V with P as the TMEM operand and V in its
+// natural token-major layout (MN-major operand).  The next S is issued before
+// the product that waits for P, so a softmax finds its next S ready and its
+// warps never stop; O stays in TMEM for all of an item.
 //   warps 0-3 (and 4-7, QT = 2)  softmax of tile 0 (1), Q into shared memory,
 //                                the rare rescaling of O, the epilogue;
 //   then one warp each           MMA issue (one thread), TMA producer, zeroing
@@ -17,9 +17,12 @@
 // O is rescaled only when a row's maximum has grown by more than 2^8 since
 // the last time (weights then stay below 2^8, exact in the sums' fp32); the
 // reference is the same for sum and product, so the result is not changed.
-// Bound by the tensor cores and, nearly as much, by the exponentials: 2 x 128
-// x 128 of them per 2048 tensor cycles are 2048 cycles of the MUFU.
+// The bound beside the tensor cores is the exponential: 2 x 128 x 64 of them
+// per key tile take the MUFU 1024 cycles, as long as the products take the
+// tensor cores.  So a part of them is computed on the FMA pipe instead.
 #include <cuda_bf16.h>
+
+#include <type_traits>
 
 #include "../../include/nvfp4.h"
 #include "abi_util.h"
@@ -34,24 +37,25 @@ static __device__ int g_attn_tc_status;
 
 namespace {
 
-constexpr int kItemCost = 1;  // of an item's beginning and end, in key tiles
+constexpr int kItemCost = 3;  // of an item's beginning and end, in key tiles
 constexpr int kSegs = 4;      // items that the scheduling warp may be ahead
+constexpr int kPolyOf8 = 2;   // of 8 pairs of exponentials, those on the FMA pipe
+
+constexpr int KT = 64;        // keys per tile
 
 template <int DP>
 struct TcCfg {
   static constexpr int QT = DP <= 128 ? 2 : 1;
   static constexpr int R = 128 * QT;
-  static constexpr int KT = DP <= 128 ? 128 : 64;   // keys per tile
   static constexpr int kTile = KT * DP * 2;         // bytes of a key or value tile
   static constexpr int kQ = 128 * DP * 2;           // bytes of a query tile
-  static constexpr int kSlots = DP == 64 ? 8 : 4;
+  static constexpr int kSlots = DP == 64 ? 16 : DP == 128 ? 9 : 4;
   static constexpr int kSoftWarps = 4 * QT;
   static constexpr int kThreads = (kSoftWarps + 4) * 32;
   static constexpr int offKV = QT * kQ;
-  static constexpr int offStage = offKV + kSlots * kTile;  // 2 KB per softmax warp
-  static constexpr int bytes = offStage + kSoftWarps * 2048 + 1024;
-  // TMEM columns: S tiles (tile t, or buffer t when QT = 1), then O.
-  static constexpr int colO = 2 * KT;
+  static constexpr int bytes = offKV + kSlots * kTile + 1024;
+  // TMEM columns: two S buffers per query tile, then O of each.
+  static constexpr int colO = 2 * QT * KT;
   static constexpr int cols = 512;
 };
 
@@ -66,39 +70,67 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[
       "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
+// 16 lanes x 16 columns: lane l gets columns 8 k + 2 (l % 4) + {0, 1} of rows
+// l / 4 (r[4 k], r[4 k + 1]) and l / 4 + 8 (r[4 k + 2], r[4 k + 3]).
+__device__ __forceinline__ void tmem_ld_16x256_x2(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// D[tmem] (+)= A[tmem] * B[smem].
-__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc,
-                                              uint32_t accumulate) {
+// The warp that issues the MMAs runs as one, its operands the same in every
+// lane (they belong in uniform registers).  Four k-steps of 16 go into one
+// block of instructions, predicated on one elected lane without a branch
+// around them: an operand that has to be made uniform for each MMA, or a
+// branch, costs as much as the MMA takes the tensor cores.
+constexpr uint32_t kDescHi = (1024u >> 4) | 1u << 14 | 2u << 29;  // 1024-byte groups, version, 128-byte swizzle
+
+// D[tmem] (+)= A[smem] B[smem]^T over 64 columns; alo, blo: low words of the
+// operands' descriptors, a k-step 32 bytes further along the swizzled rows.
+__device__ __forceinline__ void mma_ss4(uint32_t d, uint32_t alo, uint32_t blo, uint32_t idesc, uint32_t acc) {
+#define NVFP4_SS_STEP(off, pred)                        \
+  "add.u32 x, %1, " off ";\n\tadd.u32 y, %2, " off ";\n\t" \
+  "mov.b64 ad, {x, %5};\n\tmov.b64 bd, {y, %5};\n\t"      \
+  "@q tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %3, " pred ";\n\t"
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p, q, one;\n\t.reg .b32 x, y;\n\t.reg .b64 ad, bd;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.u32 one, 0, 0;\n\t" NVFP4_SS_STEP("0", "p") NVFP4_SS_STEP("2", "one")
+          NVFP4_SS_STEP("4", "one") NVFP4_SS_STEP("6", "one") "}" ::"r"(d),
+      "r"(alo), "r"(blo), "r"(idesc), "r"(acc), "r"(kDescHi)
+      : "memory");
+#undef NVFP4_SS_STEP
+}
+// D[tmem] (+)= A[tmem] B[smem] over 64 tokens: 8 columns of A and 2048 bytes
+// of B a k-step.
+__device__ __forceinline__ void mma_ts4(uint32_t d, uint32_t a, uint32_t blo, uint32_t idesc, uint32_t acc) {
+#define NVFP4_TS_STEP(aoff, boff, pred)                                  \
+  "add.u32 x, %1, " aoff ";\n\tadd.u32 y, %2, " boff ";\n\tmov.b64 bd, {y, %5};\n\t" \
+  "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x], bd, %3, " pred ";\n\t"
+  asm volatile(
+      "{\n\t.reg .pred p, q, one;\n\t.reg .b32 x, y;\n\t.reg .b64 bd;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.u32 one, 0, 0;\n\t" NVFP4_TS_STEP("0", "0", "p")
+          NVFP4_TS_STEP("8", "128", "one") NVFP4_TS_STEP("16", "256", "one") NVFP4_TS_STEP("24", "384", "one") "}" ::"r"(d),
+      "r"(a), "r"(blo), "r"(idesc), "r"(acc), "r"(kDescHi)
+      : "memory");
+#undef NVFP4_TS_STEP
+}
+__device__ __forceinline__ void commit_to(uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
       : "memory");
 }
 
-// Values [token][d], 64 columns of 128 swizzled bytes per token, as the
-// MN-major B operand: 64-column blocks `block` bytes apart (leading offset),
-// groups of 8 tokens 1024 bytes apart (stride offset).
-__device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t saddr, uint32_t block) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
-  d |= static_cast<uint64_t>(block >> 4) << 16;
-  d |= static_cast<uint64_t>(1024 >> 4) << 32;
-  d |= static_cast<uint64_t>(1) << 46;
-  d |= static_cast<uint64_t>(2) << 61;
-  return d;
+// Low word of a descriptor.  Keys and queries are K-major (the leading offset
+// is not used, 16 bytes); values [token][d], 64 columns of 128 swizzled bytes
+// per token, are an MN-major B operand: 64-column blocks KT * 128 bytes apart
+// (leading offset), groups of 8 tokens 1024 bytes apart (stride offset).
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lead) {
+  return ((saddr & 0x3FFFFu) >> 4) | (lead >> 4) << 16;
 }
 constexpr uint32_t kTransposeB = 1u << 16;
 
@@ -116,17 +148,67 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// Two fp32 at a time.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t r, float &x, float &y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x of a pair on the FMA pipe, x <= 9: x = n + f with n the nearest whole
+// number (from adding 1.5 * 2^23), 2^f on [-1/2, 1/2] by a polynomial of
+// degree 4 fitted for the least relative error (2.6e-6), n added to the
+// exponent.  x below -126 gives a weight of at most 2^-126.
+__device__ __forceinline__ void exp2_pair(uint64_t x2, float &p0, float &p1) {
+  float x0, x1;
+  unpair(x2, x0, x1);
+  x2 = pair(fmaxf(x0, -126.0f), fmaxf(x1, -126.0f));
+  const uint64_t t2 = add2(x2, pair(12582912.0f, 12582912.0f));
+  const uint64_t n2 = add2(t2, pair(-12582912.0f, -12582912.0f));
+  const uint64_t f2 = fma2(n2, pair(-1.0f, -1.0f), x2);
+  uint64_t r = fma2(f2, pair(0.009570101276040077f, 0.009570101276040077f),
+                    pair(0.05591786280274391f, 0.05591786280274391f));
+  r = fma2(r, f2, pair(0.240247443318367f, 0.240247443318367f));
+  r = fma2(r, f2, pair(0.6931217908859253f, 0.6931217908859253f));
+  r = fma2(r, f2, pair(0.9999992847442627f, 0.9999992847442627f));
+  float t0, t1, r0, r1;
+  unpair(t2, t0, t1);
+  unpair(r, r0, r1);
+  p0 = __int_as_float(__float_as_int(r0) + (__float_as_int(t0) << 23));
+  p1 = __int_as_float(__float_as_int(r1) + (__float_as_int(t1) << 23));
+}
+
+// The largest of three; not a number if one of them is.
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+
 template <int DP, bool MOD>
 __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
     attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const __grid_constant__ AttnArgs a) {
   using C = TcCfg<DP>;
-  constexpr int QT = C::QT, R = C::R, KT = C::KT, kSlots = C::kSlots;
+  constexpr int QT = C::QT, R = C::R, kSlots = C::kSlots;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                               ~static_cast<uintptr_t>(1023));
   __shared__ AttnPlanSmem plan;
-  __shared__ uint64_t bars[3 * kSlots + 9 + 2 * kSegs];
+  __shared__ uint64_t bars[3 * kSlots + 15 + 2 * kSegs];
   __shared__ AttnSegment segs[kSegs];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -135,10 +217,12 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
   const uint32_t empty = full + 8 * kSlots;   // the slot's MMAs are done
   const uint32_t edge = empty + 8 * kSlots;   // a value tile landed that needs zeroing
   const uint32_t bar_q = edge + 8 * kSlots;   // [2] queries of tile t in shared memory
-  const uint32_t bar_s = bar_q + 16;          // [2] S ready
-  const uint32_t bar_p = bar_s + 16;          // [2] P written (and O rescaled)
-  const uint32_t bar_o = bar_p + 16;          // [2] P V done (tile t; QT = 1: even and odd products)
-  const uint32_t bar_end = bar_o + 16;
+  // Of query tile t and the parity x of its key tiles' count: [2 t + x].  Two
+  // of each, so that none has more than one phase outstanding.
+  const uint32_t bar_s = bar_q + 16;          // S ready
+  const uint32_t bar_p = bar_s + 32;          // P written (and O rescaled)
+  const uint32_t bar_o = bar_p + 32;          // P V done
+  const uint32_t bar_end = bar_o + 32;
   const uint32_t seg_full = bar_end + 8;      // [kSegs] the block's next items
   const uint32_t seg_empty = seg_full + 8 * kSegs;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -150,11 +234,12 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       mbar_init(empty + 8 * i, 1);
       mbar_init(edge + 8 * i, 1);
     }
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(bar_q + 8 * t, 4);
-      mbar_init(bar_s + 8 * t, 1);
-      mbar_init(bar_p + 8 * t, 4);
-      mbar_init(bar_o + 8 * t, 1);
+    mbar_init(bar_q, 4);
+    mbar_init(bar_q + 8, 4);
+    for (int x = 0; x < 4; ++x) {
+      mbar_init(bar_s + 8 * x, 1);
+      mbar_init(bar_p + 8 * x, 4);
+      mbar_init(bar_o + 8 * x, 1);
     }
     mbar_init(bar_end, 1);
     for (int i = 0; i < kSegs; ++i) {
@@ -202,23 +287,24 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
     const int t = warp >> 2, wq = warp & 3;            // tile, lane quarter
     const int my = t * 128 + wq * 32 + lane;           // row within the item
     const uint32_t lanes = static_cast<uint32_t>(32 * wq) << 16;
-    const uint32_t tO = tmem + lanes + C::colO + (QT == 2 ? t * DP : 0);
+    const uint32_t tO = tmem + lanes + C::colO + t * DP;
     uint8_t *Q = smem + t * C::kQ;
-    const float sl2 = a.scale * kLog2e;
+    const float c2 = MOD ? 1.0f : a.scale * kLog2e;
+    const uint64_t c22 = pair(c2, c2);
 
-    // This warp's 32 rows of Q, 16-byte chunks swizzled as the MMA reads them;
-    // rows and columns beyond the item's or the head's are zeros.
-    auto load_q = [&]() {
-      const AttnSegment &x = g;
-      const int row = x.rb * R + my;
+    // This warp's 32 rows of the next item's Q, 16-byte chunks swizzled as the
+    // MMA reads them; rows and columns beyond the item's or the head's are
+    // zeros.  Started here, handed over in q_done().
+    auto q_start = [&]() {
+      const int row = g.rb * R + my;
       const __nv_bfloat16 *src = nullptr;
-      if (row < x.s.ql * a.G) {
+      if (row < g.s.ql * a.G) {
         const int i = row / a.G;
-        src = a.q + (int64_t)(x.s.tok0 + i) * a.q_ts + (int64_t)(x.h * a.G + row - i * a.G) * a.q_hs;
+        src = a.q + (int64_t)(g.s.tok0 + i) * a.q_ts + (int64_t)(g.h * a.G + row - i * a.G) * a.q_hs;
       }
       constexpr int CH = DP / 8, RPI = 32 / CH;  // chunks per row, rows per warp step
       const int c = lane % CH;
-#pragma unroll
+#pragma unroll 4
       for (int r0 = 0; r0 < 32; r0 += RPI) {
         const int r = r0 + lane / CH;
         const uint64_t p = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(src), r);
@@ -229,76 +315,90 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
                      "l"(on ? p + 16 * c : reinterpret_cast<uint64_t>(a.q)), "r"(on ? 16 : 0)
                      : "memory");
       }
+    };
+    auto q_done = [&]() {
       asm volatile("cp.async.wait_all;" ::: "memory");
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_q + 8 * t);
     };
 
-    // Product i of this query tile is in.  With QT = 1 the S that is ready
-    // may be ahead of the last two products, so these alternate between two
-    // barriers: each then has at most one phase outstanding.
-    auto o_wait = [&](uint32_t i) {
-      return QT == 2 ? attn_wait(bar_o + 8 * t, i & 1, status, kDevTimeoutAcc, abort)
-                     : attn_wait(bar_o + 8 * (i & 1), (i >> 1) & 1, status, kDevTimeoutAcc, abort);
-    };
     uint32_t n = 0;  // key tiles of this query tile so far
     bool have = next_seg(), ok = true;
-    if (have && g.take > 0 && t < tiles(g)) load_q();
+    bool fetch = have && g.take > 0 && t < tiles(g);
+    if (fetch) {
+      q_start();
+      q_done();
+    }
     while (have && ok) {
       const bool mine = t < tiles(g);
+      const int take = g.take, slot = g.slot, j_first = (g.it.u0 + g.off) * KT;
       const int row = g.rb * R + my;
-      const bool in = row < g.s.ql * a.G;
-      AttnRow ar = {};
+      const bool in = mine && row < g.s.ql * a.G;
+      if (g.last_part >= 0 && threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(g.b, g.h, g.rb, g.last_part);
+      AttnRow ar = attn_row(a, g.s, g.h, in ? row : 0);
+      if (!in) ar.lo = ar.hi = 0;
       float m = -INFINITY, l = 0.0f;
-      if (mine) {
-        ar = attn_row(a, g.s, g.h, in ? row : 0);
-        if (!in) ar.lo = ar.hi = 0;
+      if (mine && take > 0) {
+        // Keys that all rows of the warp see need no mask.
+        const int lo_all = __reduce_max_sync(0xffffffffu, ar.lo), hi_all = __reduce_min_sync(0xffffffffu, ar.hi);
         const float slope = MOD && a.slopes ? a.slopes[ar.head] * kLog2e : 0.0f;
         const int pos = ar.pos - (a.prefix_pass ? 0 : a.prefix_len);
-        for (int u = 0; u < g.take; ++u, ++n) {
-          const int j0 = (g.it.u0 + g.off + u) * KT;
-          const int b = QT == 2 ? t : (n & 1);
-          const uint32_t ph = QT == 2 ? n & 1 : (n >> 1) & 1;
-          const uint32_t tS = tmem + lanes + b * KT;
-          if (!__all_sync(0xffffffffu, attn_wait(bar_s + 8 * b, ph, status, kDevTimeoutAcc, abort))) {
+#pragma unroll 1
+        for (int u = 0; u < take; ++u, ++n) {
+          const int j0 = j_first + u * KT;
+          const uint32_t x = 2 * t + (n & 1);
+          const uint32_t tS = tmem + lanes + x * KT;
+          if (!__all_sync(0xffffffffu, attn_wait(bar_s + 8 * x, (n >> 1) & 1, status, kDevTimeoutAcc, abort))) {
             ok = false;
             break;
           }
           tc_fence_after();
-          uint32_t raw[KT / 32][32];
-#pragma unroll
-          for (int c = 0; c < KT / 32; ++c) tmem_ld_32x32b_x32(tS + 32 * c, raw[c]);
+          uint32_t raw[2][32];
+          tmem_ld_32x32b_x32(tS, raw[0]);
+          tmem_ld_32x32b_x32(tS + 32, raw[1]);
+          if (u == take - 1) {  // every S of the item is done: its Q may go
+            have = next_seg();
+            fetch = have && g.take > 0 && t < tiles(g);
+            if (fetch) q_start();
+          }
           tmem_ld_wait();
           float s[KT];
 #pragma unroll
           for (int c = 0; c < KT; ++c) s[c] = __uint_as_float(raw[c / 32][c % 32]);
           if constexpr (MOD) {
+            const float cap2 = 2.0f * kLog2e / a.softcap * a.scale;
 #pragma unroll
             for (int c = 0; c < KT; ++c) {
-              float v = s[c] * a.scale;
-              if (a.softcap > 0.0f)  // cap tanh(v / cap)
-                v = a.softcap - __fdividef(2.0f * a.softcap, 1.0f + ex2(v * (2.0f * kLog2e / a.softcap)));
+              float v;
+              if (a.softcap > 0.0f)  // cap tanh(scale s / cap)
+                v = a.softcap - __fdividef(2.0f * a.softcap, 1.0f + ex2(s[c] * cap2));
+              else
+                v = s[c] * a.scale;
               s[c] = fmaf(v, kLog2e, -slope * fabsf((float)(pos - j0 - c)));
             }
           }
-          const float c2 = MOD ? 1.0f : sl2;
-          if (__any_sync(0xffffffffu, j0 < ar.lo || j0 + KT > ar.hi)) {
+          if (j0 < lo_all || j0 + KT > hi_all) {
             const int lo = ar.lo - j0, hi = ar.hi - j0;
 #pragma unroll
             for (int c = 0; c < KT; ++c) s[c] = c >= lo && c < hi ? s[c] : -INFINITY;
           }
           float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-          for (int c = 4; c < KT; c += 4)
+          for (int c = 4; c < KT - 4; c += 8)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], s[c + i]);
-          const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c2;
+            for (int i = 0; i < 4; ++i) top[i] = max3(top[i], s[c + i], s[c + 4 + i]);
+          top[0] = max3(top[0], s[KT - 4], s[KT - 3]);
+          top[1] = max3(top[1], s[KT - 2], s[KT - 1]);
+          const float mx = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * c2;
+          if (!(mx < INFINITY)) l = NAN;  // a score that is infinite or not a number
           const bool grow = mx > m + 8.0f;
           if (__any_sync(0xffffffffu, grow)) {
             const float mn = grow ? mx : m;
             if (u > 0) {  // O of the tiles before, once they are all in
-              if (!__all_sync(0xffffffffu, o_wait(n - 1))) {
+              const uint32_t y = 2 * t + ((n - 1) & 1);
+              if (!__all_sync(0xffffffffu, attn_wait(bar_o + 8 * y, ((n - 1) >> 1) & 1, status, kDevTimeoutAcc,
+                                                     abort))) {
                 ok = false;
                 break;
               }
@@ -318,144 +418,146 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
             m = mn;
           }
           const float mu = m == -INFINITY ? 0.0f : m;
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const uint64_t nm2 = pair(-mu, -mu);
+          uint64_t sum[2] = {0, 0};
+          uint32_t p[32];
 #pragma unroll
-          for (int c = 0; c < KT; c += 64) {
-            uint32_t p[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float x = ex2(fmaf(s[c + 2 * i], c2, -mu)), y = ex2(fmaf(s[c + 2 * i + 1], c2, -mu));
-              sum[(2 * i) & 3] += x;
-              sum[(2 * i + 1) & 3] += y;
-              // Rounded to bf16 for the second product only; the sum keeps
-              // the unrounded weights.
-              p[i] = pack_bf16(x, y);
+          for (int i = 0; i < 32; ++i) {
+            const uint64_t e2 = fma2(pair(s[2 * i], s[2 * i + 1]), c22, nm2);
+            float e0, e1;
+            if (i % 8 < kPolyOf8) {
+              exp2_pair(e2, e0, e1);
+            } else {
+              unpair(e2, e0, e1);
+              e0 = ex2(e0);
+              e1 = ex2(e1);
             }
-            tmem_st_x32(tS + c / 2, p);
+            sum[i & 1] = add2(sum[i & 1], pair(e0, e1));
+            // Rounded to bf16 for the second product only; the sum keeps the
+            // unrounded weights.
+            p[i] = pack_bf16(e0, e1);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_st_x32(tS, p);
+          float l0, l1;
+          unpair(add2(sum[0], sum[1]), l0, l1);
+          l += l0 + l1;
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar_p + 8 * b);
+          if (lane == 0) mbar_arrive(bar_p + 8 * x);
         }
-      }
-      if (!ok) break;
-      // The next item's queries first (this item's S are all done), so that
-      // its first S runs under this epilogue.
-      const int e_take = g.take, e_slot = g.slot, e_rb = g.rb;
-      if (g.last_part >= 0 && threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(g.b, g.h, g.rb, g.last_part);
-      const int left = min(g.s.ql * a.G - e_rb * R - t * 128 - wq * 32, 32);  // this warp's rows in use
-      have = next_seg();
-      if (have && g.take > 0 && t < tiles(g)) load_q();
-      if (!mine) continue;
-      if (e_take > 0) {
-        if (!__all_sync(0xffffffffu, o_wait(n - 1))) break;
+        if (!ok) break;
+        if (fetch) q_done();
+        const uint32_t y = 2 * t + ((n - 1) & 1);
+        if (!__all_sync(0xffffffffu, attn_wait(bar_o + 8 * y, ((n - 1) >> 1) & 1, status, kDevTimeoutAcc, abort)))
+          break;
         tc_fence_after();
+      } else {
+        have = next_seg();
+        fetch = have && g.take > 0 && t < tiles(g);
+        if (fetch) {
+          q_start();
+          q_done();
+        }
       }
-      // O by way of shared memory, 16 columns at a time, so that 4 lanes
-      // store 16 columns of a row side by side.
+      if (!mine) continue;
+      if (m == -INFINITY) l = 0.0f;  // nothing seen: masked weights on the FMA pipe are not quite zero
+
+      // ---- epilogue: straight from TMEM (shared memory is busy with the other
+      // tile's MMAs), 16 rows by 16 columns at a time in the shape where 4
+      // lanes hold 8 columns of a row side by side.  The loops stay rolled: this
+      // code runs once per item and would come from L2 line by line.
       AttnFinish f = {};
-      if (in && e_slot < 0) {
-        f = attn_finish(a, ar, m, l);
-        attn_store_lse(a, f);
+      if (in) {
+        if (slot < 0) {
+          f = attn_finish(a, ar, m, l);
+          attn_store_lse(a, f);
+        } else {
+          a.part_ml[(int64_t)slot * R + my] = make_float2(m, l);
+          f.so = 1.0f;
+        }
       }
-      if (in && e_slot >= 0) a.part_ml[(int64_t)e_slot * R + my] = make_float2(m, l);
-      // This lane's 4 rows of a step, at its 4 columns.
-      const int64_t id = in ? (int64_t)ar.token * a.Hq + ar.head : 0;
-      const float so = e_slot < 0 ? f.so : 1.0f;
-      int64_t at[4], gat[4], pat[4];
-      float sp[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int src = 8 * i + (lane >> 2);
-        const int tok = __shfl_sync(0xffffffffu, ar.token, src), head = __shfl_sync(0xffffffffu, ar.head, src);
-        pat[i] = __shfl_sync(0xffffffffu, id, src) * DP;
-        if (e_slot >= 0) at[i] = ((int64_t)e_slot * R + t * 128 + wq * 32 + src) * DP;
-        else if (a.prefix_pass) at[i] = pat[i];
-        else at[i] = tok * a.o_ts + head * a.o_hs;
-        gat[i] = tok * a.g_ts + head * a.g_hs;
-        sp[i] = __shfl_sync(0xffffffffu, f.sp, src);
-      }
-      const bool to_f32 = e_slot >= 0 || a.prefix_pass, joins = !to_f32 && a.prev_o, gates = !to_f32 && a.gate;
-      float *f32 = e_slot >= 0 ? a.part_o : a.prev_o;
-      const uint32_t stage = sbase + C::offStage + warp * 2048;
-      const uint32_t st_w = stage + lane * 64, x_w = (lane >> 1) & 3;
-      // The gates come a step ahead of their use.
-      auto load_gates = [&](uint2 (&v)[4], int d) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (gates && 8 * i + (lane >> 2) < left && d < a.D)
-            v[i] = *reinterpret_cast<const uint2 *>(a.gate + gat[i] + d);
-      };
-      uint2 gv[4] = {}, gn[4] = {};
-      load_gates(gn, 4 * (lane & 3));
+      // MODE 0: fp32 rows (a part, or the prefix pass); 1: bf16 rows; 2: bf16
+      // rows with a gate or the prefix's part joined.  A loop of its own each,
+      // so that it runs without branches.
+      auto store_rows = [&](auto mode) {
+        constexpr int MODE = decltype(mode)::value;
 #pragma unroll 1
-      for (int c = 0; c < DP; c += 16) {
-        const int d = c + 4 * (lane & 3);
-        uint32_t o[16] = {};
-        if (e_take > 0) tmem_ld_x16(tO + c, o);
+        for (int h = 0; h < 32; h += 16) {
+          float so[2], sp[2];
+          char *dst[2];  // this lane's first column of its two rows
+          const char *gate[2], *prev[2];
+          bool on[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) gv[i] = gn[i];
-        if (c + 16 < DP) load_gates(gn, d + 16);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float v[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) v[x] = so == 0.0f ? 0.0f : __uint_as_float(o[4 * i + x]) * so;
-          asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(st_w + ((i ^ x_w) << 4)), "f"(v[0]),
-                       "f"(v[1]), "f"(v[2]), "f"(v[3])
-                       : "memory");
-        }
-        __syncwarp();
-        float4 x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 8 * i + (lane >> 2);
-          asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
-                       : "=f"(x[i].x), "=f"(x[i].y), "=f"(x[i].z), "=f"(x[i].w)
-                       : "r"(stage + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4))
-                       : "memory");
-        }
-        __syncwarp();
-        if (d >= a.D) continue;
-        if (to_f32) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (8 * i + (lane >> 2) < left) *reinterpret_cast<float4 *>(f32 + at[i] + d) = x[i];
-          continue;
-        }
-        if (joins) {
-          float4 p[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            p[i] = make_float4(0, 0, 0, 0);
-            if (sp[i] != 0.0f) p[i] = *reinterpret_cast<const float4 *>(a.prev_o + pat[i] + d);
+          for (int i = 0; i < 2; ++i) {
+            const int src = h + 8 * i + (lane >> 2);
+            const int tok = __shfl_sync(0xffffffffu, ar.token, src), head = __shfl_sync(0xffffffffu, ar.head, src);
+            const int64_t id = ((int64_t)tok * a.Hq + head) * DP + 2 * (lane & 3);
+            on[i] = __shfl_sync(0xffffffffu, (int)in, src);
+            so[i] = __shfl_sync(0xffffffffu, f.so, src);
+            if constexpr (MODE == 0) {
+              const int64_t pid = ((int64_t)slot * R + t * 128 + wq * 32 + src) * DP + 2 * (lane & 3);
+              dst[i] = reinterpret_cast<char *>(slot >= 0 ? a.part_o + pid : a.prev_o + id);
+            } else {
+              dst[i] = reinterpret_cast<char *>(a.out + tok * a.o_ts + head * a.o_hs + 2 * (lane & 3));
+            }
+            if constexpr (MODE == 2) {
+              sp[i] = __shfl_sync(0xffffffffu, f.sp, src);
+              prev[i] = reinterpret_cast<const char *>(a.prev_o + id);
+              gate[i] = reinterpret_cast<const char *>(a.gate + tok * a.g_ts + head * a.g_hs + 2 * (lane & 3));
+            }
           }
+          const int cols = MODE == 0 ? DP : a.D;
+#pragma unroll 1
+          for (int c = 0; c < cols; c += 16) {
+            // Per row i: columns c + 8 k + 2 (lane % 4) + {0, 1}.
+            uint32_t o[8] = {}, w[2][2] = {};
+            float2 p[2][2] = {};
+            if (take > 0) tmem_ld_16x256_x2(tO + ((uint32_t)h << 16) + c, o);
+            if constexpr (MODE == 2) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x[i].x = fmaf(p[i].x, sp[i], x[i].x);
-            x[i].y = fmaf(p[i].y, sp[i], x[i].y);
-            x[i].z = fmaf(p[i].z, sp[i], x[i].z);
-            x[i].w = fmaf(p[i].w, sp[i], x[i].w);
+              for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  if (a.gate && on[i] && c + 8 * k < cols)
+                    w[i][k] = *reinterpret_cast<const uint32_t *>(gate[i] + 2 * (c + 8 * k));
+                  if (sp[i] != 0.0f) p[i][k] = *reinterpret_cast<const float2 *>(prev[i] + 4 * (c + 8 * k));
+                }
+            }
+            tmem_ld_wait();
+            float x[2][2][2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const float v = __uint_as_float(o[4 * k + 2 * i + e]);
+                  x[i][k][e] = so[i] == 0.0f ? 0.0f : v * so[i];
+                  if constexpr (MODE == 2) {
+                    x[i][k][e] = fmaf(e ? p[i][k].y : p[i][k].x, sp[i], x[i][k][e]);
+                    const float g =
+                        sigmoidf(__uint_as_float(e ? w[i][k] & 0xffff0000u : w[i][k] << 16));
+                    x[i][k][e] *= a.gate ? g : 1.0f;
+                  }
+                }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                if constexpr (MODE == 0) {
+                  if (on[i]) *reinterpret_cast<float2 *>(dst[i] + 4 * (c + 8 * k)) = make_float2(x[i][k][0], x[i][k][1]);
+                } else {
+                  if (on[i] && c + 8 * k < cols)
+                    *reinterpret_cast<uint32_t *>(dst[i] + 2 * (c + 8 * k)) = pack_bf16(x[i][k][0], x[i][k][1]);
+                }
+              }
           }
         }
-        if (gates) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x[i].x *= sigmoidf(__uint_as_float(gv[i].x << 16));
-            x[i].y *= sigmoidf(__uint_as_float(gv[i].x & 0xffff0000u));
-            x[i].z *= sigmoidf(__uint_as_float(gv[i].y << 16));
-            x[i].w *= sigmoidf(__uint_as_float(gv[i].y & 0xffff0000u));
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (8 * i + (lane >> 2) < left)
-            *reinterpret_cast<uint2 *>(a.out + at[i] + d) =
-                make_uint2(pack_bf16(x[i].x, x[i].y), pack_bf16(x[i].z, x[i].w));
-      }
+      };
+      if (slot >= 0 || a.prefix_pass) store_rows(std::integral_constant<int, 0>());
+      else if (!a.gate && !a.prev_o) store_rows(std::integral_constant<int, 1>());
+      else store_rows(std::integral_constant<int, 2>());
       tc_fence_before();
     }
   } else {
@@ -463,99 +565,83 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
     const int role = warp - C::kSoftWarps;
     if (role == 0) {
       // ---------------- MMA issue ----------------
-      if (lane == 0) {
-        constexpr uint32_t idS = idesc_bf16_f32(128, KT);
-        constexpr uint32_t idO = idesc_bf16_f32(128, DP) | kTransposeB;
-        bool ok = true;
-        uint32_t tile = 0;       // key tiles so far: K in slot 2 tile, V in 2 tile + 1
-        uint32_t ns[2] = {0, 0}; // S issued per query tile
-        uint32_t nq[2] = {0, 0}; // queries awaited per query tile
-        bool pend = false, pfirst = false, more = true;
-        int pnt = 0, u = 0, nt = 0;  // pnt, pfirst: of the pending P V
-        g.take = 0;
-        auto wait = [&](uint32_t bar, uint32_t ph, int code) {
-          ok = ok && attn_wait(bar, ph, status, code, abort);
-        };
-        while (ok && (more || pend)) {
-          // The next key tile, if any; P V of the tile before it is pending.
-          if (more && u == g.take) {
-            do {
-              const uint32_t i = nseg % kSegs;
-              wait(seg_full + 8 * i, (nseg / kSegs) & 1, kDevTimeoutDec);
-              if (!ok) break;
-              g = segs[i];
-              mbar_arrive(seg_empty + 8 * i);
-              ++nseg;
-            } while (g.take == 0);
-            if (!ok) break;
-            more = g.take > 0;
-            u = 0;
-            nt = tiles(g);
-          }
-          // In which order: bits 0, 1 the query tile, bit 2 a P V, bit 3 none.
-          // Within an item QT = 2 alternates P V and S of the two tiles and
-          // QT = 1 keeps one S ahead; an item's last P V come before the next
-          // item's S, which may wait for its queries.
-          uint32_t ops;
-          const bool inner = more && pend && u > 0;
-          if (QT == 2) ops = inner ? 0x1504 : 0x1054;
-          else ops = inner ? 0x8840 : 0x8804;
-          if (!pend || pnt < 2) ops |= QT == 2 ? (inner ? 0x0800 : 0x0080) : 0;
-          if (!pend) ops |= QT == 2 ? 0x0008 : (inner ? 0x0080 : 0x0008);
-          if (!more) ops |= QT == 2 ? 0x8800 : 0x0080;
-          if (more && nt < 2 && QT == 2) ops |= 0x8000;
-          bool v_in = false, k_in = false;
-#pragma unroll 1
-          for (; ops != 0x8888 && ok; ops = (ops >> 4) | 0x8000) {
-            const int op = ops & 15, t = op & 3;
-            if (op & 8) continue;
-            if (op & 4) {
-              if (!v_in) wait(full + 8 * ((2 * tile - 1) % kSlots), ((2 * tile - 1) / kSlots) & 1, kDevTimeoutFull);
-              v_in = true;
-              const uint32_t np = QT == 2 ? ns[t] - 1 : tile - 1;  // this P V's count
-              const int b = QT == 2 ? t : (np & 1);
-              wait(bar_p + 8 * b, (QT == 2 ? np : np >> 1) & 1, kDevTimeoutDec);
-              if (!ok) break;
-              tc_fence_after();
-              const uint64_t v0 =
-                  sw128_mnmajor_desc(sbase + C::offKV + ((2 * tile - 1) % kSlots) * C::kTile, KT * 128);
-              const uint32_t d = tmem + C::colO + (QT == 2 ? t * DP : 0), p = tmem + b * KT;
+      constexpr uint32_t idS = idesc_bf16_f32(128, KT);
+      constexpr uint32_t idO = idesc_bf16_f32(128, DP) | kTransposeB;
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), sb = __shfl_sync(0xffffffffu, sbase, 0);
+      const uint32_t qd = desc_lo(sb, 16), kd = desc_lo(sb + C::offKV, 16), vd = desc_lo(sb + C::offKV, KT * 128);
+      bool ok = true;
+      // Key tiles so far and the slot of the next one's K (its V is in the
+      // slot after) with the parity of that slot's round.
+      uint32_t slot = 0, round = 0, vslot = 0, vround = 0;
+      // Per query tile: S issued, P V issued, queries awaited.
+      uint32_t ns[2] = {0, 0}, np[2] = {0, 0}, nq[2] = {0, 0};
+      bool pend = false, pfirst = false, more = true;
+      int pnt = 0, u = 0, take = 0, nt = 0;  // pnt, pfirst: of the pending P V
+      auto wait = [&](uint32_t bar, uint32_t ph, int code) {
+        ok = ok && __all_sync(0xffffffffu, attn_wait(bar, ph, status, code, abort));
+      };
+      auto s_of = [&](int t) {
+        if (u == 0) wait(bar_q + 8 * t, nq[t]++ & 1, kDevTimeoutDec);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t x = 2 * t + (ns[t]++ & 1);
+        const uint32_t k0 = kd + slot * (C::kTile >> 4), q0 = qd + t * (C::kQ >> 4);
 #pragma unroll
-              for (int k = 0; k < KT / 16; ++k)
-                tc_mma_f16_ts(d, p + 8 * k, v0 + k * (2048 >> 4), idO, !(pfirst && k == 0));
-              tc_commit(bar_o + 8 * (QT == 2 ? t : (np & 1)));
-            } else {
-              if (!k_in) wait(full + 8 * ((2 * tile) % kSlots), ((2 * tile) / kSlots) & 1, kDevTimeoutFull);
-              k_in = true;
-              if (u == 0) wait(bar_q + 8 * t, nq[t]++ & 1, kDevTimeoutDec);
-              if (!ok) break;
-              tc_fence_after();
-              const int b = QT == 2 ? t : (ns[0] & 1);
-              const uint64_t k0 = sw128_kmajor_desc(sbase + C::offKV + ((2 * tile) % kSlots) * C::kTile);
-              const uint64_t q0 = sw128_kmajor_desc(sbase + t * C::kQ);
-#pragma unroll
-              for (int k = 0; k < DP / 16; ++k)
-                tc_mma_f16(tmem + b * KT, q0 + (((k >> 2) * (128 * 128) + 32 * (k & 3)) >> 4),
-                           k0 + (((k >> 2) * (KT * 128) + 32 * (k & 3)) >> 4), idS, k != 0);
-              tc_commit(bar_s + 8 * b);
-              ++ns[t];
-            }
-          }
-          if (pend) tc_commit(empty + 8 * ((2 * tile - 1) % kSlots));
-          if (more) {
-            tc_commit(empty + 8 * ((2 * tile) % kSlots));
-            pfirst = u == 0;
-            pnt = nt;
-            ++u;
-            ++tile;
-          }
-          pend = more;
+        for (int hf = 0; hf < DP / 64; ++hf)
+          mma_ss4(tm + x * KT, q0 + hf * (128 * 128 >> 4), k0 + hf * (KT * 128 >> 4), idS, hf != 0);
+        commit_to(bar_s + 8 * x);
+      };
+      auto pv_of = [&](int t) {
+        const uint32_t x = 2 * t + (np[t] & 1);
+        wait(bar_p + 8 * x, (np[t] >> 1) & 1, kDevTimeoutDec);
+        ++np[t];
+        if (!ok) return;
+        tc_fence_after();
+        mma_ts4(tm + C::colO + t * DP, tm + x * KT, vd + vslot * (C::kTile >> 4), idO, !pfirst);
+        commit_to(bar_o + 8 * x);
+      };
+      auto s_all = [&]() {
+        wait(full + 8 * slot, round & 1, kDevTimeoutFull);
+        if (ok) s_of(0);
+        if (QT == 2 && ok && nt > 1) s_of(1);
+        commit_to(empty + 8 * slot);
+      };
+      auto pv_all = [&]() {
+        wait(full + 8 * vslot, vround & 1, kDevTimeoutFull);
+        if (ok) pv_of(0);
+        if (QT == 2 && ok && pnt > 1) pv_of(1);
+        commit_to(empty + 8 * vslot);
+        pend = false;
+      };
+      while (ok) {
+        // The next key tile, if any; P V of the tile before it is pending.
+        if (u == take) {
+          if (!next_seg()) more = false;
+          u = 0;
+          take = __shfl_sync(0xffffffffu, g.take, 0);
+          nt = __shfl_sync(0xffffffffu, tiles(g), 0);
+          // An item's last P V come before the next item's S, which may wait
+          // for its queries.
+          if (pend) pv_all();
+          if (!more) break;
+          if (take == 0) continue;
         }
-        // TMEM is given back only when every MMA has finished.
-        tc_commit(bar_end);
-        volatile int no_abort = 0;
-        attn_wait(bar_end, 0, status, kDevTimeoutAcc, &no_abort);
+        s_all();  // within an item S goes first
+        const uint32_t v = slot + 1 == kSlots ? 0 : slot + 1, vr = slot + 1 == kSlots ? round + 1 : round;
+        if (pend && ok) pv_all();
+        vslot = v;
+        vround = vr;
+        slot = v + 1 == kSlots ? 0 : v + 1;
+        round = v + 1 == kSlots ? vr + 1 : vr;
+        pfirst = u == 0;
+        pnt = nt;
+        pend = true;
+        ++u;
       }
+      // TMEM is given back only when every MMA has finished.
+      commit_to(bar_end);
+      volatile int no_abort = 0;
+      attn_wait(bar_end, 0, status, kDevTimeoutAcc, &no_abort);
       __syncwarp();
     } else if (role == 1) {
       // ---------------- TMA producer ----------------
@@ -674,7 +760,7 @@ cudaError_t launch_tc(const CUtensorMap &tk, const CUtensorMap &tv, const AttnAr
   cfg.gridDim = dim3((unsigned)grid, C::R / 4, 1);
   cfg.blockDim = dim3(128, 1, 1);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, attn_join_kernel<C::R, C::KT, DP>, a);
+  return cudaLaunchKernelEx(&cfg, attn_join_kernel<C::R, KT, DP>, a);
 }
 
 }  // namespace
