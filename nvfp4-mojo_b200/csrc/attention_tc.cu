@@ -11,15 +11,17 @@
 // warps never stop; O stays in TMEM for all of an item.
 //   warps 0-3 (and 4-7, QT = 2)  softmax of tile 0 (1), Q into shared memory,
 //                                the rare rescaling of O, the epilogue;
-//   then one warp each           MMA issue (one thread), TMA producer, zeroing
-//                                of values that no row sees, and the block's
-//                                list of items.
+//   then one warp each           MMA issue for each query tile, TMA producer,
+//                                and the block's list of items with the
+//                                zeroing of values that no row sees.
 // O is rescaled only when a row's maximum has grown by more than 2^8 since
 // the last time (weights then stay below 2^8, exact in the sums' fp32); the
 // reference is the same for sum and product, so the result is not changed.
-// The bound beside the tensor cores is the exponential: 2 x 128 x 64 of them
-// per key tile take the MUFU 1024 cycles, as long as the products take the
-// tensor cores.  So a part of them is computed on the FMA pipe instead.
+// Besides the tensor cores the exponentials bound it: 2 x 128 x 64 of them per
+// key tile take the MUFU 1024 cycles, as long as the products take the tensor
+// cores.  (A part of them on the FMA pipe, by a polynomial, measured slower:
+// 650 us with one in eight against 629 us, a prompt of 8192 at 32 / 4 heads of
+// 128: the issue slots are as scarce.)
 #include <cuda_bf16.h>
 
 #include <type_traits>
@@ -39,7 +41,6 @@ namespace {
 
 constexpr int kItemCost = 3;  // of an item's beginning and end, in key tiles
 constexpr int kSegs = 4;      // items that the scheduling warp may be ahead
-constexpr int kPolyOf8 = 2;   // of 8 pairs of exponentials, those on the FMA pipe
 
 constexpr int KT = 64;        // keys per tile
 
@@ -70,13 +71,16 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[
       "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
-// 16 lanes x 16 columns: lane l gets columns 8 k + 2 (l % 4) + {0, 1} of rows
+// 16 lanes x 32 columns: lane l gets columns 8 k + 2 (l % 4) + {0, 1} of rows
 // l / 4 (r[4 k], r[4 k + 1]) and l / 4 + 8 (r[4 k + 2], r[4 k + 3]).
-__device__ __forceinline__ void tmem_ld_16x256_x2(uint32_t taddr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr)
-               : "memory");
+__device__ __forceinline__ void tmem_ld_16x256_x4(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -168,33 +172,10 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// 2^x of a pair on the FMA pipe, x <= 9: x = n + f with n the nearest whole
-// number (from adding 1.5 * 2^23), 2^f on [-1/2, 1/2] by a polynomial of
-// degree 4 fitted for the least relative error (2.6e-6), n added to the
-// exponent.  x below -126 gives a weight of at most 2^-126.
-__device__ __forceinline__ void exp2_pair(uint64_t x2, float &p0, float &p1) {
-  float x0, x1;
-  unpair(x2, x0, x1);
-  x2 = pair(fmaxf(x0, -126.0f), fmaxf(x1, -126.0f));
-  const uint64_t t2 = add2(x2, pair(12582912.0f, 12582912.0f));
-  const uint64_t n2 = add2(t2, pair(-12582912.0f, -12582912.0f));
-  const uint64_t f2 = fma2(n2, pair(-1.0f, -1.0f), x2);
-  uint64_t r = fma2(f2, pair(0.009570101276040077f, 0.009570101276040077f),
-                    pair(0.05591786280274391f, 0.05591786280274391f));
-  r = fma2(r, f2, pair(0.240247443318367f, 0.240247443318367f));
-  r = fma2(r, f2, pair(0.6931217908859253f, 0.6931217908859253f));
-  r = fma2(r, f2, pair(0.9999992847442627f, 0.9999992847442627f));
-  float t0, t1, r0, r1;
-  unpair(t2, t0, t1);
-  unpair(r, r0, r1);
-  p0 = __int_as_float(__float_as_int(r0) + (__float_as_int(t0) << 23));
-  p1 = __int_as_float(__float_as_int(r1) + (__float_as_int(t1) << 23));
-}
-
-// The largest of three; not a number if one of them is.
+// The largest of three.
 __device__ __forceinline__ float max3(float x, float y, float z) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
   return r;
 }
 
@@ -231,7 +212,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
     abort_flag = 0;
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(full + 8 * i, 1);
-      mbar_init(empty + 8 * i, 1);
+      mbar_init(empty + 8 * i, QT);  // a warp per query tile
       mbar_init(edge + 8 * i, 1);
     }
     mbar_init(bar_q, 4);
@@ -241,10 +222,10 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       mbar_init(bar_p + 8 * x, 4);
       mbar_init(bar_o + 8 * x, 1);
     }
-    mbar_init(bar_end, 1);
+    mbar_init(bar_end, QT);
     for (int i = 0; i < kSegs; ++i) {
       mbar_init(seg_full + 8 * i, 1);
-      mbar_init(seg_empty + 8 * i, C::kSoftWarps + 3);
+      mbar_init(seg_empty + 8 * i, C::kSoftWarps + QT + 2);
     }
     mbar_fence_init();
     prefetch_tmap(&tmK);
@@ -391,7 +372,6 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
           top[0] = max3(top[0], s[KT - 4], s[KT - 3]);
           top[1] = max3(top[1], s[KT - 2], s[KT - 1]);
           const float mx = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * c2;
-          if (!(mx < INFINITY)) l = NAN;  // a score that is infinite or not a number
           const bool grow = mx > m + 8.0f;
           if (__any_sync(0xffffffffu, grow)) {
             const float mn = grow ? mx : m;
@@ -425,13 +405,9 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
           for (int i = 0; i < 32; ++i) {
             const uint64_t e2 = fma2(pair(s[2 * i], s[2 * i + 1]), c22, nm2);
             float e0, e1;
-            if (i % 8 < kPolyOf8) {
-              exp2_pair(e2, e0, e1);
-            } else {
-              unpair(e2, e0, e1);
-              e0 = ex2(e0);
-              e1 = ex2(e1);
-            }
+            unpair(e2, e0, e1);
+            e0 = ex2(e0);
+            e1 = ex2(e1);
             sum[i & 1] = add2(sum[i & 1], pair(e0, e1));
             // Rounded to bf16 for the second product only; the sum keeps the
             // unrounded weights.
@@ -461,10 +437,9 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
         }
       }
       if (!mine) continue;
-      if (m == -INFINITY) l = 0.0f;  // nothing seen: masked weights on the FMA pipe are not quite zero
 
       // ---- epilogue: straight from TMEM (shared memory is busy with the other
-      // tile's MMAs), 16 rows by 16 columns at a time in the shape where 4
+      // tile's MMAs), 16 rows at a time in the shape where 4
       // lanes hold 8 columns of a row side by side.  The loops stay rolled: this
       // code runs once per item and would come from L2 line by line.
       AttnFinish f = {};
@@ -507,49 +482,49 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
               gate[i] = reinterpret_cast<const char *>(a.gate + tok * a.g_ts + head * a.g_hs + 2 * (lane & 3));
             }
           }
+          // 32 columns a step; with a gate or a prefix part 64, whose loads are
+          // in flight together.
+          constexpr int W = MODE == 2 ? 64 : 32;
           const int cols = MODE == 0 ? DP : a.D;
 #pragma unroll 1
-          for (int c = 0; c < cols; c += 16) {
-            // Per row i: columns c + 8 k + 2 (lane % 4) + {0, 1}.
-            uint32_t o[8] = {}, w[2][2] = {};
-            float2 p[2][2] = {};
-            if (take > 0) tmem_ld_16x256_x2(tO + ((uint32_t)h << 16) + c, o);
+          for (int c0 = 0; c0 < cols; c0 += W) {
+            // Per row i: columns c0 + 8 k + 2 (lane % 4) + {0, 1}.
+            uint32_t o[W / 32][16] = {}, w[2][W / 8] = {};
+            float2 p[2][W / 8] = {};
+            if (take > 0)
+#pragma unroll
+              for (int x = 0; x < W / 32; ++x) tmem_ld_16x256_x4(tO + ((uint32_t)h << 16) + c0 + 32 * x, o[x]);
             if constexpr (MODE == 2) {
 #pragma unroll
               for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                  if (a.gate && on[i] && c + 8 * k < cols)
-                    w[i][k] = *reinterpret_cast<const uint32_t *>(gate[i] + 2 * (c + 8 * k));
-                  if (sp[i] != 0.0f) p[i][k] = *reinterpret_cast<const float2 *>(prev[i] + 4 * (c + 8 * k));
+                for (int k = 0; k < W / 8; ++k) {
+                  if (a.gate && on[i] && c0 + 8 * k < cols)
+                    w[i][k] = *reinterpret_cast<const uint32_t *>(gate[i] + 2 * (c0 + 8 * k));
+                  if (sp[i] != 0.0f) p[i][k] = *reinterpret_cast<const float2 *>(prev[i] + 4 * (c0 + 8 * k));
                 }
             }
             tmem_ld_wait();
-            float x[2][2][2];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-              for (int k = 0; k < 2; ++k)
+              for (int k = 0; k < W / 8; ++k) {
+                float x[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                  const float v = __uint_as_float(o[4 * k + 2 * i + e]);
-                  x[i][k][e] = so[i] == 0.0f ? 0.0f : v * so[i];
+                  const float v = __uint_as_float(o[k / 4][4 * (k % 4) + 2 * i + e]);
+                  x[e] = so[i] == 0.0f ? 0.0f : v * so[i];
                   if constexpr (MODE == 2) {
-                    x[i][k][e] = fmaf(e ? p[i][k].y : p[i][k].x, sp[i], x[i][k][e]);
-                    const float g =
-                        sigmoidf(__uint_as_float(e ? w[i][k] & 0xffff0000u : w[i][k] << 16));
-                    x[i][k][e] *= a.gate ? g : 1.0f;
+                    x[e] = fmaf(e ? p[i][k].y : p[i][k].x, sp[i], x[e]);
+                    const float g = sigmoidf(__uint_as_float(e ? w[i][k] & 0xffff0000u : w[i][k] << 16));
+                    x[e] *= a.gate ? g : 1.0f;
                   }
                 }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
                 if constexpr (MODE == 0) {
-                  if (on[i]) *reinterpret_cast<float2 *>(dst[i] + 4 * (c + 8 * k)) = make_float2(x[i][k][0], x[i][k][1]);
+                  if (on[i]) *reinterpret_cast<float2 *>(dst[i] + 4 * (c0 + 8 * k)) = make_float2(x[0], x[1]);
                 } else {
-                  if (on[i] && c + 8 * k < cols)
-                    *reinterpret_cast<uint32_t *>(dst[i] + 2 * (c + 8 * k)) = pack_bf16(x[i][k][0], x[i][k][1]);
+                  if (on[i] && c0 + 8 * k < cols)
+                    *reinterpret_cast<uint32_t *>(dst[i] + 2 * (c0 + 8 * k)) = pack_bf16(x[0], x[1]);
                 }
               }
           }
@@ -563,78 +538,71 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
   } else {
     if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     const int role = warp - C::kSoftWarps;
-    if (role == 0) {
-      // ---------------- MMA issue ----------------
+    if (role == 0 || (role == 3 && QT == 2)) {
+      // ---------------- MMA issue, a warp per query tile ----------------
+      const int t = role == 0 ? 0 : 1;
       constexpr uint32_t idS = idesc_bf16_f32(128, KT);
       constexpr uint32_t idO = idesc_bf16_f32(128, DP) | kTransposeB;
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), sb = __shfl_sync(0xffffffffu, sbase, 0);
-      const uint32_t qd = desc_lo(sb, 16), kd = desc_lo(sb + C::offKV, 16), vd = desc_lo(sb + C::offKV, KT * 128);
+      const uint32_t qd = desc_lo(sb + t * C::kQ, 16), kd = desc_lo(sb + C::offKV, 16),
+                     vd = desc_lo(sb + C::offKV, KT * 128);
       bool ok = true;
-      // Key tiles so far and the slot of the next one's K (its V is in the
-      // slot after) with the parity of that slot's round.
+      // The slot of the next key tile's K (its V is in the slot after) and of
+      // the pending tile's V, with the parities of their rounds.
       uint32_t slot = 0, round = 0, vslot = 0, vround = 0;
-      // Per query tile: S issued, P V issued, queries awaited.
-      uint32_t ns[2] = {0, 0}, np[2] = {0, 0}, nq[2] = {0, 0};
-      bool pend = false, pfirst = false, more = true;
-      int pnt = 0, u = 0, take = 0, nt = 0;  // pnt, pfirst: of the pending P V
+      uint32_t ns = 0, np = 0, nq = 0;  // S issued, P V issued, queries awaited
+      bool pend = false, pfirst = false, puse = false, use = false, more = true;
+      int u = 0, take = 0;  // pfirst, puse: of the pending P V
       auto wait = [&](uint32_t bar, uint32_t ph, int code) {
         ok = ok && __all_sync(0xffffffffu, attn_wait(bar, ph, status, code, abort));
       };
-      auto s_of = [&](int t) {
-        if (u == 0) wait(bar_q + 8 * t, nq[t]++ & 1, kDevTimeoutDec);
-        if (!ok) return;
-        tc_fence_after();
-        const uint32_t x = 2 * t + (ns[t]++ & 1);
-        const uint32_t k0 = kd + slot * (C::kTile >> 4), q0 = qd + t * (C::kQ >> 4);
-#pragma unroll
-        for (int hf = 0; hf < DP / 64; ++hf)
-          mma_ss4(tm + x * KT, q0 + hf * (128 * 128 >> 4), k0 + hf * (KT * 128 >> 4), idS, hf != 0);
-        commit_to(bar_s + 8 * x);
-      };
-      auto pv_of = [&](int t) {
-        const uint32_t x = 2 * t + (np[t] & 1);
-        wait(bar_p + 8 * x, (np[t] >> 1) & 1, kDevTimeoutDec);
-        ++np[t];
-        if (!ok) return;
-        tc_fence_after();
-        mma_ts4(tm + C::colO + t * DP, tm + x * KT, vd + vslot * (C::kTile >> 4), idO, !pfirst);
-        commit_to(bar_o + 8 * x);
-      };
-      auto s_all = [&]() {
-        wait(full + 8 * slot, round & 1, kDevTimeoutFull);
-        if (ok) s_of(0);
-        if (QT == 2 && ok && nt > 1) s_of(1);
-        commit_to(empty + 8 * slot);
-      };
-      auto pv_all = [&]() {
+      auto pv = [&]() {
         wait(full + 8 * vslot, vround & 1, kDevTimeoutFull);
-        if (ok) pv_of(0);
-        if (QT == 2 && ok && pnt > 1) pv_of(1);
+        if (puse) {
+          const uint32_t x = 2 * t + (np & 1);
+          wait(bar_p + 8 * x, (np >> 1) & 1, kDevTimeoutDec);
+          ++np;
+          if (ok) {
+            tc_fence_after();
+            mma_ts4(tm + C::colO + t * DP, tm + x * KT, vd + vslot * (C::kTile >> 4), idO, !pfirst);
+            commit_to(bar_o + 8 * x);
+          }
+        }
         commit_to(empty + 8 * vslot);
         pend = false;
       };
       while (ok) {
-        // The next key tile, if any; P V of the tile before it is pending.
-        if (u == take) {
+        if (u == take) {  // the next item
           if (!next_seg()) more = false;
           u = 0;
           take = __shfl_sync(0xffffffffu, g.take, 0);
-          nt = __shfl_sync(0xffffffffu, tiles(g), 0);
-          // An item's last P V come before the next item's S, which may wait
+          use = t < __shfl_sync(0xffffffffu, tiles(g), 0);
+          // An item's last P V comes before the next item's S, which may wait
           // for its queries.
-          if (pend) pv_all();
+          if (pend) pv();
           if (!more) break;
           if (take == 0) continue;
         }
-        s_all();  // within an item S goes first
-        const uint32_t v = slot + 1 == kSlots ? 0 : slot + 1, vr = slot + 1 == kSlots ? round + 1 : round;
-        if (pend && ok) pv_all();
-        vslot = v;
-        vround = vr;
-        slot = v + 1 == kSlots ? 0 : v + 1;
-        round = v + 1 == kSlots ? vr + 1 : vr;
+        wait(full + 8 * slot, round & 1, kDevTimeoutFull);
+        if (use) {  // S; within an item it goes before the P V of the tile before
+          if (u == 0) wait(bar_q + 8 * t, nq++ & 1, kDevTimeoutDec);
+          if (ok) {
+            tc_fence_after();
+            const uint32_t x = 2 * t + (ns++ & 1), k0 = kd + slot * (C::kTile >> 4);
+#pragma unroll
+            for (int hf = 0; hf < DP / 64; ++hf)
+              mma_ss4(tm + x * KT, qd + hf * (128 * 128 >> 4), k0 + hf * (KT * 128 >> 4), idS, hf != 0);
+            commit_to(bar_s + 8 * x);
+          }
+        }
+        commit_to(empty + 8 * slot);
+        if (pend && ok) pv();
+        vslot = slot + 1 == kSlots ? 0 : slot + 1;
+        vround = slot + 1 == kSlots ? round + 1 : round;
+        slot = vslot + 1 == kSlots ? 0 : vslot + 1;
+        round = vslot + 1 == kSlots ? vround + 1 : vround;
         pfirst = u == 0;
-        pnt = nt;
+        puse = use;
         pend = true;
         ++u;
       }
@@ -693,9 +661,24 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       // Rows of a value tile before the first or from the last key on (never
       // loaded, or the rest of a page) are zeroed: their weights are zero,
       // but what lies there may not be finite.
-      uint32_t at = 0, phase = 0;
-      bool ok = true;
-      while (ok && next_seg()) {
+      // This warp also lists the block's items, three ahead of its own.
+      uint32_t at = 0, phase = 0, listed = 0;
+      bool ok = true, more = true;
+      while (ok) {
+        if (lane == 0) {
+          for (; more && listed < nseg + kSegs - 1; ++listed) {
+            const uint32_t i = listed % kSegs;
+            if (listed >= kSegs &&
+                !attn_wait(seg_empty + 8 * i, (listed / kSegs - 1) & 1, status, kDevTimeoutEmpty, abort))
+              break;
+            more = attn_segment<R, KT, kItemCost>(a, cur, g);
+            if (!more) g.take = -1;
+            segs[i] = g;
+            mbar_arrive(seg_full + 8 * i);
+          }
+        }
+        __syncwarp();
+        if (!next_seg()) break;
         for (int u = 0; u < g.take; ++u, at += 2) {
           const int j0 = (g.it.u0 + g.off + u) * KT;
           if (j0 >= g.it.lo && j0 + KT <= g.it.hi) continue;
@@ -717,17 +700,6 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(full + 8 * slot);
         }
-      }
-    } else if (lane == 0) {
-      // ---------------- the block's items, ahead of the other warps --------
-      for (uint32_t n = 0;; ++n) {
-        const uint32_t i = n % kSegs;
-        if (n >= kSegs && !attn_wait(seg_empty + 8 * i, (n / kSegs - 1) & 1, status, kDevTimeoutEmpty, abort)) break;
-        const bool more = attn_segment<R, KT, kItemCost>(a, cur, g);
-        if (!more) g.take = -1;
-        segs[i] = g;
-        mbar_arrive(seg_full + 8 * i);
-        if (!more) break;
       }
     }
   }
