@@ -377,7 +377,7 @@ __device__ __forceinline__ AttnFinish attn_finish(const AttnArgs &a, const AttnR
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a row that sees nothing is 0
   f.so = w * inv;
-  f.sp *= inv;
+  if (f.sp != 0.0f) f.sp *= inv;  // stays 0 without a prefix part, whatever l is
   f.lse2 = l == 0.0f ? -INFINITY : m + log2f(l);
   return f;
 }
@@ -404,7 +404,7 @@ __device__ __forceinline__ void attn_store(const AttnArgs &a, const AttnRow &r, 
           make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
     return;
   }
-  if (f.sp != 0.0f) {
+  if (a.prev_o && f.sp != 0.0f) {
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
       const float4 p = *reinterpret_cast<const float4 *>(a.prev_o + f.id * DP + d + i);

@@ -39,7 +39,7 @@ static __device__ int g_attn_tc_status;
 
 namespace {
 
-constexpr int kItemCost = 3;  // of an item's beginning and end, in key tiles
+constexpr int kItemCost = 5;  // of an item's beginning and end, in key tiles
 constexpr int kSegs = 4;      // items that the scheduling warp may be ahead
 
 constexpr int KT = 64;        // keys per tile
@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
                 for (int k = 0; k < W / 8; ++k) {
                   if (a.gate && on[i] && c0 + 8 * k < cols)
                     w[i][k] = *reinterpret_cast<const uint32_t *>(gate[i] + 2 * (c0 + 8 * k));
-                  if (sp[i] != 0.0f) p[i][k] = *reinterpret_cast<const float2 *>(prev[i] + 4 * (c0 + 8 * k));
+                  if (a.prev_o && sp[i] != 0.0f) p[i][k] = *reinterpret_cast<const float2 *>(prev[i] + 4 * (c0 + 8 * k));
                 }
             }
             tmem_ld_wait();

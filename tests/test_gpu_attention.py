@@ -197,6 +197,32 @@ def test_shared_prefix_is_the_whole_sequence():
     run_and_check(s)
 
 
+@pytest.mark.parametrize("qlens", [[1, 1, 1], [3, 60, 200]])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("prefix", [0, 50])
+def test_queries_that_are_not_finite(qlens, gated, prefix):
+    """A query with a NaN or an infinity spoils its own row and no other, with
+    and without a gate or a prefix part in the last step."""
+    import nvfp4
+
+    for D, H, KV in ((128, 8, 2), (256, 8, 1)):
+        s = make(28, [q + 70 for q in qlens], qlens, KV, D, H, 16, prefix=prefix)
+        gate = torch.randn(s["T"], H, D, generator=s["g"]).to(torch.bfloat16) if gated else None
+        bad = s["q"].clone()
+        bad[1, 2, 5], bad[s["T"] - 1, 0, 0], bad[0, 4, 1] = math.nan, math.inf, -math.inf
+        out = nvfp4.paged_attention(bad.cuda(), s["cache"], batch_of(s), nvfp4.AttentionConfig(H, KV, D),
+                                    gate=None if gate is None else gate.cuda())
+        hit = [(1, 2), (s["T"] - 1, 0), (0, 4)]
+        for t, h in hit:
+            assert torch.isnan(out[t, h]).all()
+            out[t, h] = 0
+        o, _, tol, _ = ref.attention(s["q"], s["k"], s["v"], s["kv_len"], s["table"], s["q_start"],
+                                     prefix_pages=s["prefix_pages"], prefix_len=prefix, gate=gate)
+        for t, h in hit:
+            o[t, h] = 0
+        ref.check(out, o, tol, "out")
+
+
 def test_repeats_bit_for_bit():
     import nvfp4
 
