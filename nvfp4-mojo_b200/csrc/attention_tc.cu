@@ -338,11 +338,6 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
           uint32_t raw[2][32];
           tmem_ld_32x32b_x32(tS, raw[0]);
           tmem_ld_32x32b_x32(tS + 32, raw[1]);
-          if (u == take - 1) {  // every S of the item is done: its Q may go
-            have = next_seg();
-            fetch = have && g.take > 0 && t < tiles(g);
-            if (fetch) q_start();
-          }
           tmem_ld_wait();
           float s[KT];
 #pragma unroll
@@ -423,7 +418,13 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
           if (lane == 0) mbar_arrive(bar_p + 8 * x);
         }
         if (!ok) break;
-        if (fetch) q_done();
+        // Every S of the item is done: its Q may go.
+        have = next_seg();
+        fetch = have && g.take > 0 && t < tiles(g);
+        if (fetch) {
+          q_start();
+          q_done();
+        }
         const uint32_t y = 2 * t + ((n - 1) & 1);
         if (!__all_sync(0xffffffffu, attn_wait(bar_o + 8 * y, ((n - 1) >> 1) & 1, status, kDevTimeoutAcc, abort)))
           break;
