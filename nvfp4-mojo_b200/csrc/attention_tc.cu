@@ -344,6 +344,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
           for (int c = 0; c < KT; ++c) s[c] = __uint_as_float(raw[c / 32][c % 32]);
           if constexpr (MOD) {
             const float cap2 = 2.0f * kLog2e / a.softcap * a.scale;
+            const float dist = (float)(pos - j0);  // a conversion per element would be on the MUFU, too
 #pragma unroll
             for (int c = 0; c < KT; ++c) {
               float v;
@@ -351,7 +352,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
                 v = a.softcap - __fdividef(2.0f * a.softcap, 1.0f + ex2(s[c] * cap2));
               else
                 v = s[c] * a.scale;
-              s[c] = fmaf(v, kLog2e, -slope * fabsf((float)(pos - j0 - c)));
+              s[c] = fmaf(v, kLog2e, -slope * fabsf(dist - (float)c));
             }
           }
           if (j0 < lo_all || j0 + KT > hi_all) {
