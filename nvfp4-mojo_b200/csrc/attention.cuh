@@ -7,10 +7,11 @@
 // item is (sequence, key/value head, R consecutive rows); its keys, the union
 // of what its rows see, are walked in units of KT.  All items' units, in the
 // order sequence, head, rows, form one line of W units that the launch's
-// blocks divide evenly: block c takes [c W / parts, (c + 1) W / parts).  W is
-// below 2^31 (checked by the caller from the bounds of the call).  An
-// item cut by a block boundary leaves unnormalised parts in the workspace, at
-// most two per block, which a second launch joins in the order of the blocks.
+// workers (blocks, or single warps) divide evenly: worker c takes
+// [c W / parts, (c + 1) W / parts).  W is below 2^31 (checked by the caller from
+// the bounds of the call).  An
+// item cut by such a boundary leaves unnormalised parts in the workspace, at
+// most two per worker, which a second launch joins in the order of the workers.
 // The division depends on the lengths alone, so results repeat bit for bit.
 #pragma once
 
@@ -24,6 +25,13 @@ namespace nvfp4 {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kPlanCache = 1024;  // sequences whose units the plan keeps in shared memory
+
+// What a worker leads: an item that starts in its share and goes on in later
+// ones (last_part < 0: none).
+struct __align__(16) AttnMeta {
+  int last_part, tok0, h, row0;  // the item's first row (token * G + head) of its sequence
+  int live, unused[3];           // its rows in use
+};
 
 struct AttnArgs {
   int B, T, Hq, Hkv, G, D;
@@ -40,11 +48,11 @@ struct AttnArgs {
   __nv_bfloat16 *out;
   int64_t q_ts, q_hs, g_ts, g_hs, o_ts, o_hs;
   float *lse;
-  // Workspace: parts [2 * grid][R][DP] with their (max, sum), who joins what,
+  // Workspace: parts [2 * workers][R][DP] with their (max, sum), who joins what,
   // and the prefix pass's normalised rows [T, Hq, DP] with their lse (base 2).
   float *part_o;
   float2 *part_ml;
-  int4 *meta;
+  AttnMeta *meta;
   float *prev_o;
   float *prev_lse;
 };
@@ -192,18 +200,19 @@ __device__ __forceinline__ bool attn_wait(uint32_t bar, uint32_t parity, int *st
   return ok;
 }
 
-// Where a block starts on the line, and how far it goes.
+// Where a worker starts on the line, and how far it goes.
 struct AttnCursor {
   int b, h, rb, off;  // item and unit within it
   int at, end;        // on the line
-  int total, parts;   // W and the blocks that have a share
+  int total, parts;   // W and the workers that have a share
+  int worker;
 };
 
-// The first unit of part c: floor(c total / parts).  The quotient's fraction
-// is a multiple of 1 / parts, so a quarter unit before the division keeps the
-// rounded product on the right side.
-__device__ __forceinline__ int attn_line_at(int c, int total, int parts, double inv) {
-  return (int)(((double)c * (double)total + 0.25) * inv);
+// The first unit of part c: floor(c total / parts), in 32 bits (c and parts are
+// at most a few hundred).
+__device__ __forceinline__ int attn_line_at(int c, int total, int parts) {
+  const int q = total / parts, r = total - q * parts;
+  return c * q + c * r / parts;
 }
 
 struct AttnPlanSmem {
@@ -212,9 +221,10 @@ struct AttnPlanSmem {
   AttnCursor cur;
 };
 
-// Plans this block's share; every thread of the block calls it.  parts: at
-// most gridDim.x and one per `min_units` units.
-template <int R, int KT, int E>
+// Plans a worker's share; every thread of the block calls it.  Workers are the
+// blocks (WARPS 0: one result for all threads), or the first WARPS warps of
+// each.  parts: at most all workers and one per `min_units` units.
+template <int R, int KT, int E, int WARPS>
 __device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units, AttnPlanSmem *sm) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
   const int NS = attn_num_seqs(a);
@@ -227,36 +237,42 @@ __device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units
     for (int rb = start; rb < nb; rb += step) u += attn_item_units<R, KT, E>(a, s, rb);
     return u;
   };
-  // Sequences of few items: a thread each; of many: a warp each.
+  // Sequences of few items: a thread each; of many: a warp each.  For up to
+  // 128 sequences of few items each warp that works alone plans alone.
   const bool by_warp = a.max_blocks > 4;
+  const bool alone = WARPS && !by_warp && NS <= 128;
   int sum = 0;
 #pragma unroll 1
-  for (int b = by_warp ? warp : tid; b < NS; b += by_warp ? nw : (int)blockDim.x) {
+  for (int b = alone ? lane : by_warp ? warp : tid; b < NS; b += alone ? 32 : by_warp ? nw : (int)blockDim.x) {
     int u = seq_units(b, by_warp ? lane : 0, by_warp ? 32 : 1);
     if (by_warp) u = __reduce_add_sync(0xffffffffu, u);
     if (!by_warp || lane == 0) {
-      if (b < kPlanCache) sm->units[b] = u;
+      if (!alone && b < kPlanCache) sm->units[b] = u;
       sum += u;
     }
   }
+  __syncwarp();
   sum = __reduce_add_sync(0xffffffffu, sum);
-  if (lane == 0) sm->sum[warp] = sum;
-  __syncthreads();
-  if (warp == 0) {
-    AttnCursor c = {};
-    c.total = a.Hkv * __reduce_add_sync(0xffffffffu, lane < nw ? sm->sum[lane] : 0);
-    c.parts = min((c.total + min_units - 1) / min_units, (int)gridDim.x);
-    if ((int)blockIdx.x < c.parts) {
-      const double inv = 1.0 / (double)c.parts;
-      c.at = attn_line_at(blockIdx.x, c.total, c.parts, inv);
-      c.end = attn_line_at(blockIdx.x + 1, c.total, c.parts, inv);
+  if (!alone) {
+    if (lane == 0) sm->sum[warp] = sum;
+    __syncthreads();
+    sum = __reduce_add_sync(0xffffffffu, lane < nw ? sm->sum[lane] : 0);
+  }
+  AttnCursor c = {};
+  if (warp < (WARPS ? WARPS : 1)) {
+    c.worker = WARPS ? blockIdx.x * WARPS + warp : blockIdx.x;
+    c.total = a.Hkv * sum;
+    c.parts = min((c.total + min_units - 1) / min_units, (int)gridDim.x * (WARPS ? WARPS : 1));
+    if (c.worker < c.parts) {
+      c.at = attn_line_at(c.worker, c.total, c.parts);
+      c.end = attn_line_at(c.worker + 1, c.total, c.parts);
       // The sequence that holds unit c.at, 32 sequences at a time; then, with
       // its units per head, the item in the same way.
       int o = c.at, ub = 0;
 #pragma unroll 1
       for (int base = 0; base < NS; base += 32) {
         const int b = base + lane;
-        const int u = b >= NS ? 0 : b < kPlanCache ? sm->units[b] : seq_units(b, 0, 1);
+        const int u = b >= NS ? 0 : !alone && b < kPlanCache ? sm->units[b] : seq_units(b, 0, 1);
         int inc = u * a.Hkv;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -296,19 +312,20 @@ __device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units
         o -= __shfl_sync(0xffffffffu, inc, 31);
       }
     }
-    if (lane == 0) sm->cur = c;
+    if (!WARPS && lane == 0) sm->cur = c;
   }
+  if (WARPS) return c;
   __syncthreads();
   return sm->cur;
 }
 
-// One stretch of a block's share: key units [off, off + take) of an item.
+// One stretch of a worker's share: key units [off, off + take) of an item.
 struct AttnSegment {
   AttnSeq s;
   AttnItem it;
   int b, h, rb, off, take;
-  int slot;        // workspace part; -1: the block has all of the item
-  int last_part;   // >= 0: the item starts here and goes on up to this block
+  int slot;        // workspace part; -1: the worker has all of the item
+  int last_part;   // >= 0: the item starts here and goes on up to this worker
 };
 
 template <int R, int KT, int E>
@@ -335,14 +352,15 @@ __device__ __forceinline__ bool attn_segment(const AttnArgs &a, AttnCursor &c, A
     g.take = min(off + take, g.it.units) - min(off, g.it.units);
     const bool real = g.take > 0 || (g.it.units == 0 && off == 0);
     const bool first = off == 0, last = off + take >= g.it.units;
-    g.slot = first && last ? -1 : 2 * (int)blockIdx.x + (first ? 1 : 0);
+    g.slot = first && last ? -1 : 2 * c.worker + (first ? 1 : 0);
     g.last_part = -1;
     if (first && !last) {
       const int x = c.at + g.it.units - 1;  // the item's last unit
-      const double inv = 1.0 / (double)c.parts;
-      int p = min((int)((double)x * (double)c.parts / (double)c.total), c.parts - 1);
-      while (p + 1 < c.parts && attn_line_at(p + 1, c.total, c.parts, inv) <= x) ++p;
-      while (attn_line_at(p, c.total, c.parts, inv) > x) --p;
+      int p = min((int)__fdividef((float)x * (float)c.parts, (float)c.total), c.parts - 1);  // near it
+#pragma unroll 1
+      while (p + 1 < c.parts && attn_line_at(p + 1, c.total, c.parts) <= x) ++p;
+#pragma unroll 1
+      while (attn_line_at(p, c.total, c.parts) > x) --p;
       g.last_part = p;
     }
     c.at += take;
@@ -351,6 +369,17 @@ __device__ __forceinline__ bool attn_segment(const AttnArgs &a, AttnCursor &c, A
     if (real) return true;
   }
   return false;
+}
+
+template <int R>
+__device__ __forceinline__ AttnMeta attn_meta(const AttnArgs &a, const AttnSegment &g) {
+  AttnMeta m;
+  m.last_part = g.last_part;
+  m.tok0 = g.s.tok0;
+  m.h = g.h;
+  m.row0 = g.rb * R;
+  m.live = min(g.s.ql * a.G - m.row0, R);
+  return m;
 }
 
 // The last step of a row: its output is o * so + prefix part * sp, gated.
@@ -389,109 +418,130 @@ __device__ __forceinline__ void attn_store_lse(const AttnArgs &a, const AttnFini
 
 __device__ __forceinline__ float sigmoidf(float x) { return __fdividef(1.0f, 1.0f + ex2(-x * kLog2e)); }
 
-// N = 4 or 8 values of the row from column d on (the prefix pass keeps the
-// normalised row in fp32).
-template <int N>
-__device__ __forceinline__ void attn_store(const AttnArgs &a, const AttnRow &r, const AttnFinish &f, int d,
-                                           int DP, float (&v)[N]) {
+// 4 values of the row from column d on (the prefix pass keeps the normalised
+// row in fp32).
+__device__ __forceinline__ void attn_store4(const AttnArgs &a, const AttnRow &r, const AttnFinish &f, int d,
+                                            int DP, float (&v)[4]) {
   if (d >= a.D) return;
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = f.so == 0.0f ? 0.0f : v[i] * f.so;
+  for (int i = 0; i < 4; ++i) v[i] = f.so == 0.0f ? 0.0f : v[i] * f.so;
   if (a.prefix_pass) {
-#pragma unroll
-    for (int i = 0; i < N; i += 4)
-      *reinterpret_cast<float4 *>(a.prev_o + f.id * DP + d + i) =
-          make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    *reinterpret_cast<float4 *>(a.prev_o + f.id * DP + d) = make_float4(v[0], v[1], v[2], v[3]);
     return;
   }
   if (a.prev_o && f.sp != 0.0f) {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const float4 p = *reinterpret_cast<const float4 *>(a.prev_o + f.id * DP + d + i);
-      v[i] = fmaf(p.x, f.sp, v[i]);
-      v[i + 1] = fmaf(p.y, f.sp, v[i + 1]);
-      v[i + 2] = fmaf(p.z, f.sp, v[i + 2]);
-      v[i + 3] = fmaf(p.w, f.sp, v[i + 3]);
-    }
+    const float4 p = *reinterpret_cast<const float4 *>(a.prev_o + f.id * DP + d);
+    v[0] = fmaf(p.x, f.sp, v[0]);
+    v[1] = fmaf(p.y, f.sp, v[1]);
+    v[2] = fmaf(p.z, f.sp, v[2]);
+    v[3] = fmaf(p.w, f.sp, v[3]);
   }
   if (a.gate) {
-    const __nv_bfloat16 *gp = a.gate + r.token * a.g_ts + r.head * a.g_hs + d;
-    uint32_t g[N / 2];
-    if constexpr (N == 8) {
-      const uint4 x = *reinterpret_cast<const uint4 *>(gp);
-      g[0] = x.x, g[1] = x.y, g[2] = x.z, g[3] = x.w;
-    } else {
-      const uint2 x = *reinterpret_cast<const uint2 *>(gp);
-      g[0] = x.x, g[1] = x.y;
-    }
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      v[i] *= sigmoidf(__uint_as_float(g[i / 2] << 16));
-      v[i + 1] *= sigmoidf(__uint_as_float(g[i / 2] & 0xffff0000u));
-    }
+    const uint2 g = *reinterpret_cast<const uint2 *>(a.gate + r.token * a.g_ts + r.head * a.g_hs + d);
+    v[0] *= sigmoidf(__uint_as_float(g.x << 16));
+    v[1] *= sigmoidf(__uint_as_float(g.x & 0xffff0000u));
+    v[2] *= sigmoidf(__uint_as_float(g.y << 16));
+    v[3] *= sigmoidf(__uint_as_float(g.y & 0xffff0000u));
   }
-  uint32_t w[N / 2];
-#pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(v[i], v[i + 1]);
-    w[i / 2] = *reinterpret_cast<const uint32_t *>(&h);
-  }
-  __nv_bfloat16 *op = a.out + r.token * a.o_ts + r.head * a.o_hs + d;
-  if constexpr (N == 8) *reinterpret_cast<uint4 *>(op) = make_uint4(w[0], w[1], w[2], w[3]);
-  else *reinterpret_cast<uint2 *>(op) = make_uint2(w[0], w[1]);
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+  *reinterpret_cast<uint2 *>(a.out + r.token * a.o_ts + r.head * a.o_hs + d) =
+      make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
 }
 
-// Joins the parts of the items that blocks cut: blockIdx.x is the block that
-// leads the item, a warp takes a row.
-template <int R, int KT, int DP>
-__global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnArgs a) {
+// Joins the parts of the items that workers cut.  Block (x, y): the items led
+// by the workers WPB x .. WPB x + WPB - 1, rows RPB y .. RPB y + RPB - 1.  With
+// few parts a warp takes a row; with many all eight take every eighth part of
+// a row and join through shared memory.
+template <int R, int DP, int WPB, int RPB>
+__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnArgs a) {
+  __shared__ float4 s_o[8][DP / 4];
+  __shared__ float2 s_ml[8];
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 w = a.meta[blockIdx.x];  // (sequence, head, rows, last part)
-  if (w.w < 0) return;
-  const AttnSeq s = attn_seq(a, w.x);
-  const int r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int row = w.z * R + r;
-  if (r >= R || row >= s.ql * a.G) return;
-  const int c0 = blockIdx.x, np = w.w - c0 + 1;
-  auto slot = [&](int i) -> int64_t { return i == 0 ? 2 * c0 + 1 : 2 * (c0 + i); };
-  // The largest maximum and the joined sum, by the lanes over the parts.
-  float m = -INFINITY;
-  for (int i = lane; i < np; i += 32) m = fmaxf(m, a.part_ml[slot(i) * R + r].x);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float mu = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int V = DP >= 128 ? DP / 128 : 1;  // float4 per lane
-  float4 acc[V];
+#pragma unroll 1
+  for (int k = 0; k < WPB; ++k) {
+    const int c0 = blockIdx.x * WPB + k;
+    const AttnMeta w = a.meta[c0];
+    if (w.last_part < 0) continue;
+    const int np = w.last_part - c0 + 1;
+    const bool many = np > 6;  // parts enough to share a row
+#pragma unroll 1
+    for (int i = many ? 0 : warp; i < RPB; i += many ? 1 : 8) {
+      const int r = blockIdx.y * RPB + i;
+      if (r >= w.live) break;  // the same for all warps where they share rows
+      float m = -INFINITY, l = 0.0f;
+      float4 acc[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) acc[v] = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-  for (int i = 0; i < np; ++i) {
-    const float2 ml = a.part_ml[slot(i) * R + r];
-    const float wt = ex2(ml.x - mu);
-    l = fmaf(ml.y, wt, l);
-    const float *o = a.part_o + (slot(i) * R + r) * DP;
+      for (int v = 0; v < V; ++v) acc[v] = make_float4(0, 0, 0, 0);
+      auto add = [&](const float2 ml, const float4 (&x)[V]) {
+        const float top = fmaxf(m, ml.x), mu = top == -INFINITY ? 0.0f : top;
+        const float f = ex2(m - mu), g = ex2(ml.x - mu);
+        m = top;
+        l = l * f + ml.y * g;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int d = 4 * lane + 128 * v;
-      if (d < DP) {
-        const float4 x = *reinterpret_cast<const float4 *>(o + d);
-        acc[v].x = fmaf(x.x, wt, acc[v].x);
-        acc[v].y = fmaf(x.y, wt, acc[v].y);
-        acc[v].z = fmaf(x.z, wt, acc[v].z);
-        acc[v].w = fmaf(x.w, wt, acc[v].w);
+        for (int v = 0; v < V; ++v) {
+          acc[v].x = acc[v].x * f + x[v].x * g;
+          acc[v].y = acc[v].y * f + x[v].y * g;
+          acc[v].z = acc[v].z * f + x[v].z * g;
+          acc[v].w = acc[v].w * f + x[v].w * g;
+        }
+      };
+      // Four parts' loads in flight.
+#pragma unroll 1
+      for (int p = many ? warp : 0; p < np; p += many ? 32 : 4) {
+        float2 ml[4];
+        float4 x[4][V];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int pp = p + (many ? 8 * q : q);
+          ml[q] = make_float2(-INFINITY, 0.0f);
+          const int64_t at = ((int64_t)(pp == 0 ? 2 * c0 + 1 : 2 * (c0 + pp))) * R + r;
+          if (pp < np) ml[q] = a.part_ml[at];
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            x[q][v] = make_float4(0, 0, 0, 0);
+            if (pp < np && 4 * lane + 128 * v < DP)
+              x[q][v] = *reinterpret_cast<const float4 *>(a.part_o + at * DP + 4 * lane + 128 * v);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) add(ml[q], x[q]);
       }
+      if (many) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (4 * lane + 128 * v < DP) s_o[warp][lane + 32 * v] = acc[v];
+        if (lane == 0) s_ml[warp] = make_float2(m, l);
+        __syncthreads();
+        if (warp == 0) {
+#pragma unroll 1
+          for (int q = 1; q < 8; ++q) {
+            float4 x[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+              x[v] = 4 * lane + 128 * v < DP ? s_o[q][lane + 32 * v] : make_float4(0, 0, 0, 0);
+            add(s_ml[q], x);
+          }
+        }
+      }
+      if (!many || warp == 0) {
+        AttnRow ar;
+        const int t = (w.row0 + r) / a.G;
+        ar.token = w.tok0 + t;
+        ar.head = w.h * a.G + w.row0 + r - t * a.G;
+        const AttnFinish f = attn_finish(a, ar, m, l);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          float x[4] = {acc[v].x, acc[v].y, acc[v].z, acc[v].w};
+          attn_store4(a, ar, f, 4 * lane + 128 * v, DP, x);
+        }
+        if (lane == 0) attn_store_lse(a, f);
+      }
+      if (many) __syncthreads();
     }
   }
-  const AttnRow ar = attn_row(a, s, w.y, row);
-  const AttnFinish f = attn_finish(a, ar, m, l);
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    float x[4] = {acc[v].x, acc[v].y, acc[v].z, acc[v].w};
-    attn_store<4>(a, ar, f, 4 * lane + 128 * v, DP, x);
-  }
-  if (lane == 0) attn_store_lse(a, f);
 }
 
 }  // namespace nvfp4

@@ -87,15 +87,17 @@ AttnLayout attn_layout(const nvfp4_attention_desc &d, const nvfp4_attention_batc
   L.dp = d.head_dim <= 64 ? 64 : d.head_dim <= 128 ? 128 : 256;
   L.R1 = rows_of(d, (int64_t)b.max_q_len * G);
   L.R0 = b.prefix_len > 0 ? rows_of(d, b.num_tokens * G) : 0;
-  const size_t R = L.R0 > L.R1 ? L.R0 : L.R1;
+  // Rows of parts: two per worker, of the larger pass.
+  auto part_rows = [&](int R) -> size_t { return (size_t)2 * grid * R * (R <= 32 ? kAttnRowsWorkers : 1); };
+  const size_t rows = part_rows(L.R0) > part_rows(L.R1) ? part_rows(L.R0) : part_rows(L.R1);
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   size_t at = 0;
   L.part_o = at;
-  at += up((size_t)2 * grid * R * L.dp * 4);
+  at += up(rows * L.dp * 4);
   L.part_ml = at;
-  at += up((size_t)2 * grid * R * 8);
+  at += up(rows * 8);
   L.meta = at;
-  at += up((size_t)grid * 16);
+  at += up((size_t)grid * kAttnRowsWorkers * sizeof(AttnMeta));
   L.prev_o = at;
   if (b.prefix_len > 0) at += up((size_t)b.num_tokens * d.num_heads * L.dp * 4);
   L.prev_lse = at;
@@ -110,7 +112,7 @@ int check_size(const nvfp4_attention_desc &d, const nvfp4_attention_batch &b, in
   const double keys = (double)b.max_pages * page_size, rows = (double)b.num_tokens * G;
   const AttnLayout L = attn_layout(d, b, 1);
   auto line = [&](int R, double n, double seqs) {
-    return d.num_kv_heads * (rows / R + seqs) * (n / 64 + 3);
+    return d.num_kv_heads * (rows / R + seqs) * (n / (R <= 32 ? attn_rows_tile(d.head_dim) : 64) + 8);
   };
   if (rows >= (double)(1ll << 30) || line(L.R1, keys, b.num_seqs) >= 2147483648.0 ||
       (b.prefix_len > 0 && line(L.R0, b.prefix_len, 1) >= 2147483648.0))
@@ -195,11 +197,12 @@ extern "C" int nvfp4_paged_attention(const nvfp4_attention_desc *desc, const nvf
   uint8_t *w = static_cast<uint8_t *>(ws);
   a.part_o = reinterpret_cast<float *>(w + L.part_o);
   a.part_ml = reinterpret_cast<float2 *>(w + L.part_ml);
-  a.meta = reinterpret_cast<int4 *>(w + L.meta);
+  a.meta = reinterpret_cast<AttnMeta *>(w + L.meta);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto pass = [&](int R, const char *what) -> int {
     // A box of the cache map: a page, or as much of it as a key tile takes.
-    const int box = cache->page_size < 64 ? cache->page_size : 64;
+    const int tile = R <= 32 ? attn_rows_tile(desc->head_dim) : 64;
+    const int box = cache->page_size < tile ? cache->page_size : tile;
     CUtensorMap tk, tv;
     if (!make_cache_map(&tk, cache->k, cache->k_strides, *cache, box) ||
         !make_cache_map(&tv, cache->v, cache->v_strides, *cache, box))

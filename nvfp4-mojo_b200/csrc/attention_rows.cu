@@ -2,13 +2,14 @@
 // tokens, a few tokens of speculative decoding) over the paged cache.
 //
 // Bound by HBM: every key and value is read once for the R = 16 or 32 rows
-// that share it, in one launch whose blocks divide all sequences' keys evenly
+// that share it, in one launch whose warps divide all sequences' keys evenly
 // (attention.cuh), so a batch of ragged lengths keeps every SM streaming to
-// the end.  One block per SM: a TMA producer warp keeps a ring of key and
-// value tiles of 64 tokens in flight (a box per page, 128-byte swizzle), four
-// warps each take 16 tokens of a tile: S = Q K^T and O += P V on mma.sync from
-// registers (16 rows would fill an eighth of a tcgen05 tile), a softmax state
-// (max, sum, O) per warp, no exchange between warps until the item ends.
+// the end.  Each of a block's four warps works alone, without a barrier: it
+// keeps a ring of tiles of 32 tokens (16 above head size 128) in flight by TMA
+// (a box per page, 128-byte swizzle), across the ends of its items, and turns
+// each into S = Q K^T, its softmax state and O += P V on mma.sync from registers
+// (16 rows would fill an eighth of a tcgen05 tile).  A cut item's parts go to
+// the workspace as they are; there is nothing to join within a block.
 #include <cuda_bf16.h>
 
 #include "../../include/nvfp4.h"
@@ -20,24 +21,21 @@
 namespace nvfp4 {
 
 static __device__ int g_attn_rows_status;
+static_assert(kAttnRowsWorkers == 4, "warps per block below");
 
 namespace {
 
-constexpr int kKT = 64;      // tokens per tile
-constexpr int kWarps = 4;    // consumer warps, 16 tokens of a tile each
-constexpr int kThreads = (kWarps + 1) * 32;
-constexpr int kMergeBytes = 32768;
-constexpr int kItemCost = 1;  // of an item's beginning and end, in tiles
+constexpr int kWarps = 4;
+constexpr int kItemCost = 2;  // of an item's beginning and end, in tiles
+constexpr int kSegs = 4;      // items that a warp's loads may be ahead
 
 template <int MT, int DP>
 struct RowsCfg {
   static constexpr int R = 16 * MT;
-  static constexpr int kTile = kKT * DP * 2;  // bytes of a key or value tile
-  static constexpr int kMaxSlots = (227 * 1024 - kMergeBytes - 1024 - 8192) / kTile;
-  static constexpr int kSlots = kMaxSlots > 16 ? 16 : kMaxSlots;
-  static constexpr int MC = kMergeBytes / (kWarps * R * 4) < DP ? kMergeBytes / (kWarps * R * 4) : DP;
-  static constexpr int offMerge = kSlots * kTile;
-  static constexpr int bytes = offMerge + kMergeBytes + 1024;
+  static constexpr int KT = DP <= 128 ? 32 : 16;  // tokens per tile
+  static constexpr int kTile = KT * DP * 2;       // bytes of a tile's keys, or values
+  static constexpr int kRing = DP == 64 ? 6 : 3;  // tiles in flight per warp
+  static constexpr int bytes = kWarps * kRing * 2 * kTile + 1024;
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -73,108 +71,118 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
       : "memory");
 }
 
-__device__ __forceinline__ void consumers_sync() {
-  asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
-}
-
 // MOD: scores are capped or biased.
 template <int MT, int DP, bool MOD>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kWarps * 32, 1)
     attn_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                      const __grid_constant__ AttnArgs a) {
   using C = RowsCfg<MT, DP>;
-  constexpr int R = C::R, kSlots = C::kSlots;
+  constexpr int R = C::R, KT = C::KT, kRing = C::kRing, NT = KT / 8;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                               ~static_cast<uintptr_t>(1023));
-  float *merge = reinterpret_cast<float *>(smem + C::offMerge);
   __shared__ AttnPlanSmem plan;
-  __shared__ uint64_t bars[2 * 16];
-  __shared__ float2 s_ml[kWarps][R];
-  __shared__ int abort_flag;
-  const uint32_t sbase = smem_u32(smem);
-  const uint32_t full = smem_u32(bars), empty = full + 8 * 16;
+  __shared__ uint64_t bars[kWarps * kRing];
+  __shared__ AttnSegment segs[kWarps][kSegs];
+  __shared__ AttnCursor curs[kWarps];
+  __shared__ int aborts[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t full = smem_u32(bars + warp * kRing);
+  uint8_t *ring = smem + warp * kRing * 2 * C::kTile;
+  const uint32_t rbase = smem_u32(ring);
 
   asm volatile("griddepcontrol.launch_dependents;");
-  if (threadIdx.x == 0) {
-    abort_flag = 0;
-    for (int i = 0; i < kSlots; ++i) {
-      mbar_init(full + 8 * i, 1);
-      mbar_init(empty + 8 * i, kWarps);
-    }
+  if (lane == 0) {
+    aborts[warp] = 0;
+    for (int i = 0; i < kRing; ++i) mbar_init(full + 8 * i, 1);
     mbar_fence_init();
     prefetch_tmap(&tmK);
     prefetch_tmap(&tmV);
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  AttnCursor cur = attn_plan<R, kKT, kItemCost>(a, 1 + kItemCost, &plan);
-  if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, -1);
-  volatile int *abort = &abort_flag;
-  AttnSegment g;
+  {
+    const AttnCursor c = attn_plan<R, KT, kItemCost, kWarps>(a, 1 + kItemCost, &plan);
+    if (lane == 0) {
+      curs[warp] = c;
+      a.meta[c.worker].last_part = -1;
+    }
+  }
+  __syncwarp();
+  volatile int *abort = &aborts[warp];
+  int *status = &g_attn_rows_status;
 
-  if (warp == kWarps) {
-    // ---------------- TMA producer ----------------
-    const uint64_t policy = l2_evict_first_policy();
-    const int box = a.page_size < kKT ? a.page_size : kKT;
-    const int per = kKT / box;  // boxes (pages) per tile and 64 columns
-    const int halves = DP / 64;
-    int slot = 0, round = 0;
-    bool ok = true;
-    while (ok && attn_segment<R, kKT, kItemCost>(a, cur, g)) {
-      const int *pages = a.page_table + (a.prefix_pass ? 0 : (int64_t)g.b * a.pt_stride);
-      int ids = 0, ids_at = -64;
-      for (int u = g.it.u0 + g.off; u < g.it.u0 + g.off + g.take && ok; ++u) {
-        const int j0 = u * kKT;
-        // This lane's box of the tile: rows j0 + i box .. of columns 64 hf.
-        const int i = lane % per, hf = lane / per;
-        const int tok = j0 + i * box;
-        const bool mine = hf < halves && tok < g.it.hi && tok + box > g.it.lo;
-        const int p0 = j0 >> a.page_shift, p1 = (j0 + kKT - 1) >> a.page_shift;
-        if (p1 >= ids_at + 32 || p0 < ids_at) {  // the next 32 page ids, one per lane
-          ids_at = p0;
-          const int last = (g.it.hi - 1) >> a.page_shift;
-          ids = pages[min(p0 + lane, last)];
+  // Loads run up to kRing tiles ahead of the arithmetic.  The items lie in
+  // shared memory; registers hold what every tile needs.
+  int l_left = 0, l_j0 = 0, l_lo = 0, l_hi = 0, l_h = 0;  // the item being loaded
+  const int *l_pages = nullptr;
+  int ids = 0, ids_at = -64;
+  int take = 0, j0 = 0, it_lo = 0, it_hi = 0;             // the item being computed: tiles left
+  uint32_t issued = 0, done = 0, pushed = 0, popped = 0;
+  bool more = true, have = false;
+  const int box = a.page_size < KT ? a.page_size : KT, per = KT / box;
+  // This lane's box of a tile: keys or values, rows i box .., columns 64 hf.
+  const int bi = lane % per, bh = (lane / per) % (DP / 64), bv = lane / (per * (DP / 64));
+  const uint64_t policy = l2_evict_first_policy();
+
+  const int qr = lane >> 2, qc = lane & 3;
+  const float sl2 = a.scale * kLog2e;
+  uint32_t qf[MT][DP / 16][4];
+  int lo[MT][2], hi[MT][2];
+  float slope[MT][2], dist[MT][2], m[MT][2], l[MT][2], o[MT][DP / 8][4];
+
+  while (true) {
+    // ---- loads
+#pragma unroll 1
+    while (more && issued - done < kRing && (l_left > 0 || pushed - popped < kSegs)) {
+      if (l_left == 0) {
+        AttnCursor c = curs[warp];
+        AttnSegment g;
+        more = attn_segment<R, KT, kItemCost>(a, c, g);
+        if (!more) break;
+        __syncwarp();
+        if (lane == 0) {
+          curs[warp] = c;
+          segs[warp][pushed % kSegs] = g;
         }
-        const int page = __shfl_sync(0xffffffffu, ids, ((tok >> a.page_shift) - ids_at) & 31);
-        const int row = tok & (a.page_size - 1);
-        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * box * 128;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          if (round > 0) {
-            const bool w = attn_wait(empty + 8 * slot, (round - 1) & 1, &g_attn_rows_status,
-                                     kDevTimeoutEmpty, abort);
-            if (!__all_sync(0xffffffffu, w)) {
-              ok = false;
-              break;
-            }
-          }
-          if (lane == 0) mbar_arrive_expect_tx(full + 8 * slot, bytes);
-          __syncwarp();
-          if (mine)
-            tma_load_4d(sbase + slot * C::kTile + hf * (kKT * 128) + i * box * 128, kv ? &tmV : &tmK,
-                        64 * hf, g.h, row, page, full + 8 * slot, policy);
-          if (++slot == kSlots) slot = 0, ++round;
-        }
+        __syncwarp();
+        ++pushed;
+        l_left = g.take;
+        l_j0 = (g.it.u0 + g.off) * KT;
+        l_lo = g.it.lo;
+        l_hi = g.it.hi;
+        l_h = g.h;
+        l_pages = a.page_table + (a.prefix_pass ? 0 : (int64_t)g.b * a.pt_stride);
+        ids_at = -64;
+        continue;
       }
+      const int tok = l_j0 + bi * box;
+      const bool mine = bv < 2 && tok < l_hi && tok + box > l_lo;
+      const int p0 = l_j0 >> a.page_shift, p1 = (l_j0 + KT - 1) >> a.page_shift;
+      if (p1 >= ids_at + 32) {  // the next 32 page ids, one per lane
+        ids_at = p0;
+        ids = l_pages[min(p0 + lane, (l_hi - 1) >> a.page_shift)];
+      }
+      l_j0 += KT;
+      --l_left;
+      const int page = __shfl_sync(0xffffffffu, ids, ((tok >> a.page_shift) - ids_at) & 31);
+      const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * box * 128;
+      const uint32_t st = issued % kRing;
+      if (lane == 0) mbar_arrive_expect_tx(full + 8 * st, bytes);
+      __syncwarp();
+      if (mine)
+        tma_load_4d(rbase + (2 * st + bv) * C::kTile + bh * (KT * 128) + bi * box * 128, bv ? &tmV : &tmK,
+                    64 * bh, l_h, tok & (a.page_size - 1), page, full + 8 * st, policy);
+      ++issued;
     }
-    // Drain: the block never exits with a copy still writing its memory.
-    const int issued = round * kSlots + slot;
-    for (int q = issued > kSlots ? issued - kSlots : 0; q < issued; ++q) {
-      volatile int no_abort = 0;
-      attn_wait(full + 8 * (q % kSlots), (q / kSlots) & 1, &g_attn_rows_status, kDevTimeoutFull, &no_abort);
-    }
-  } else {
-    // ---------------- consumers ----------------
-    const int qr = lane >> 2, qc = lane & 3;
-    const float sl2 = a.scale * kLog2e;
-    int slot = 0, round = 0;
-    bool ok = true;
-    while (ok && attn_segment<R, kKT, kItemCost>(a, cur, g)) {
-      // Q fragments and the rows' key intervals.
-      uint32_t qf[MT][DP / 16][4];
-      int lo[MT][2], hi[MT][2], pos[MT][2];
-      float slope[MT][2];
+    // ---- the next item
+    if (!have) {
+      if (popped == pushed) break;
+      const AttnSegment &g = segs[warp][popped % kSegs];
+      have = true;
+      take = g.take;
+      j0 = (g.it.u0 + g.off) * KT;
+      it_lo = g.it.lo;
+      it_hi = g.it.hi;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         const uint32_t *src[2];
@@ -185,9 +193,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           const AttnRow r = attn_row(a, g.s, g.h, in ? row : 0);
           lo[mt][e] = in ? r.lo : 0;
           hi[mt][e] = in ? r.hi : 0;
-          pos[mt][e] = r.pos - (a.prefix_pass ? 0 : a.prefix_len);
+          dist[mt][e] = (float)(r.pos - (a.prefix_pass ? 0 : a.prefix_len));
           slope[mt][e] = MOD && a.slopes ? a.slopes[r.head] * kLog2e : 0.0f;
           src[e] = in ? reinterpret_cast<const uint32_t *>(a.q + r.token * a.q_ts + r.head * a.q_hs) : nullptr;
+          m[mt][e] = -INFINITY;
+          l[mt][e] = 0.0f;
         }
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k)
@@ -196,145 +206,125 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int d = 16 * k + 8 * (x >> 1) + 2 * qc;
             qf[mt][k][x] = src[x & 1] && d < a.D ? src[x & 1][d >> 1] : 0u;
           }
-      }
-      float o[MT][DP / 8][4], m[MT][2], l[MT][2];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        m[mt][0] = m[mt][1] = -INFINITY;
-        l[mt][0] = l[mt][1] = 0.0f;
 #pragma unroll
         for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
           for (int x = 0; x < 4; ++x) o[mt][n][x] = 0.0f;
       }
-
-      for (int u = g.it.u0 + g.off; u < g.it.u0 + g.off + g.take; ++u) {
-        const int j0 = u * kKT + warp * 16;  // this warp's 16 tokens
-        const bool any = j0 < g.it.hi && j0 + 16 > g.it.lo;
-        float s[MT][2][4];
-        // ---- S = Q K^T
-        bool w = attn_wait(full + 8 * slot, round & 1, &g_attn_rows_status, kDevTimeoutFull, abort);
-        if (!__all_sync(0xffffffffu, w)) {
-          ok = false;
-          break;
-        }
-        if (any) {
+    }
+    // ---- a tile
+    if (take > 0) {
+      const uint32_t st = done % kRing;
+      if (!__all_sync(0xffffffffu, attn_wait(full + 8 * st, (done / kRing) & 1, status, kDevTimeoutFull, abort)))
+        break;
+      ++done;
+      const uint32_t kb0 = rbase + 2 * st * C::kTile, vb0 = kb0 + C::kTile;
+      float s[MT][NT][4];
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int x = 0; x < 8; ++x) s[mt][x >> 2][x & 3] = 0.0f;
-          // Matrix lane / 8: tokens 8 (lane / 16), columns 8 ((lane / 8) & 1).
-          const int t = warp * 16 + (lane & 7) + 8 * (lane >> 4), cc = (lane >> 3) & 1;
-          const uint32_t kb = sbase + slot * C::kTile + t * 128;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int k = 0; k < DP / 16; ++k) {
+          for (int x = 0; x < 4; ++x) s[mt][n][x] = 0.0f;
+      {  // S = Q K^T: matrix lane / 8 holds tokens 8 (lane / 16), columns 8 ((lane / 8) & 1)
+        const int t = (lane & 7) + 8 * (lane >> 4), cc = (lane >> 3) & 1;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+          for (int n = 0; n < NT; n += 2) {
             uint32_t b[4];
             const int c = (2 * k + cc) & 7;
-            ldsm4(kb + (k >> 2) * (kKT * 128) + ((c ^ (t & 7)) << 4), b);
+            ldsm4(kb0 + (k >> 2) * (KT * 128) + (t + 8 * n) * 128 + ((c ^ (t & 7)) << 4), b);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              mma_bf16(s[mt][0], qf[mt][k], b[0], b[1]);
-              mma_bf16(s[mt][1], qf[mt][k], b[2], b[3]);
+              mma_bf16(s[mt][n], qf[mt][k], b[0], b[1]);
+              mma_bf16(s[mt][n + 1], qf[mt][k], b[2], b[3]);
             }
           }
+      }
+      uint32_t p[MT][NT / 2][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int j = j0 + 8 * n + 2 * qc + x;
+              float v = s[mt][n][2 * e + x];
+              if constexpr (MOD) {
+                v *= a.scale;
+                if (a.softcap > 0.0f)  // cap tanh(v / cap)
+                  v = a.softcap - __fdividef(2.0f * a.softcap, 1.0f + ex2(v * (2.0f * kLog2e / a.softcap)));
+                v = fmaf(v, kLog2e, -slope[mt][e] * fabsf(dist[mt][e] - (float)j));
+              } else {
+                v *= sl2;
+              }
+              v = j >= lo[mt][e] && j < hi[mt][e] ? v : -INFINITY;
+              s[mt][n][2 * e + x] = v;
+              top = fmaxf(top, v);
+            }
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const float mn = fmaxf(m[mt][e], top);
+          const float mu = mn == -INFINITY ? 0.0f : mn;
+          if (__any_sync(0xffffffffu, mn > m[mt][e])) {
+            const float f = ex2(m[mt][e] - mu);
+            l[mt][e] *= f;
+#pragma unroll
+            for (int n = 0; n < DP / 8; ++n) {
+              o[mt][n][2 * e] *= f;
+              o[mt][n][2 * e + 1] *= f;
+            }
+            m[mt][e] = mn;
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const float p0 = ex2(s[mt][n][2 * e] - mu), p1 = ex2(s[mt][n][2 * e + 1] - mu);
+            l[mt][e] += p0 + p1;
+            // Rounded to bf16 for the second product only; the sum above
+            // keeps the unrounded values.
+            p[mt][n >> 1][2 * (n & 1) + e] = pack_bf16(p0, p1);
+          }
         }
-        fence_proxy_async_smem();
+      if (j0 < it_lo || j0 + KT > it_hi) {
+        // Tokens that no row sees (never loaded, or the rest of a page): their
+        // zero weights must not meet what lies there.
+        for (int x = lane; x < KT * (DP / 8); x += 32) {
+          const int t = x / (DP / 8), c = x % (DP / 8);
+          if (j0 + t < it_lo || j0 + t >= it_hi)
+            *reinterpret_cast<uint4 *>(ring + (2 * st + 1) * C::kTile + (c >> 3) * (KT * 128) + t * 128 +
+                                       (((c & 7) ^ (t & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+        }
         __syncwarp();
-        if (lane == 0) mbar_arrive(empty + 8 * slot);
-        if (++slot == kSlots) slot = 0, ++round;
-        // ---- softmax of this warp's 16 tokens
-        uint32_t p[MT][4];
-        if (any) {
+      }
+      {  // O += P V: matrix lane / 8 holds tokens 8 ((lane / 8) & 1), columns 8 (lane / 16)
+        const int t = lane & 15, cc = lane >> 4;
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float top = -INFINITY;
-#pragma unroll
-              for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                  const int j = j0 + 8 * n + 2 * qc + x;
-                  float v = s[mt][n][2 * e + x];
-                  if constexpr (MOD) {
-                    v *= a.scale;
-                    if (a.softcap > 0.0f)  // cap tanh(v / cap)
-                      v = a.softcap - __fdividef(2.0f * a.softcap, 1.0f + ex2(v * (2.0f * kLog2e / a.softcap)));
-                    v = fmaf(v, kLog2e, -slope[mt][e] * fabsf((float)(pos[mt][e] - j)));
-                  } else {
-                    v *= sl2;
-                  }
-                  v = j >= lo[mt][e] && j < hi[mt][e] ? v : -INFINITY;
-                  s[mt][n][2 * e + x] = v;
-                  top = fmaxf(top, v);
-                }
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-              const float mn = fmaxf(m[mt][e], top);
-              const float mu = mn == -INFINITY ? 0.0f : mn;
-              if (__any_sync(0xffffffffu, mn > m[mt][e])) {
-                const float f = ex2(m[mt][e] - mu);
-                l[mt][e] *= f;
-#pragma unroll
-                for (int n = 0; n < DP / 8; ++n) {
-                  o[mt][n][2 * e] *= f;
-                  o[mt][n][2 * e + 1] *= f;
-                }
-                m[mt][e] = mn;
-              }
-#pragma unroll
-              for (int n = 0; n < 2; ++n) {
-                const float p0 = ex2(s[mt][n][2 * e] - mu), p1 = ex2(s[mt][n][2 * e + 1] - mu);
-                l[mt][e] += p0 + p1;
-                // Rounded to bf16 for the second product only; the sum above
-                // keeps the unrounded values.
-                p[mt][2 * n + e] = pack_bf16(p0, p1);
-              }
-            }
-          }
-        }
-        // ---- O += P V
-        w = attn_wait(full + 8 * slot, round & 1, &g_attn_rows_status, kDevTimeoutFull, abort);
-        if (!__all_sync(0xffffffffu, w)) {
-          ok = false;
-          break;
-        }
-        if (any) {
-          const uint32_t vb0 = sbase + slot * C::kTile;
-          if (j0 < g.it.lo || j0 + 16 > g.it.hi) {
-            // Tokens that no row sees (never loaded, or the rest of a page):
-            // their zero weights must not meet what lies there.
-            for (int x = lane; x < 16 * (DP / 8); x += 32) {
-              const int tt = warp * 16 + x / (DP / 8), j = j0 + x / (DP / 8), c = x % (DP / 8);
-              if (j < g.it.lo || j >= g.it.hi)
-                *reinterpret_cast<uint4 *>(smem + slot * C::kTile + (c >> 3) * (kKT * 128) + tt * 128 +
-                                           (((c & 7) ^ (tt & 7)) << 4)) = make_uint4(0, 0, 0, 0);
-            }
-            __syncwarp();
-          }
-          // Matrix lane / 8: tokens 8 ((lane / 8) & 1), columns 8 (lane / 16).
-          const int t = warp * 16 + (lane & 15), cc = lane >> 4;
-          const uint32_t vb = vb0 + t * 128;
+        for (int k = 0; k < NT / 2; ++k)
 #pragma unroll
           for (int n = 0; n < DP / 16; ++n) {
             uint32_t b[4];
             const int c = (2 * n + cc) & 7;
-            ldsm4t(vb + (n >> 2) * (kKT * 128) + ((c ^ (t & 7)) << 4), b);
+            ldsm4t(vb0 + (n >> 2) * (KT * 128) + (t + 16 * k) * 128 + ((c ^ (t & 7)) << 4), b);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              mma_bf16(o[mt][2 * n], p[mt], b[0], b[1]);
-              mma_bf16(o[mt][2 * n + 1], p[mt], b[2], b[3]);
+              mma_bf16(o[mt][2 * n], p[mt][k], b[0], b[1]);
+              mma_bf16(o[mt][2 * n + 1], p[mt][k], b[2], b[3]);
             }
           }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(empty + 8 * slot);
-        if (++slot == kSlots) slot = 0, ++round;
       }
-      if (!ok) break;
-
-      // ---- the four warps' states joined, MC columns at a time
+      // The tile's reads (and zeros) come before the copy that refills it.
+      fence_proxy_async_smem();
+      __syncwarp();
+      j0 += KT;
+      --take;
+    }
+    // ---- the item's end
+    if (take == 0) {
+      const AttnSegment &g = segs[warp][popped % kSegs];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -342,55 +332,66 @@ __global__ void __launch_bounds__(kThreads, 1)
           float x = l[mt][e];
           x += __shfl_xor_sync(0xffffffffu, x, 1);
           x += __shfl_xor_sync(0xffffffffu, x, 2);
-          if (qc == 0) s_ml[warp][mt * 16 + e * 8 + qr] = make_float2(m[mt][e], x);
-        }
-      constexpr int MC = C::MC;
-#pragma unroll
-      for (int c0 = 0; c0 < DP; c0 += MC) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int n = 0; n < MC / 8; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              *reinterpret_cast<float2 *>(merge + (warp * R + mt * 16 + e * 8 + qr) * MC + 8 * n + 2 * qc) =
-                  make_float2(o[mt][c0 / 8 + n][2 * e], o[mt][c0 / 8 + n][2 * e + 1]);
-        consumers_sync();
-        for (int x = threadIdx.x; x < R * (MC / 4); x += kWarps * 32) {
-          const int r = x / (MC / 4), d = 4 * (x % (MC / 4));
-          const int row = g.rb * R + r;
+          const int r = mt * 16 + e * 8 + qr, row = g.rb * R + r;
           if (row >= g.s.ql * a.G) continue;
-          float mm = -INFINITY;
+          if (g.slot >= 0) {
+            const int64_t at = (int64_t)g.slot * R + r;
+            if (qc == 0) a.part_ml[at] = make_float2(m[mt][e], x);
+            float *dst = a.part_o + at * DP + 2 * qc;
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_ml[w][r].x);
-          const float mu = mm == -INFINITY ? 0.0f : mm;
-          float ll = 0.0f;
-          float4 acc = make_float4(0, 0, 0, 0);
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            const float f = ex2(s_ml[w][r].x - mu);
-            ll = fmaf(s_ml[w][r].y, f, ll);
-            const float4 v = *reinterpret_cast<const float4 *>(merge + (w * R + r) * MC + d);
-            acc.x = fmaf(v.x, f, acc.x);
-            acc.y = fmaf(v.y, f, acc.y);
-            acc.z = fmaf(v.z, f, acc.z);
-            acc.w = fmaf(v.w, f, acc.w);
+            for (int n = 0; n < DP / 8; ++n)
+              *reinterpret_cast<float2 *>(dst + 8 * n) = make_float2(o[mt][n][2 * e], o[mt][n][2 * e + 1]);
+            continue;
           }
-          if (g.slot < 0) {
-            const AttnRow ar = attn_row(a, g.s, g.h, row);
-            const AttnFinish f = attn_finish(a, ar, mm, ll);
-            float x[4] = {acc.x, acc.y, acc.z, acc.w};
-            attn_store<4>(a, ar, f, c0 + d, DP, x);
-            if (c0 + d == 0) attn_store_lse(a, f);
-          } else {
-            *reinterpret_cast<float4 *>(a.part_o + ((int64_t)g.slot * R + r) * DP + c0 + d) = acc;
-            if (c0 + d == 0) a.part_ml[(int64_t)g.slot * R + r] = make_float2(mm, ll);
+          const AttnRow ar = attn_row(a, g.s, g.h, row);
+          const AttnFinish f = attn_finish(a, ar, m[mt][e], x);
+          if (qc == 0) attn_store_lse(a, f);
+          const int64_t pat = f.id * DP + 2 * qc;
+          if (a.prefix_pass) {
+#pragma unroll
+            for (int n = 0; n < DP / 8; ++n)
+              *reinterpret_cast<float2 *>(a.prev_o + pat + 8 * n) =
+                  f.so == 0.0f ? make_float2(0.0f, 0.0f)
+                               : make_float2(o[mt][n][2 * e] * f.so, o[mt][n][2 * e + 1] * f.so);
+            continue;
+          }
+          const __nv_bfloat16 *gate = a.gate + ar.token * a.g_ts + ar.head * a.g_hs + 2 * qc;
+          __nv_bfloat16 *dst = a.out + ar.token * a.o_ts + ar.head * a.o_hs + 2 * qc;
+#pragma unroll
+          for (int n0 = 0; n0 < DP / 8; n0 += 8) {
+            uint32_t w[8];
+            float2 q[8];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {  // in flight together
+              w[n] = 0u;
+              q[n] = make_float2(0.0f, 0.0f);
+              if (a.gate && 8 * (n0 + n) < a.D) w[n] = *reinterpret_cast<const uint32_t *>(gate + 8 * (n0 + n));
+              if (a.prev_o && f.sp != 0.0f) q[n] = *reinterpret_cast<const float2 *>(a.prev_o + pat + 8 * (n0 + n));
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+              float v0 = f.so == 0.0f ? 0.0f : o[mt][n0 + n][2 * e] * f.so;
+              float v1 = f.so == 0.0f ? 0.0f : o[mt][n0 + n][2 * e + 1] * f.so;
+              v0 = fmaf(q[n].x, f.sp, v0);
+              v1 = fmaf(q[n].y, f.sp, v1);
+              if (a.gate) {
+                v0 *= sigmoidf(__uint_as_float(w[n] << 16));
+                v1 *= sigmoidf(__uint_as_float(w[n] & 0xffff0000u));
+              }
+              if (8 * (n0 + n) < a.D) *reinterpret_cast<uint32_t *>(dst + 8 * (n0 + n)) = pack_bf16(v0, v1);
+            }
           }
         }
-        consumers_sync();
-      }
-      if (g.last_part >= 0 && threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(g.b, g.h, g.rb, g.last_part);
+      if (g.last_part >= 0 && lane == 0) a.meta[blockIdx.x * kWarps + warp] = attn_meta<R>(a, g);
+      __syncwarp();
+      ++popped;
+      have = false;
     }
+  }
+  // Drain: the block never exits with a copy still writing its memory.
+  for (; done < issued; ++done) {
+    volatile int no_abort = 0;
+    attn_wait(full + 8 * (done % kRing), (done / kRing) & 1, status, kDevTimeoutFull, &no_abort);
   }
 }
 
@@ -404,7 +405,7 @@ cudaError_t launch_rows(const CUtensorMap &tk, const CUtensorMap &tv, const Attn
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid, 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.blockDim = dim3(kWarps * 32, 1, 1);
   cfg.dynamicSmemBytes = C::bytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -413,10 +414,11 @@ cudaError_t launch_rows(const CUtensorMap &tk, const CUtensorMap &tv, const Attn
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if ((e = cudaLaunchKernelEx(&cfg, k, tk, tv, a)) != cudaSuccess) return e;
-  cfg.gridDim = dim3((unsigned)grid, C::R / 4, 1);
-  cfg.blockDim = dim3(128, 1, 1);
+  constexpr int RPB = 2;
+  cfg.gridDim = dim3((unsigned)grid, C::R / RPB, 1);
+  cfg.blockDim = dim3(256, 1, 1);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, attn_join_kernel<C::R, kKT, DP>, a);
+  return cudaLaunchKernelEx(&cfg, attn_join_kernel<C::R, DP, kWarps, RPB>, a);
 }
 
 }  // namespace

@@ -239,11 +239,11 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
     tmem_relinquish();
   }
   tc_fence_before();
-  AttnCursor cur = attn_plan<R, KT, kItemCost>(a, 2 + kItemCost, &plan);  // ends with __syncthreads
+  AttnCursor cur = attn_plan<R, KT, kItemCost, 0>(a, 2 + kItemCost, &plan);  // ends with __syncthreads
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;");
   const uint32_t tmem = tmem_slot;
-  if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, -1);
+  if (threadIdx.x == 0) a.meta[blockIdx.x].last_part = -1;
   volatile int *abort = &abort_flag;
   int *status = &g_attn_tc_status;
   AttnSegment g;
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       const int take = g.take, slot = g.slot, j_first = (g.it.u0 + g.off) * KT;
       const int row = g.rb * R + my;
       const bool in = mine && row < g.s.ql * a.G;
-      if (g.last_part >= 0 && threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(g.b, g.h, g.rb, g.last_part);
+      if (g.last_part >= 0 && threadIdx.x == 0) a.meta[blockIdx.x] = attn_meta<R>(a, g);
       AttnRow ar = attn_row(a, g.s, g.h, in ? row : 0);
       if (!in) ar.lo = ar.hi = 0;
       float m = -INFINITY, l = 0.0f;
@@ -731,10 +731,11 @@ cudaError_t launch_tc(const CUtensorMap &tk, const CUtensorMap &tv, const AttnAr
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if ((e = cudaLaunchKernelEx(&cfg, k, tk, tv, a)) != cudaSuccess) return e;
-  cfg.gridDim = dim3((unsigned)grid, C::R / 4, 1);
-  cfg.blockDim = dim3(128, 1, 1);
+  constexpr int RPB = 16;
+  cfg.gridDim = dim3((unsigned)grid, C::R / RPB, 1);
+  cfg.blockDim = dim3(256, 1, 1);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, attn_join_kernel<C::R, KT, DP>, a);
+  return cudaLaunchKernelEx(&cfg, attn_join_kernel<C::R, DP, 1, RPB>, a);
 }
 
 }  // namespace
