@@ -1,5 +1,6 @@
 // attention_abi.cu -- nvfp4_paged_attention: checks, the workspace's layout
 // and the passes (include/nvfp4_attention.h).
+#include <atomic>
 #include <cmath>
 
 #include "../../include/nvfp4.h"
@@ -43,11 +44,23 @@ static bool make_cache_map(CUtensorMap *m, void *base, const int64_t (&st)[3], c
 }
 
 static int attn_sms() {
+  static std::atomic<int> count[64];  // per device
   int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
-    n = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if ((n = count[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+  count[dev].store(n, std::memory_order_relaxed);
   return n;
+}
+
+cudaError_t attn_allow_smem(const void *kernel, int bytes, std::atomic<uint64_t> &devices) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && (devices.load(std::memory_order_relaxed) >> dev & 1)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) devices.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return e;
 }
 
 namespace {

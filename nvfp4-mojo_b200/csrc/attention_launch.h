@@ -1,9 +1,15 @@
 // attention_launch.h -- host launchers of the attention kernels.
 #pragma once
 
+#include <atomic>
+
 #include "attention.cuh"
 
 namespace nvfp4 {
+
+// Lets a kernel use `bytes` of dynamic shared memory on the current device;
+// `devices` remembers where that has been done.
+cudaError_t attn_allow_smem(const void *kernel, int bytes, std::atomic<uint64_t> &devices);
 
 // attention_rows.cu: items of R = 16 or 32 rows (16 above head size 128), and
 // the launch that joins what its workers (warps) cut.  Key tiles of

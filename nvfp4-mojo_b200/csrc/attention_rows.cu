@@ -401,7 +401,8 @@ cudaError_t launch_rows(const CUtensorMap &tk, const CUtensorMap &tv, const Attn
   using C = RowsCfg<MT, DP>;
   const bool mod = a.softcap > 0.0f || a.slopes;
   auto k = mod ? attn_rows_kernel<MT, DP, true> : attn_rows_kernel<MT, DP, false>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::bytes);
+  static std::atomic<uint64_t> allowed[2];
+  cudaError_t e = attn_allow_smem(reinterpret_cast<const void *>(k), C::bytes, allowed[mod]);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid, 1, 1);

@@ -717,8 +717,10 @@ template <int DP>
 cudaError_t launch_tc(const CUtensorMap &tk, const CUtensorMap &tv, const AttnArgs &a, int grid,
                       cudaStream_t st) {
   using C = TcCfg<DP>;
-  auto k = a.softcap > 0.0f || a.slopes ? attn_tc_kernel<DP, true> : attn_tc_kernel<DP, false>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::bytes);
+  const bool mod = a.softcap > 0.0f || a.slopes;
+  auto k = mod ? attn_tc_kernel<DP, true> : attn_tc_kernel<DP, false>;
+  static std::atomic<uint64_t> allowed[2];
+  cudaError_t e = attn_allow_smem(reinterpret_cast<const void *>(k), C::bytes, allowed[mod]);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid, 1, 1);

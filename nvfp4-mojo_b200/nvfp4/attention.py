@@ -8,7 +8,6 @@ for every layer.  They keep their tensors alive and read no device memory.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 from typing import Optional
@@ -17,64 +16,49 @@ import torch
 
 from . import _lib
 
+_byref = ctypes.byref
 _DT = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
 
-class _Here:
-    """The calling stream as a raw handle, and nothing to restore."""
-
-    __slots__ = ("st",)
-
-    def __init__(self, st):
-        self.st = st
-
-    def __enter__(self):
-        return self.st
-
-    def __exit__(self, *_):
-        return False
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
-class _Elsewhere:
-    """The same while another device than the tensors' is the current one."""
-
-    def __init__(self, device, st):
-        self.guard, self.st = torch.cuda.device(device), st
-
-    def __enter__(self):
-        self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream if self.st is None else self.st
-
-    def __exit__(self, *e):
-        return self.guard.__exit__(*e)
-
-
-def _call_stream(t: torch.Tensor, stream):
-    """Context in which t's device is current; yields the raw stream (None:
-    the current stream of t's device)."""
-    if stream is not None:
-        stream = stream.cuda_stream if isinstance(stream, torch.cuda.Stream) else int(stream)
-    if t.get_device() != torch.cuda.current_device():
-        return _Elsewhere(t.device, stream)
-    return _Here(torch._C._cuda_getCurrentRawStream(t.get_device()) if stream is None else stream)
-
-
-def _on_stream(t: torch.Tensor, stream):
-    """Context for allocations that the call on `stream` uses: the memory
-    belongs to that stream, not to the current one."""
+def _launch(t: torch.Tensor, stream, fn, *args) -> None:
+    """fn(*args, stream) with t's device current; stream None: the current one
+    of t's device.  Raises what fn reports."""
+    dev = t.get_device()
     if stream is None:
-        return contextlib.nullcontext()
-    if not isinstance(stream, torch.cuda.Stream):
-        stream = torch.cuda.ExternalStream(int(stream), device=t.device)
-    return torch.cuda.stream(stream)
+        stream = _raw_stream(dev)
+    elif isinstance(stream, torch.cuda.Stream):
+        stream = stream.cuda_stream
+    if dev == _current_device():
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc)
+
+
+def _new(t: torch.Tensor, stream, shape, dtype) -> torch.Tensor:
+    """Memory on t's device that belongs to the stream of the call."""
+    if stream is not None:
+        if not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(int(stream), device=t.device)
+        with torch.cuda.stream(stream):
+            return torch.empty(shape, dtype=dtype, device=t.device)
+    if t.dtype is dtype and t.shape == shape and t.is_contiguous():
+        return torch.empty_like(t)
+    return t.new_empty(shape, dtype=dtype)
 
 
 def _check_device(t: torch.Tensor, **others) -> None:
-    if not t.is_cuda:
-        raise ValueError("tensors must be CUDA tensors (there is no CPU path)")
     d = t.get_device()
+    if d < 0:
+        raise ValueError("tensors must be CUDA tensors (there is no CPU path)")
     for name, o in others.items():
-        if o is not None and (not o.is_cuda or o.get_device() != d):
+        if o is not None and o.get_device() != d:
             raise ValueError(f"{name} must be a CUDA tensor on {t.device}")
 
 
@@ -100,7 +84,7 @@ class PagedKVCache:
         if k.stride(3) != 1 or v.stride(3) != 1:
             raise ValueError("head rows must be contiguous")
         _check_device(k, v=v)
-        self.k, self.v = k, v
+        self.k, self.v, self.device = k, v, k.get_device()
         n, self.page_size, self.num_kv_heads, self.head_dim = k.shape
         s = ctypes.c_int64 * 3
         self._c = _lib.KvCache(k.data_ptr(), v.data_ptr(), s(*k.stride()[:3]), s(*v.stride()[:3]),
@@ -209,12 +193,6 @@ def _head_rows(t: torch.Tensor, name: str, tokens: int, heads: int, dim: int) ->
     return _lib.HeadRows(t.data_ptr(), s[0], s[1])
 
 
-def _same_device(device: int, **others) -> None:
-    for name, o in others.items():
-        if o is not None and o.device != device:
-            raise ValueError(f"{name} is on another device than the tensors")
-
-
 def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: PagedKVCache,
               batch: AttentionBatch, rotary: Optional[Rotary] = None,
               positions: Optional[torch.Tensor] = None, q_norm: Optional[torch.Tensor] = None,
@@ -231,23 +209,30 @@ def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: PagedKVC
     bf16 [T, num_heads, D]; it may be q."""
     L = _lib.load()
     T, D = batch.num_tokens, cache.head_dim
-    if q.dtype not in _DT or k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype = q.dtype
+    if dtype not in _DT or k.dtype is not dtype or v.dtype is not dtype:
         raise TypeError("q, k and v must all be bf16 or all fp32")
     H = q.shape[1] if q.dim() == 3 else 0
     rq = _head_rows(q, "q", T, H, D)
     rk = _head_rows(k, "k", T, cache.num_kv_heads, D)
     rv = _head_rows(v, "v", T, cache.num_kv_heads, D)
     if q_out is None:
-        with _on_stream(q, stream):
-            q_out = torch.empty((T, H, D), dtype=torch.bfloat16, device=q.device)
-    elif q_out.dtype != torch.bfloat16:
+        q_out = _new(q, stream, (T, H, D), torch.bfloat16)
+    elif q_out.dtype is not torch.bfloat16:
         raise TypeError("q_out must be bf16")
     ro = _head_rows(q_out, "q_out", T, H, D)
+    dev = q.get_device()
+    if dev < 0 or k.get_device() != dev or v.get_device() != dev or q_out.get_device() != dev or \
+            cache.device != dev or batch.device != dev or \
+            (rotary is not None and rotary.device != dev):
+        raise ValueError("q, k, v, q_out, cache, batch and rotary must be on one CUDA device")
     pos, stride, axes = None, 0, 1
     if positions is not None:
-        if positions.dtype != torch.int32 or positions.dim() not in (1, 2) or \
+        if positions.dtype is not torch.int32 or positions.dim() not in (1, 2) or \
                 positions.shape[-1] != T or (T > 1 and positions.stride(-1) != 1):
             raise ValueError("positions must be int32 [T] or [axes, T] with contiguous rows")
+        if positions.get_device() != dev:
+            raise ValueError("positions must be on the tensors' device")
         pos = positions.data_ptr()
         if positions.dim() == 2:
             axes, stride = positions.shape[0], max(positions.stride(0), T)
@@ -256,31 +241,31 @@ def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: PagedKVC
     norm = None
     if q_norm is not None or k_norm is not None:
         for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-            if w is not None and (w.dtype != torch.bfloat16 or w.shape != (D,) or not w.is_contiguous()):
-                raise ValueError(f"{name} must be contiguous bf16 [head_dim]")
-        norm = ctypes.byref(_lib.QkNorm(None if q_norm is None else q_norm.data_ptr(),
-                                        None if k_norm is None else k_norm.data_ptr(), norm_eps,
-                                        norm_offset))
-    _check_device(q, k=k, v=v, cache=cache.k, positions=positions, q_norm=q_norm, k_norm=k_norm,
-                  q_out=q_out)
-    _same_device(q.get_device(), batch=batch, rotary=rotary)
-    with _call_stream(q, stream) as st:
-        rc = L.nvfp4_kv_append(cache._ref, batch._ref, None if rotary is None else rotary._ref, norm,
-                               ctypes.byref(rq), ctypes.byref(rk), ctypes.byref(rv), _DT[q.dtype], H,
-                               pos, stride, axes, ctypes.byref(ro), st)
-    _lib.check(rc)
+            if w is not None and (w.dtype is not torch.bfloat16 or w.shape != (D,) or
+                                  not w.is_contiguous() or w.get_device() != dev):
+                raise ValueError(f"{name} must be contiguous bf16 [head_dim] on the tensors' device")
+        norm = _byref(_lib.QkNorm(None if q_norm is None else q_norm.data_ptr(),
+                                  None if k_norm is None else k_norm.data_ptr(), norm_eps,
+                                  norm_offset))
+    _launch(q, stream, L.nvfp4_kv_append, cache._ref, batch._ref,
+            None if rotary is None else rotary._ref, norm, _byref(rq), _byref(rk), _byref(rv),
+            _DT[dtype], H, pos, stride, axes, _byref(ro))
     return q_out
 
 
-def attention_workspace(config: AttentionConfig, batch: AttentionBatch, device="cuda") -> torch.Tensor:
-    """A workspace for `paged_attention` calls of this shape (or any smaller
-    one: fewer tokens, a shorter max_q_len), one call at a time."""
+def _workspace_bytes(config: AttentionConfig, batch: AttentionBatch, device) -> int:
     L = _lib.load()
     with torch.cuda.device(device):
         need = L.nvfp4_attention_workspace_size(config._ref, batch._ref)
     if need == 0:
         raise ValueError("unsupported attention: " + L.nvfp4_last_error_string().decode())
-    return torch.empty(need, dtype=torch.uint8, device=device)
+    return need
+
+
+def attention_workspace(config: AttentionConfig, batch: AttentionBatch, device="cuda") -> torch.Tensor:
+    """A workspace for `paged_attention` calls of this shape (or any smaller
+    one: fewer tokens, a shorter max_q_len), one call at a time."""
+    return torch.empty(_workspace_bytes(config, batch, device), dtype=torch.uint8, device=device)
 
 
 def paged_attention(q: torch.Tensor, cache: PagedKVCache, batch: AttentionBatch,
@@ -297,36 +282,35 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, batch: AttentionBatch,
     and -inf.  `workspace`: from `attention_workspace` (None: allocated)."""
     L = _lib.load()
     T, H, D = batch.num_tokens, config.num_heads, config.head_dim
-    if q.dtype != torch.bfloat16:
+    bf16 = torch.bfloat16
+    if q.dtype is not bf16:
         raise TypeError("q must be bf16")
     rq = _head_rows(q, "q", T, H, D)
-    lse = None
-    if out is None or return_lse or workspace is None:
-        with _on_stream(q, stream):
-            if out is None:
-                out = torch.empty((T, H, D), dtype=torch.bfloat16, device=q.device)
-            if return_lse:
-                lse = torch.empty((T, H), dtype=torch.float32, device=q.device)
-            if workspace is None:
-                workspace = attention_workspace(config, batch, q.device)
-    if out.dtype != torch.bfloat16 or (gate is not None and gate.dtype != torch.bfloat16):
+    if out is None:
+        out = _new(q, stream, (T, H, D), bf16)
+    lse = _new(q, stream, (T, H), torch.float32) if return_lse else None
+    if workspace is None:
+        workspace = _new(q, stream, _workspace_bytes(config, batch, q.get_device()), torch.uint8)
+    if out.dtype is not bf16 or (gate is not None and gate.dtype is not bf16):
         raise TypeError("out and gate must be bf16")
     ro = _head_rows(out, "out", T, H, D)
-    rg = None if gate is None else ctypes.byref(_head_rows(gate, "gate", T, H, D))
-    if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (H,) or
+    rg = None if gate is None else _byref(_head_rows(gate, "gate", T, H, D))
+    if slopes is not None and (slopes.dtype is not torch.float32 or slopes.shape != (H,) or
                                not slopes.is_contiguous()):
         raise ValueError("slopes must be contiguous fp32 [num_heads]")
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
     if batch.prefix_len:
         batch._check_pages(cache.page_size)
-    _check_device(q, cache=cache.k, slopes=slopes, gate=gate, out=out, workspace=workspace)
-    _same_device(q.get_device(), batch=batch)
-    with _call_stream(q, stream) as st:
-        rc = L.nvfp4_paged_attention(config._ref, ctypes.byref(rq), cache._ref, batch._ref,
-                                     None if slopes is None else slopes.data_ptr(), rg,
-                                     ctypes.byref(ro), None if lse is None else lse.data_ptr(),
-                                     workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-                                     st)
-    _lib.check(rc)
+    dev = q.get_device()
+    if dev < 0 or out.get_device() != dev or workspace.get_device() != dev or \
+            cache.device != dev or batch.device != dev or \
+            (gate is not None and gate.get_device() != dev) or \
+            (slopes is not None and slopes.get_device() != dev):
+        raise ValueError("q, out, gate, slopes, workspace, cache and batch must be on one CUDA device")
+    _launch(q, stream, L.nvfp4_paged_attention, config._ref, _byref(rq), cache._ref, batch._ref,
+            None if slopes is None else slopes.data_ptr(), rg, _byref(ro),
+            None if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.nbytes)
     return (out, lse) if return_lse else out
 
 
