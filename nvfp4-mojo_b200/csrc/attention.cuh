@@ -42,6 +42,7 @@ struct AttnArgs {
   int prefix_pass;  // 1: all tokens against the shared prefix; 0: own keys
   int causal, window;
   int max_blocks;   // bound on items per sequence and head (max_q_len)
+  int wide;         // a copy brings all columns of its rows, not 64 of them
   float scale, softcap;
   const float *slopes;
   const __nv_bfloat16 *q, *gate;
@@ -61,6 +62,16 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// a / b for 0 <= a < 2^31, b > 0: the hardware's reciprocal, corrected (the
+// plain quotient is several times as long, and much of a short call's time).
+__device__ __forceinline__ int div_pos(int a, int b) {
+  int q = (int)__fdividef((float)a, (float)b);
+  int r = a - q * b;
+  while (r < 0) --q, r += b;
+  while (r >= b) ++q, r -= b;
+  return q;
 }
 
 // One sequence of a pass: its tokens, its keys in this pass and where the
@@ -108,7 +119,7 @@ struct AttnRow {
 
 __device__ __forceinline__ AttnRow attn_row(const AttnArgs &a, const AttnSeq &s, int h, int row) {
   AttnRow r;
-  const int i = row / a.G;
+  const int i = div_pos(row, a.G);
   r.head = h * a.G + (row - i * a.G);
   r.token = s.tok0 + i;
   r.lo = r.hi = 0;
@@ -158,7 +169,7 @@ __device__ __forceinline__ AttnItem attn_item(const AttnArgs &a, const AttnSeq &
     it.hi = s.n;
   } else {
     const int rows = s.ql * a.G;
-    const int i0 = rb * R / a.G, i1 = (min((rb + 1) * R, rows) - 1) / a.G;
+    const int i0 = rb ? div_pos(rb * R, a.G) : 0, i1 = (rb + 1) * R < rows ? div_pos((rb + 1) * R - 1, a.G) : s.ql - 1;
     it.lo = attn_interval(a, s.pos0 + i0, s.vis, s.n).x;
     it.hi = attn_interval(a, s.pos0 + i1, s.vis, s.n).y;
   }
@@ -200,6 +211,21 @@ __device__ __forceinline__ bool attn_wait(uint32_t bar, uint32_t parity, int *st
   return ok;
 }
 
+// A box of the cache map into this block's shared memory: slots of one head and
+// page, 64 columns from x on (or, wide, all of them, 64 columns after 64).
+__device__ __forceinline__ void attn_load_box(uint32_t dst, const CUtensorMap *map, int x, int slot, int h, int page,
+                                              uint32_t bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7], %8;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(slot), "r"(0), "r"(h), "r"(page), "r"(bar), "l"(policy)
+      : "memory");
+}
+__device__ __forceinline__ uint64_t l2_evict_normal_policy() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
 // Where a worker starts on the line, and how far it goes.
 struct AttnCursor {
   int b, h, rb, off;  // item and unit within it
@@ -211,8 +237,8 @@ struct AttnCursor {
 // The first unit of part c: floor(c total / parts), in 32 bits (c and parts are
 // at most a few hundred).
 __device__ __forceinline__ int attn_line_at(int c, int total, int parts) {
-  const int q = total / parts, r = total - q * parts;
-  return c * q + c * r / parts;
+  const int q = div_pos(total, parts), r = total - q * parts;
+  return c * q + div_pos(c * r, parts);
 }
 
 struct AttnPlanSmem {
@@ -238,9 +264,9 @@ __device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units
     return u;
   };
   // Sequences of few items: a thread each; of many: a warp each.  For up to
-  // 128 sequences of few items each warp that works alone plans alone.
+  // 32 sequences of few items each warp that works alone plans alone.
   const bool by_warp = a.max_blocks > 4;
-  const bool alone = WARPS && !by_warp && NS <= 128;
+  const bool alone = WARPS && !by_warp && NS <= 32;
   int sum = 0;
 #pragma unroll 1
   for (int b = alone ? lane : by_warp ? warp : tid; b < NS; b += alone ? 32 : by_warp ? nw : (int)blockDim.x) {
@@ -262,7 +288,7 @@ __device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units
   if (warp < (WARPS ? WARPS : 1)) {
     c.worker = WARPS ? blockIdx.x * WARPS + warp : blockIdx.x;
     c.total = a.Hkv * sum;
-    c.parts = min((c.total + min_units - 1) / min_units, (int)gridDim.x * (WARPS ? WARPS : 1));
+    c.parts = min(div_pos(c.total + min_units - 1, min_units), (int)gridDim.x * (WARPS ? WARPS : 1));
     if (c.worker < c.parts) {
       c.at = attn_line_at(c.worker, c.total, c.parts);
       c.end = attn_line_at(c.worker + 1, c.total, c.parts);
@@ -289,7 +315,7 @@ __device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units
         }
         o -= __shfl_sync(0xffffffffu, inc, 31);
       }
-      c.h = o / ub;
+      c.h = div_pos(o, ub);
       o -= c.h * ub;
       const AttnSeq s = attn_seq(a, c.b);
       const int nb = attn_blocks<R>(a, s);
@@ -460,11 +486,11 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int V = DP >= 128 ? DP / 128 : 1;  // float4 per lane
+  unsigned lead = __ballot_sync(0xffffffffu, lane < WPB && a.meta[blockIdx.x * WPB + min(lane, WPB - 1)].last_part >= 0);
 #pragma unroll 1
-  for (int k = 0; k < WPB; ++k) {
-    const int c0 = blockIdx.x * WPB + k;
+  for (; lead; lead &= lead - 1) {
+    const int c0 = blockIdx.x * WPB + __ffs(lead) - 1;
     const AttnMeta w = a.meta[c0];
-    if (w.last_part < 0) continue;
     const int np = w.last_part - c0 + 1;
     const bool many = np > 6;  // parts enough to share a row
 #pragma unroll 1
@@ -528,7 +554,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
       }
       if (!many || warp == 0) {
         AttnRow ar;
-        const int t = (w.row0 + r) / a.G;
+        const int t = div_pos(w.row0 + r, a.G);
         ar.token = w.tok0 + t;
         ar.head = w.h * a.G + w.row0 + r - t * a.G;
         const AttnFinish f = attn_finish(a, ar, m, l);

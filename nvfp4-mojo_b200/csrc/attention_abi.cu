@@ -27,18 +27,20 @@ static EncodeFn attn_encode() {
   return fn;
 }
 
-// (d, head, slot, page) of the keys or values, boxes of 64 columns by `rows`
-// slots of one head and page.
-static bool make_cache_map(CUtensorMap *m, void *base, const int64_t (&st)[3], const nvfp4_kv_cache &c,
-                           int rows) {
+// (column, slot, 64-column block, head, page) of the keys or values, boxes of 64
+// columns by `rows` slots of one head and page: all blocks of columns at once
+// (wide), or one, with the columns beyond the head reading as zeros.
+static bool make_cache_map(CUtensorMap *m, void *base, const int64_t (&st)[3], const nvfp4_kv_cache &c, int rows,
+                           bool wide) {
   EncodeFn fn = attn_encode();
   if (!fn) return false;
-  cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.num_kv_heads, (cuuint64_t)c.page_size,
-                        (cuuint64_t)c.num_pages};
-  cuuint64_t strides[3] = {(cuuint64_t)st[2] * 2, (cuuint64_t)st[1] * 2, (cuuint64_t)st[0] * 2};
-  cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1};
-  cuuint32_t es[4] = {1, 1, 1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, box, es,
+  const cuuint64_t blocks = wide ? c.head_dim / 64 : 1;
+  cuuint64_t dims[5] = {wide ? 64 : (cuuint64_t)c.head_dim, (cuuint64_t)c.page_size, blocks,
+                        (cuuint64_t)c.num_kv_heads, (cuuint64_t)c.num_pages};
+  cuuint64_t strides[4] = {(cuuint64_t)st[1] * 2, 128, (cuuint64_t)st[2] * 2, (cuuint64_t)st[0] * 2};
+  cuuint32_t box[5] = {64, (cuuint32_t)rows, (cuuint32_t)blocks, 1, 1};
+  cuuint32_t es[5] = {1, 1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, base, dims, strides, box, es,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -216,9 +218,12 @@ extern "C" int nvfp4_paged_attention(const nvfp4_attention_desc *desc, const nvf
     // A box of the cache map: a page, or as much of it as a key tile takes.
     const int tile = R <= 32 ? attn_rows_tile(desc->head_dim) : 64;
     const int box = cache->page_size < tile ? cache->page_size : tile;
+    // One copy for all columns where they fill the kernel's tile; the MMA's
+    // operands also need the tile's rows in one piece.
+    a.wide = desc->head_dim == L.dp && (R <= 32 || box == tile);
     CUtensorMap tk, tv;
-    if (!make_cache_map(&tk, cache->k, cache->k_strides, *cache, box) ||
-        !make_cache_map(&tv, cache->v, cache->v_strides, *cache, box))
+    if (!make_cache_map(&tk, cache->k, cache->k_strides, *cache, box, a.wide) ||
+        !make_cache_map(&tv, cache->v, cache->v_strides, *cache, box, a.wide))
       return fail(NVFP4_ERR_CUDA, "tensor map of the cache");
     return check_launch(R <= 32 ? launch_attn_rows(tk, tv, a, R, grid, st) : launch_attn_tc(tk, tv, a, grid, st),
                         what);

@@ -14,7 +14,7 @@ cudaError_t attn_allow_smem(const void *kernel, int bytes, std::atomic<uint64_t>
 // attention_rows.cu: items of R = 16 or 32 rows (16 above head size 128), and
 // the launch that joins what its workers (warps) cut.  Key tiles of
 // attn_rows_tile tokens.
-constexpr int kAttnRowsWorkers = 4;  // per block
+constexpr int kAttnRowsWorkers = 8;  // per block
 inline int attn_rows_tile(int head_dim) { return head_dim <= 128 ? 32 : 16; }
 cudaError_t launch_attn_rows(const CUtensorMap &tk, const CUtensorMap &tv, const AttnArgs &a, int R,
                              int grid, cudaStream_t st);

@@ -4,8 +4,8 @@
 // Bound by HBM: every key and value is read once for the R = 16 or 32 rows
 // that share it, in one launch whose warps divide all sequences' keys evenly
 // (attention.cuh), so a batch of ragged lengths keeps every SM streaming to
-// the end.  Each of a block's four warps works alone, without a barrier: it
-// keeps a ring of tiles of 32 tokens (16 above head size 128) in flight by TMA
+// the end.  Each of a block's eight warps works alone, without a barrier: it
+// keeps key and value tiles of 32 tokens (16 above head size 128) in flight by TMA
 // (a box per page, 128-byte swizzle), across the ends of its items, and turns
 // each into S = Q K^T, its softmax state and O += P V on mma.sync from registers
 // (16 rows would fill an eighth of a tcgen05 tile).  A cut item's parts go to
@@ -21,12 +21,12 @@
 namespace nvfp4 {
 
 static __device__ int g_attn_rows_status;
-static_assert(kAttnRowsWorkers == 4, "warps per block below");
+static_assert(kAttnRowsWorkers == 8, "warps per block below");
 
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kItemCost = 2;  // of an item's beginning and end, in tiles
+constexpr int kWarps = 8;
+constexpr int kItemCost = 1;  // of an item's beginning and end, in tiles
 constexpr int kSegs = 4;      // items that a warp's loads may be ahead
 
 template <int MT, int DP>
@@ -34,8 +34,8 @@ struct RowsCfg {
   static constexpr int R = 16 * MT;
   static constexpr int KT = DP <= 128 ? 32 : 16;  // tokens per tile
   static constexpr int kTile = KT * DP * 2;       // bytes of a tile's keys, or values
-  static constexpr int kRing = DP == 64 ? 6 : 3;  // tiles in flight per warp
-  static constexpr int bytes = kWarps * kRing * 2 * kTile + 1024;
+  static constexpr int kRing = DP == 64 ? 6 : 3;  // tiles (keys or values) per warp
+  static constexpr int bytes = kWarps * kRing * kTile + 1024;
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -62,15 +62,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int h, int row,
-                                            int page, uint32_t bar, uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      ".L2::cache_hint [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(h), "r"(row), "r"(page), "r"(bar), "l"(policy)
-      : "memory");
-}
-
 // MOD: scores are capped or biased.
 template <int MT, int DP, bool MOD>
 __global__ void __launch_bounds__(kWarps * 32, 1)
@@ -88,7 +79,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   __shared__ int aborts[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t full = smem_u32(bars + warp * kRing);
-  uint8_t *ring = smem + warp * kRing * 2 * C::kTile;
+  uint8_t *ring = smem + warp * kRing * C::kTile;
   const uint32_t rbase = smem_u32(ring);
 
   asm volatile("griddepcontrol.launch_dependents;");
@@ -111,17 +102,23 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   volatile int *abort = &aborts[warp];
   int *status = &g_attn_rows_status;
 
-  // Loads run up to kRing tiles ahead of the arithmetic.  The items lie in
+  // Loads run up to kRing tiles (keys and values in turn) ahead of the
+  // arithmetic.  The items lie in
   // shared memory; registers hold what every tile needs.
   int l_left = 0, l_j0 = 0, l_lo = 0, l_hi = 0, l_h = 0;  // the item being loaded
   const int *l_pages = nullptr;
+  bool l_v = false;                                       // its next copy is of values
   int ids = 0, ids_at = -64;
   int take = 0, j0 = 0, it_lo = 0, it_hi = 0;             // the item being computed: tiles left
   uint32_t issued = 0, done = 0, pushed = 0, popped = 0;
   bool more = true, have = false;
-  const int box = a.page_size < KT ? a.page_size : KT, per = KT / box;
-  // This lane's box of a tile: keys or values, rows i box .., columns 64 hf.
-  const int bi = lane % per, bh = (lane / per) % (DP / 64), bv = lane / (per * (DP / 64));
+  // A tile lies in shared memory box by box (a page's rows), a box as blocks
+  // of 64 columns; 16 rows never cross a box.
+  const int box = a.page_size < KT ? a.page_size : KT;
+  const int per = KT / box, blocks = a.wide ? 1 : DP / 64;  // boxes per tile, copies per box
+  const int bi = lane % per, bx = lane / per;               // this lane's copy
+  const uint32_t cstride = box * 128;                     // from 64 columns to the next
+  const uint32_t rstride = box == 16 ? 16 * DP * 2 : 16 * 128;  // from 16 rows to the next
   const uint64_t policy = l2_evict_first_policy();
 
   const int qr = lane >> 2, qc = lane & 3;
@@ -155,24 +152,27 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
         ids_at = -64;
         continue;
       }
-      const int tok = l_j0 + bi * box;
-      const bool mine = bv < 2 && tok < l_hi && tok + box > l_lo;
       const int p0 = l_j0 >> a.page_shift, p1 = (l_j0 + KT - 1) >> a.page_shift;
       if (p1 >= ids_at + 32) {  // the next 32 page ids, one per lane
         ids_at = p0;
         ids = l_pages[min(p0 + lane, (l_hi - 1) >> a.page_shift)];
       }
-      l_j0 += KT;
-      --l_left;
-      const int page = __shfl_sync(0xffffffffu, ids, ((tok >> a.page_shift) - ids_at) & 31);
-      const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * box * 128;
       const uint32_t st = issued % kRing;
+      const int tok = l_j0 + bi * box;
+      const bool mine = bx < blocks && tok < l_hi && tok + box > l_lo;  // holds a key that some row sees
+      const int page = __shfl_sync(0xffffffffu, ids, ((tok >> a.page_shift) - ids_at) & 31);
+      const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * box * (a.wide ? DP * 2 : 128);
       if (lane == 0) mbar_arrive_expect_tx(full + 8 * st, bytes);
       __syncwarp();
       if (mine)
-        tma_load_4d(rbase + (2 * st + bv) * C::kTile + bh * (KT * 128) + bi * box * 128, bv ? &tmV : &tmK,
-                    64 * bh, l_h, tok & (a.page_size - 1), page, full + 8 * st, policy);
+        attn_load_box(rbase + st * C::kTile + bi * box * DP * 2 + bx * cstride, l_v ? &tmV : &tmK, 64 * bx,
+                      tok & (a.page_size - 1), l_h, page, full + 8 * st, policy);
       ++issued;
+      if (l_v) {
+        l_j0 += KT;
+        --l_left;
+      }
+      l_v = !l_v;
     }
     // ---- the next item
     if (!have) {
@@ -217,8 +217,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       const uint32_t st = done % kRing;
       if (!__all_sync(0xffffffffu, attn_wait(full + 8 * st, (done / kRing) & 1, status, kDevTimeoutFull, abort)))
         break;
-      ++done;
-      const uint32_t kb0 = rbase + 2 * st * C::kTile, vb0 = kb0 + C::kTile;
+      const uint32_t sv = (done + 1) % kRing, kb0 = rbase + st * C::kTile, vb0 = rbase + sv * C::kTile;
       float s[MT][NT][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
@@ -234,7 +233,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
           for (int n = 0; n < NT; n += 2) {
             uint32_t b[4];
             const int c = (2 * k + cc) & 7;
-            ldsm4(kb0 + (k >> 2) * (KT * 128) + (t + 8 * n) * 128 + ((c ^ (t & 7)) << 4), b);
+            ldsm4(kb0 + (k >> 2) * cstride + (n >> 1) * rstride + t * 128 + ((c ^ (t & 7)) << 4), b);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
               mma_bf16(s[mt][n], qf[mt][k], b[0], b[1]);
@@ -289,14 +288,16 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
             p[mt][n >> 1][2 * (n & 1) + e] = pack_bf16(p0, p1);
           }
         }
+      if (!__all_sync(0xffffffffu, attn_wait(full + 8 * sv, ((done + 1) / kRing) & 1, status, kDevTimeoutFull, abort)))
+        break;
       if (j0 < it_lo || j0 + KT > it_hi) {
         // Tokens that no row sees (never loaded, or the rest of a page): their
         // zero weights must not meet what lies there.
         for (int x = lane; x < KT * (DP / 8); x += 32) {
           const int t = x / (DP / 8), c = x % (DP / 8);
           if (j0 + t < it_lo || j0 + t >= it_hi)
-            *reinterpret_cast<uint4 *>(ring + (2 * st + 1) * C::kTile + (c >> 3) * (KT * 128) + t * 128 +
-                                       (((c & 7) ^ (t & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4 *>(ring + sv * C::kTile + (c >> 3) * cstride + (t >> 4) * rstride +
+                                       (t & 15) * 128 + (((c & 7) ^ (t & 7)) << 4)) = make_uint4(0, 0, 0, 0);
         }
         __syncwarp();
       }
@@ -308,7 +309,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
           for (int n = 0; n < DP / 16; ++n) {
             uint32_t b[4];
             const int c = (2 * n + cc) & 7;
-            ldsm4t(vb0 + (n >> 2) * (KT * 128) + (t + 16 * k) * 128 + ((c ^ (t & 7)) << 4), b);
+            ldsm4t(vb0 + (n >> 2) * cstride + k * rstride + t * 128 + ((c ^ (t & 7)) << 4), b);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
               mma_bf16(o[mt][2 * n], p[mt][k], b[0], b[1]);
@@ -319,6 +320,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       // The tile's reads (and zeros) come before the copy that refills it.
       fence_proxy_async_smem();
       __syncwarp();
+      done += 2;
       j0 += KT;
       --take;
     }
@@ -415,7 +417,7 @@ cudaError_t launch_rows(const CUtensorMap &tk, const CUtensorMap &tv, const Attn
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if ((e = cudaLaunchKernelEx(&cfg, k, tk, tv, a)) != cudaSuccess) return e;
-  constexpr int RPB = 2;
+  constexpr int RPB = 1;
   cfg.gridDim = dim3((unsigned)grid, C::R / RPB, 1);
   cfg.blockDim = dim3(256, 1, 1);
   cfg.dynamicSmemBytes = 0;

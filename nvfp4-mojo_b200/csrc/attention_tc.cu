@@ -138,15 +138,6 @@ __device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lead) {
 }
 constexpr uint32_t kTransposeB = 1u << 16;
 
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int h, int row,
-                                            int page, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(h), "r"(row), "r"(page), "r"(bar)
-      : "memory");
-}
-
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t *>(&h);
@@ -280,7 +271,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       const int row = g.rb * R + my;
       const __nv_bfloat16 *src = nullptr;
       if (row < g.s.ql * a.G) {
-        const int i = row / a.G;
+        const int i = div_pos(row, a.G);
         src = a.q + (int64_t)(g.s.tok0 + i) * a.q_ts + (int64_t)(g.h * a.G + row - i * a.G) * a.q_hs;
       }
       constexpr int CH = DP / 8, RPI = 32 / CH;  // chunks per row, rows per warp step
@@ -617,26 +608,30 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       // ---------------- TMA producer ----------------
       const int box = a.page_size < KT ? a.page_size : KT;
       const int per = KT / box;
-      constexpr int halves = DP / 64;
+      // This lane's box of a tile and its columns (wide: all of them).
+      const int bi = lane % per, bx = lane / per;
+      const bool used = bx < (a.wide ? 1 : DP / 64);
+      const uint64_t policy = l2_evict_normal_policy();
       uint32_t at = 0;
       bool ok = true;
       while (ok && next_seg()) {
         const int *pages = a.page_table + (a.prefix_pass ? 0 : (int64_t)g.b * a.pt_stride);
+        const int take = __shfl_sync(0xffffffffu, g.take, 0), h = __shfl_sync(0xffffffffu, g.h, 0);
+        const int lo = __shfl_sync(0xffffffffu, g.it.lo, 0), hi = __shfl_sync(0xffffffffu, g.it.hi, 0);
+        int j0 = __shfl_sync(0xffffffffu, (g.it.u0 + g.off) * KT, 0);
         int ids = 0, ids_at = -64;
-        for (int u = 0; u < g.take && ok; ++u) {
-          const int j0 = (g.it.u0 + g.off + u) * KT;
-          const int i = lane % per, hf = lane / per;
-          const int tok = j0 + i * box;
-          const bool mine = hf < halves && tok < g.it.hi && tok + box > g.it.lo;
+        for (int u = 0; u < take && ok; ++u, j0 += KT) {
           const int p0 = j0 >> a.page_shift, p1 = (j0 + KT - 1) >> a.page_shift;
-          if (p1 >= ids_at + 32 || p0 < ids_at) {
+          if (p1 >= ids_at + 32) {  // the next 32 page ids, one per lane
             ids_at = p0;
-            ids = pages[min(p0 + lane, (g.it.hi - 1) >> a.page_shift)];
+            ids = pages[min(p0 + lane, (hi - 1) >> a.page_shift)];
           }
+          const bool ragged = j0 < lo || j0 + KT > hi;
+          const int tok = j0 + bi * box;
+          const bool mine = used && tok < hi && tok + box > lo;  // holds a key that some row sees
           const int page = __shfl_sync(0xffffffffu, ids, ((tok >> a.page_shift) - ids_at) & 31);
           const int row = tok & (a.page_size - 1);
-          const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * box * 128;
-          const bool ragged = j0 < g.it.lo || j0 + KT > g.it.hi;
+          const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * box * (a.wide ? DP * 2 : 128);
           for (int kv = 0; kv < 2; ++kv, ++at) {
             const uint32_t slot = at % kSlots, round = at / kSlots;
             if (round > 0 && !__all_sync(0xffffffffu, attn_wait(empty + 8 * slot, (round - 1) & 1, status,
@@ -648,8 +643,8 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
             if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
             __syncwarp();
             if (mine)
-              tma_load_4d(sbase + C::offKV + slot * C::kTile + hf * (KT * 128) + i * box * 128,
-                          kv ? &tmV : &tmK, 64 * hf, g.h, row, page, bar);
+              attn_load_box(sbase + C::offKV + slot * C::kTile + bx * (KT * 128) + bi * box * 128, kv ? &tmV : &tmK,
+                            64 * bx, row, h, page, bar, policy);
           }
         }
       }
