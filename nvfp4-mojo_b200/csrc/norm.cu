@@ -87,30 +87,28 @@ __device__ __forceinline__ void store8(const float (&v)[8], void *base, int dtyp
   }
 }
 
-// Sum over the nt threads of a row (nt a power of two >= 32); `red` holds one
-// float per warp of the block.  Every thread of the block calls it.
+// Sum over the nt threads of a row: a warp, or the whole block, whose warps
+// meet in `red`.
 __device__ __forceinline__ float row_sum(float s, int nt, float *red) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (nt > 32) {
-    const int warp = threadIdx.x >> 5, per = nt >> 5, first = warp & ~(per - 1);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[warp] = s;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
     __syncthreads();
     s = 0.0f;
-    for (int i = 0; i < per; ++i) s += red[first + i];
+    for (int i = 0; i < (nt >> 5); ++i) s += red[i];
   }
   return s;
 }
 
-// nt threads per row, blockDim.x / nt rows per block, VPT groups of 8 values
-// per thread.
-template <int VPT, bool VEC>
-__global__ void __launch_bounds__(1024) norm_residual_kernel(NormArgs a, int nt) {
-  __shared__ float red[32];
+// nt threads per row (32: eight rows per block, else a block per row), VPT
+// groups of 8 values per thread.
+template <int VPT, bool VEC, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 1280 / THREADS) norm_residual_kernel(NormArgs a, int nt) {
+  __shared__ float red[2][32];  // one per sum: the second needs no barrier before it
   const nvfp4_norm_desc &d = a.d;
-  const int H = d.hidden, t = threadIdx.x & (nt - 1);
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / nt) + threadIdx.x / nt;
+  const int H = d.hidden, t = nt == 32 ? threadIdx.x & 31 : threadIdx.x;
+  const int64_t row = nt == 32 ? (int64_t)blockIdx.x * 8 + threadIdx.x / 32 : blockIdx.x;
   const bool live = row < d.rows;
   const float inv_h = 1.0f / (float)H;
   asm volatile("griddepcontrol.launch_dependents;");
@@ -136,7 +134,7 @@ __global__ void __launch_bounds__(1024) norm_residual_kernel(NormArgs a, int nt)
     for (int v = 0; v < VPT; ++v)
 #pragma unroll
       for (int i = 0; i < 8; ++i) s = fmaf(u[v][i], u[v][i], s);
-    const float inv = rsqrtf(row_sum(s, nt, red) * inv_h + d.eps);
+    const float inv = rsqrtf(row_sum(s, nt, red[0]) * inv_h + d.eps);
 #pragma unroll
     for (int v = 0; v < VPT; ++v)
       if (in[v]) {
@@ -170,7 +168,7 @@ __global__ void __launch_bounds__(1024) norm_residual_kernel(NormArgs a, int nt)
       if (a.r_out) store8<VEC>(r[v], a.r_out, d.residual_dtype, row * d.residual_out_stride, col[v], nt, H);
     }
   if (a.pre) {
-    const float inv = rsqrtf(row_sum(s, nt, red) * inv_h + d.eps);
+    const float inv = rsqrtf(row_sum(s, nt, red[1]) * inv_h + d.eps);
 #pragma unroll
     for (int v = 0; v < VPT; ++v)
       if (in[v]) {
@@ -183,17 +181,11 @@ __global__ void __launch_bounds__(1024) norm_residual_kernel(NormArgs a, int nt)
   }
 }
 
-template <bool VEC>
-cudaError_t launch_norm(const NormArgs &a, cudaStream_t st) {
-  // A row's threads hold 8 values each, up to 32 in the longest rows; short
-  // rows share a block of 256 threads.
-  int nt = 32;
-  while (nt < 1024 && nt * 8 < a.d.hidden) nt *= 2;
-  const int vpt = (a.d.hidden + nt * 8 - 1) / (nt * 8);
-  const int rows_per_block = nt >= 256 ? 1 : 256 / nt;
-  const int64_t blocks = (a.d.rows + rows_per_block - 1) / rows_per_block;
+template <int VPT, bool VEC, int THREADS>
+cudaError_t launch_norm_as(const NormArgs &a, int nt, cudaStream_t st) {
+  const int rows_per_block = nt > 32 ? 1 : 8;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+  cfg.gridDim = dim3((unsigned)((a.d.rows + rows_per_block - 1) / rows_per_block), 1, 1);
   cfg.blockDim = dim3((unsigned)(nt * rows_per_block), 1, 1);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -201,9 +193,30 @@ cudaError_t launch_norm(const NormArgs &a, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (vpt <= 1) return cudaLaunchKernelEx(&cfg, norm_residual_kernel<1, VEC>, a, nt);
-  if (vpt <= 2) return cudaLaunchKernelEx(&cfg, norm_residual_kernel<2, VEC>, a, nt);
-  return cudaLaunchKernelEx(&cfg, norm_residual_kernel<4, VEC>, a, nt);
+  return cudaLaunchKernelEx(&cfg, norm_residual_kernel<VPT, VEC, THREADS>, a, nt);
+}
+
+template <int VPT, bool VEC>
+cudaError_t launch_norm_vpt(const NormArgs &a, int nt, cudaStream_t st) {
+  if constexpr (VPT == 4) return launch_norm_as<VPT, VEC, 1024>(a, nt, st);  // rows beyond 16384
+  if (nt <= 32) return launch_norm_as<VPT, VEC, 256>(a, nt, st);
+  if (nt <= 128) return launch_norm_as<VPT, VEC, 128>(a, nt, st);
+  if (nt <= 256) return launch_norm_as<VPT, VEC, 256>(a, nt, st);
+  if (nt <= 512) return launch_norm_as<VPT, VEC, 512>(a, nt, st);
+  return launch_norm_as<VPT, VEC, 1024>(a, nt, st);
+}
+
+template <bool VEC>
+cudaError_t launch_norm(const NormArgs &a, cudaStream_t st) {
+  // Few rows: 8 values a thread, for the shortest way through.  Rows enough to
+  // fill the GPU: 16, so that more bytes are in flight per thread and fewer
+  // threads meet at each sum (16384 rows of 2048, norms on both sides, fp32
+  // residual: 86 us with 8 values a thread, 76 with 16, 96 with 32).
+  const int H = a.d.hidden, per = H > 16384 ? 32 : H > 8192 || a.d.rows >= 592 ? 16 : 8;
+  const int nt = ((H + per - 1) / per + 31) / 32 * 32;
+  return per == 8 ? launch_norm_vpt<1, VEC>(a, nt, st)
+         : per == 16 ? launch_norm_vpt<2, VEC>(a, nt, st)
+                     : launch_norm_vpt<4, VEC>(a, nt, st);
 }
 
 bool norm_dt(int t) { return t == NVFP4_DTYPE_F32 || t == NVFP4_DTYPE_BF16; }
