@@ -6,8 +6,11 @@
 // norm by shuffles, turns its pairs and stores them.  A warp keeps its token's
 // sines and cosines in registers and walks over that token's heads, so the
 // angles (the only 64-bit arithmetic) are computed once per token and warp.
-// HBM-bound for many tokens, latency-bound for a few: then a token's heads are
-// spread over more warps.
+// Norm weight and rotation are one 2 x 2 matrix per pair, inv (x A - y B, y C +
+// x D), and the rows ahead are loaded before the present ones are turned: at
+// 220 instructions a row this kernel was bound by their issue, not by HBM.
+// Latency-bound for a few tokens: then a token's heads are spread over more
+// warps, and the first rows' loads run under the angles.
 #include <cuda_bf16.h>
 
 #include "../../include/nvfp4.h"
@@ -60,6 +63,7 @@ int check_attention_batch(const nvfp4_attention_batch *b, int page_size) {
 namespace {
 
 constexpr int kAppendWarps = 8;
+constexpr int kAhead = 4;  // rows a lane has in flight
 
 struct AppendArgs {
   nvfp4_kv_cache c;
@@ -71,51 +75,64 @@ struct AppendArgs {
   int64_t pos_stride;
   int num_axes, num_heads, page_shift;
   int chunks;       // warps per token
-  int chunk_rows;   // rows (heads of q, k, v in that order) per warp
+  int chunk_steps;  // steps (of rows) per warp
 };
 
 __device__ __forceinline__ float bf(uint32_t w, int hi) {
   return __uint_as_float(hi ? (w & 0xffff0000u) : (w << 16));
 }
 
-// Pairs p0 .. p0+3 of a row: first members at i0, second at i1 (VEC: both
-// runs of 4 consecutive elements; interleaved: one run of 8 at i0).
+// Four pairs as they lie in memory: runs of 4 consecutive elements from ei[0]
+// and ej[0] on (VEC; interleaved: one run of 8 from ei[0] on), or by element.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_pairs(const T *row, const int (&ei)[4], const int (&ej)[4],
-                                           bool inter, float (&a)[4], float (&b)[4]) {
-  if constexpr (VEC && sizeof(T) == 2) {
-    uint32_t w[4];
-    if (inter) {
-      const uint4 q = *reinterpret_cast<const uint4 *>(row + ei[0]);
-      w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+struct RawPairs {
+  static constexpr int N = sizeof(T) == 2 ? 4 : 8;
+  uint32_t w[N];
+  __device__ __forceinline__ void load(const T *row, const int (&ei)[4], const int (&ej)[4], bool inter, bool on) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = bf(w[i], 0), b[i] = bf(w[i], 1);
+    for (int i = 0; i < N; ++i) w[i] = 0u;
+    if (!on) return;
+    if constexpr (VEC && sizeof(T) == 2) {
+      if (inter) {
+        const uint4 q = *reinterpret_cast<const uint4 *>(row + ei[0]);
+        w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2 *>(row + ei[0]), y = *reinterpret_cast<const uint2 *>(row + ej[0]);
+        w[0] = x.x, w[1] = x.y, w[2] = y.x, w[3] = y.y;
+      }
+    } else if constexpr (VEC) {
+      const uint4 x = *reinterpret_cast<const uint4 *>(row + ei[0]);
+      const uint4 y = *reinterpret_cast<const uint4 *>(inter ? row + ei[0] + 4 : row + ej[0]);
+      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+      w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
     } else {
-      const uint2 x = *reinterpret_cast<const uint2 *>(row + ei[0]);
-      const uint2 y = *reinterpret_cast<const uint2 *>(row + ej[0]);
-      a[0] = bf(x.x, 0), a[1] = bf(x.x, 1), a[2] = bf(x.y, 0), a[3] = bf(x.y, 1);
-      b[0] = bf(y.x, 0), b[1] = bf(y.x, 1), b[2] = bf(y.y, 0), b[3] = bf(y.y, 1);
-    }
-  } else if constexpr (VEC) {
-    if (inter) {
-      const float4 x = *reinterpret_cast<const float4 *>(row + ei[0]);
-      const float4 y = *reinterpret_cast<const float4 *>(row + ei[0] + 4);
-      a[0] = x.x, b[0] = x.y, a[1] = x.z, b[1] = x.w;
-      a[2] = y.x, b[2] = y.y, a[3] = y.z, b[3] = y.w;
-    } else {
-      const float4 x = *reinterpret_cast<const float4 *>(row + ei[0]);
-      const float4 y = *reinterpret_cast<const float4 *>(row + ej[0]);
-      a[0] = x.x, a[1] = x.y, a[2] = x.z, a[3] = x.w;
-      b[0] = y.x, b[1] = y.y, b[2] = y.z, b[3] = y.w;
-    }
-  } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[i] = ei[i] < 0 ? 0.0f : (float)row[ei[i]];
-      b[i] = ej[i] < 0 ? 0.0f : (float)row[ej[i]];
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 2) {
+          const uint16_t *r = reinterpret_cast<const uint16_t *>(row);
+          w[i] = (ei[i] < 0 ? 0u : (uint32_t)r[ei[i]]) | (ej[i] < 0 ? 0u : (uint32_t)r[ej[i]]) << 16;
+        } else {
+          const uint32_t *r = reinterpret_cast<const uint32_t *>(row);
+          w[i] = ei[i] < 0 ? 0u : r[ei[i]];
+          w[4 + i] = ej[i] < 0 ? 0u : r[ej[i]];
+        }
+      }
     }
   }
-}
+  __device__ __forceinline__ void get(bool inter, float (&a)[4], float (&b)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        const bool side = inter || !VEC;  // a pair in one word
+        a[i] = side ? bf(w[i], 0) : bf(w[i >> 1], i & 1);
+        b[i] = side ? bf(w[i], 1) : bf(w[2 + (i >> 1)], i & 1);
+      } else {
+        a[i] = __uint_as_float(VEC && inter ? w[2 * i] : w[i]);
+        b[i] = __uint_as_float(VEC && inter ? w[2 * i + 1] : w[4 + i]);
+      }
+    }
+  }
+};
 
 template <bool VEC>
 __device__ __forceinline__ void store_pairs(__nv_bfloat16 *row, const int (&ei)[4], const int (&ej)[4],
@@ -146,7 +163,7 @@ __device__ __forceinline__ void store_pairs(__nv_bfloat16 *row, const int (&ei)[
 
 // LPR lanes per row (4 pairs each), 32 / LPR rows per warp step.
 template <typename T, int LPR, bool VEC>
-__global__ void __launch_bounds__(kAppendWarps * 32) kv_append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(kAppendWarps * 32, 3) kv_append_kernel(AppendArgs a) {
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int RPW = 32 / LPR;
@@ -188,81 +205,101 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kv_append_kernel(AppendArgs
   const bool inter = a.rot.interleaved;
   const bool active = l * 8 < D;
   int ei[4], ej[4];
-  float cs[4], sn[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int p = 4 * l + i;
     ei[i] = ej[i] = -1;
-    cs[i] = 1.0f, sn[i] = 0.0f;
     if (2 * p < D) {
       if (inter) ei[i] = 2 * p, ej[i] = 2 * p + 1;
       else if (p < half) ei[i] = p, ej[i] = p + half;
       else ei[i] = R + (p - half), ej[i] = R + (p - half) + (D - R) / 2;
-      if (p < half) {
-        int axis = a.rot.axis ? a.rot.axis[p] : 0;
-        axis = axis < 0 ? 0 : axis >= a.num_axes ? a.num_axes - 1 : axis;
-        const int64_t pos = a.pos ? a.pos[axis * a.pos_stride + t] : key + a.b.prefix_len;
-        // Whole turns are taken off in 64 bits: pos * inv_freq / (2 pi) keeps
-        // 2^-53 of up to 2^31 turns, far below fp32's step of the remainder.
-        const double turns = (double)pos * (double)a.rot.inv_freq[p] * 0.15915494309189533577;
-        sincospif(2.0f * (float)(turns - rint(turns)), &sn[i], &cs[i]);
-        cs[i] *= a.rot.scale;
-        sn[i] *= a.rot.scale;
-      }
     }
-  }
-  float wq[2][4], wk[2][4];  // norm weights of the pairs' members
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(a.norm.q_weight);
-    const __nv_bfloat16 *k = static_cast<const __nv_bfloat16 *>(a.norm.k_weight);
-    wq[0][i] = q && ei[i] >= 0 ? __bfloat162float(q[ei[i]]) + a.norm.weight_offset : 1.0f;
-    wq[1][i] = q && ej[i] >= 0 ? __bfloat162float(q[ej[i]]) + a.norm.weight_offset : 1.0f;
-    wk[0][i] = k && ei[i] >= 0 ? __bfloat162float(k[ei[i]]) + a.norm.weight_offset : 1.0f;
-    wk[1][i] = k && ej[i] >= 0 ? __bfloat162float(k[ej[i]]) + a.norm.weight_offset : 1.0f;
   }
 
-  const int HQ = a.num_heads, KV = a.c.num_kv_heads, rows = HQ + 2 * KV;
-  const int r0 = chunk * a.chunk_rows, r1 = min(rows, r0 + a.chunk_rows);
+  // The token's rows in steps of RPW: heads of q, then of k, then of v, each
+  // kind filled up to whole steps.
+  const int HQ = a.num_heads, KV = a.c.num_kv_heads;
+  const int sq = (HQ + RPW - 1) / RPW, sk = (KV + RPW - 1) / RPW;
+  const int s0 = chunk * a.chunk_steps, s1 = min(sq + 2 * sk, s0 + a.chunk_steps);
+  auto kind_of = [&](int st) { return st < sq ? 0 : st < sq + sk ? 1 : 2; };
+  auto head_of = [&](int st, int kind) { return (st - (kind == 0 ? 0 : kind == 1 ? sq : sq + sk)) * RPW + sub; };
+  RawPairs<T, VEC> raw[kAhead];
+  auto fetch = [&](RawPairs<T, VEC> &r, int st) {
+    const int kind = kind_of(st), h = head_of(st, kind);
+    const nvfp4_head_rows &in = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+    r.load(static_cast<const T *>(in.data) + t * in.token_stride + h * in.head_stride, ei, ej, inter,
+           st < s1 && active && h < (kind ? KV : HQ) && (kind == 0 || cached));
+  };
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) fetch(raw[i], s0 + i);
+
+  float cs[4], sn[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int p = 4 * l + i;
+    cs[i] = 1.0f, sn[i] = 0.0f;
+    if (p < half) {
+      int axis = a.rot.axis ? a.rot.axis[p] : 0;
+      axis = axis < 0 ? 0 : axis >= a.num_axes ? a.num_axes - 1 : axis;
+      const int64_t pos = a.pos ? a.pos[axis * a.pos_stride + t] : key + a.b.prefix_len;
+      // Whole turns are taken off in 64 bits: pos * inv_freq / (2 pi) keeps
+      // 2^-53 of up to 2^31 turns, far below fp32's step of the remainder.
+      const double turns = (double)pos * (double)a.rot.inv_freq[p] * 0.15915494309189533577;
+      sincospif(2.0f * (float)(turns - rint(turns)), &sn[i], &cs[i]);
+      cs[i] *= a.rot.scale;
+      sn[i] *= a.rot.scale;
+    }
+  }
+
   const float inv_d = 1.0f / (float)D;
-#pragma unroll 2
-  for (int rr = r0; rr < r1; rr += RPW) {
-    const int r = rr + sub;
-    const bool isq = r < HQ, isk = !isq && r < HQ + KV;
-    const int h = isq ? r : isk ? r - HQ : r - HQ - KV;
-    const bool on = r < r1 && active && (isq || cached);
-    float x[4] = {0, 0, 0, 0}, y[4] = {0, 0, 0, 0};
-    if (on) {
-      const nvfp4_head_rows &in = isq ? a.q : isk ? a.k : a.v;
-      load_pairs<T, VEC>(static_cast<const T *>(in.data) + t * in.token_stride + h * in.head_stride, ei,
-                         ej, inter, x, y);
+  float A[4], B[4], C[4], E[4];  // x' = x A - y B, y' = y C + x E
+  int have = -1;                 // the kind that they are for
+  bool normed = false;
+#pragma unroll 1
+  for (int sb = s0; sb < s1; sb += kAhead)
+#pragma unroll
+  for (int ring = 0; ring < kAhead; ++ring) {
+    const int st = sb + ring;
+    if (st >= s1) break;
+    const int kind = kind_of(st), h = head_of(st, kind);
+    if (kind != have) {
+      have = kind;
+      const __nv_bfloat16 *w = static_cast<const __nv_bfloat16 *>(kind == 0   ? a.norm.q_weight
+                                                                  : kind == 1 ? a.norm.k_weight
+                                                                              : nullptr);
+      normed = w != nullptr;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float wx = w && ei[i] >= 0 ? __bfloat162float(w[ei[i]]) + a.norm.weight_offset : 1.0f;
+        const float wy = w && ej[i] >= 0 ? __bfloat162float(w[ej[i]]) + a.norm.weight_offset : 1.0f;
+        const float c = kind == 2 ? 1.0f : cs[i], s = kind == 2 ? 0.0f : sn[i];
+        A[i] = wx * c, B[i] = wy * s, C[i] = wy * c, E[i] = wx * s;
+      }
     }
-    const bool normed = isq ? a.norm.q_weight != nullptr : isk && a.norm.k_weight != nullptr;
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s = fmaf(x[i], x[i], fmaf(y[i], y[i], s));
-#pragma unroll
-    for (int o = LPR / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    float x[4], y[4];
+    raw[ring].get(inter, x, y);
+    fetch(raw[ring], st + kAhead);
+    float inv = 1.0f;
     if (normed) {
-      const float inv = rsqrtf(s * inv_d + a.norm.eps);
+      float s = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] *= inv * (isq ? wq[0][i] : wk[0][i]);
-        y[i] *= inv * (isq ? wq[1][i] : wk[1][i]);
-      }
-    }
-    if (isq || isk) {
+      for (int i = 0; i < 4; ++i) s = fmaf(x[i], x[i], fmaf(y[i], y[i], s));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float u = x[i] * cs[i] - y[i] * sn[i], w = y[i] * cs[i] + x[i] * sn[i];
-        x[i] = u, y[i] = w;
-      }
+      for (int o = LPR / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      inv = rsqrtf(s * inv_d + a.norm.eps);
     }
-    if (on) {
+    if (active && h < (kind ? KV : HQ) && (kind == 0 || cached)) {
+      if (kind < 2) {  // values pass as they are, whatever they are
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float u = x[i] * A[i] - y[i] * B[i], w = y[i] * C[i] + x[i] * E[i];
+          x[i] = u * inv, y[i] = w * inv;
+        }
+      }
       __nv_bfloat16 *dst;
-      if (isq)
+      if (kind == 0)
         dst = static_cast<__nv_bfloat16 *>(a.qo.data) + t * a.qo.token_stride + h * a.qo.head_stride;
-      else if (isk)
+      else if (kind == 1)
         dst = static_cast<__nv_bfloat16 *>(a.c.k) + page * a.c.k_strides[0] + slot * a.c.k_strides[1] +
               h * a.c.k_strides[2];
       else
@@ -276,15 +313,14 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kv_append_kernel(AppendArgs
 template <typename T, int LPR>
 cudaError_t launch_append(AppendArgs &a, bool vec, cudaStream_t st) {
   constexpr int RPW = 32 / LPR;
-  const int rows = a.num_heads + 2 * a.c.num_kv_heads;
+  const int steps = (a.num_heads + RPW - 1) / RPW + 2 * ((a.c.num_kv_heads + RPW - 1) / RPW);
   // A warp takes a whole token where there are tokens enough for 16 warps on
   // every SM; fewer tokens are split over up to one warp per step of rows.
   const int64_t want = 148 * 16;
   int64_t chunks = a.b.num_tokens >= want ? 1 : (want + a.b.num_tokens - 1) / a.b.num_tokens;
-  const int steps = (rows + RPW - 1) / RPW;
   if (chunks > steps) chunks = steps;
-  a.chunk_rows = (int)((steps + chunks - 1) / chunks) * RPW;
-  a.chunks = (rows + a.chunk_rows - 1) / a.chunk_rows;
+  a.chunk_steps = (int)((steps + chunks - 1) / chunks);
+  a.chunks = (steps + a.chunk_steps - 1) / a.chunk_steps;
   const int64_t warps = a.b.num_tokens * a.chunks;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((warps + kAppendWarps - 1) / kAppendWarps), 1, 1);
