@@ -63,7 +63,6 @@ int check_attention_batch(const nvfp4_attention_batch *b, int page_size) {
 namespace {
 
 constexpr int kAppendWarps = 8;
-constexpr int kAhead = 4;  // rows a lane has in flight
 
 struct AppendArgs {
   nvfp4_kv_cache c;
@@ -83,26 +82,27 @@ __device__ __forceinline__ float bf(uint32_t w, int hi) {
 }
 
 // Four pairs as they lie in memory: runs of 4 consecutive elements from ei[0]
-// and ej[0] on (VEC; interleaved: one run of 8 from ei[0] on), or by element.
-template <typename T, bool VEC>
+// and ej[0] on (HALVES), one run of 8 from ei[0] on (INTERLEAVED), or by element.
+enum PairMode { kByElement = 0, kHalves = 1, kInterleaved = 2 };
+template <typename T, int MODE>
 struct RawPairs {
   static constexpr int N = sizeof(T) == 2 ? 4 : 8;
   uint32_t w[N];
-  __device__ __forceinline__ void load(const T *row, const int (&ei)[4], const int (&ej)[4], bool inter, bool on) {
+  __device__ __forceinline__ void load(const T *row, const int (&ei)[4], const int (&ej)[4], bool on) {
 #pragma unroll
     for (int i = 0; i < N; ++i) w[i] = 0u;
     if (!on) return;
-    if constexpr (VEC && sizeof(T) == 2) {
-      if (inter) {
+    if constexpr (MODE != kByElement && sizeof(T) == 2) {
+      if constexpr (MODE == kInterleaved) {
         const uint4 q = *reinterpret_cast<const uint4 *>(row + ei[0]);
         w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
       } else {
         const uint2 x = *reinterpret_cast<const uint2 *>(row + ei[0]), y = *reinterpret_cast<const uint2 *>(row + ej[0]);
         w[0] = x.x, w[1] = x.y, w[2] = y.x, w[3] = y.y;
       }
-    } else if constexpr (VEC) {
+    } else if constexpr (MODE != kByElement) {
       const uint4 x = *reinterpret_cast<const uint4 *>(row + ei[0]);
-      const uint4 y = *reinterpret_cast<const uint4 *>(inter ? row + ei[0] + 4 : row + ej[0]);
+      const uint4 y = *reinterpret_cast<const uint4 *>(MODE == kInterleaved ? row + ei[0] + 4 : row + ej[0]);
       w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
       w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
     } else {
@@ -119,25 +119,26 @@ struct RawPairs {
       }
     }
   }
-  __device__ __forceinline__ void get(bool inter, float (&a)[4], float (&b)[4]) const {
+  __device__ __forceinline__ void get(float (&a)[4], float (&b)[4]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (sizeof(T) == 2) {
-        const bool side = inter || !VEC;  // a pair in one word
+        constexpr bool side = MODE != kHalves;  // a pair in one word
         a[i] = side ? bf(w[i], 0) : bf(w[i >> 1], i & 1);
         b[i] = side ? bf(w[i], 1) : bf(w[2 + (i >> 1)], i & 1);
       } else {
-        a[i] = __uint_as_float(VEC && inter ? w[2 * i] : w[i]);
-        b[i] = __uint_as_float(VEC && inter ? w[2 * i + 1] : w[4 + i]);
+        a[i] = __uint_as_float(MODE == kInterleaved ? w[2 * i] : w[i]);
+        b[i] = __uint_as_float(MODE == kInterleaved ? w[2 * i + 1] : w[4 + i]);
       }
     }
   }
 };
 
-template <bool VEC>
+template <int MODE>
 __device__ __forceinline__ void store_pairs(__nv_bfloat16 *row, const int (&ei)[4], const int (&ej)[4],
-                                            bool inter, const float (&a)[4], const float (&b)[4]) {
-  if constexpr (VEC) {
+                                            const float (&a)[4], const float (&b)[4]) {
+  constexpr bool inter = MODE == kInterleaved;
+  if constexpr (MODE != kByElement) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -146,7 +147,7 @@ __device__ __forceinline__ void store_pairs(__nv_bfloat16 *row, const int (&ei)[
                                        : __floats2bfloat162_rn(b[2 * i - 4], b[2 * i - 3]);
       w[i] = *reinterpret_cast<const uint32_t *>(&h);
     }
-    if (inter) {
+    if constexpr (inter) {
       *reinterpret_cast<uint4 *>(row + ei[0]) = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
       *reinterpret_cast<uint2 *>(row + ei[0]) = make_uint2(w[0], w[1]);
@@ -162,11 +163,12 @@ __device__ __forceinline__ void store_pairs(__nv_bfloat16 *row, const int (&ei)[
 }
 
 // LPR lanes per row (4 pairs each), 32 / LPR rows per warp step.
-template <typename T, int LPR, bool VEC>
+template <typename T, int LPR, int MODE>
 __global__ void __launch_bounds__(kAppendWarps * 32, 3) kv_append_kernel(AppendArgs a) {
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int RPW = 32 / LPR;
+  constexpr int kAhead = sizeof(T) == 2 ? 4 : 2;  // rows a lane has in flight
   const int lane = threadIdx.x & 31, sub = lane / LPR, l = lane % LPR;
   const int64_t unit = (int64_t)blockIdx.x * kAppendWarps + (threadIdx.x >> 5);
   const int64_t t = unit / a.chunks;
@@ -202,7 +204,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 3) kv_append_kernel(AppendA
   // This lane's pairs: p < rotary_dim / 2 are turned; the rest of the head is
   // paired half against half and only normed.
   const int D = a.c.head_dim, R = a.rot.rotary_dim, half = R / 2;
-  const bool inter = a.rot.interleaved;
+  const bool inter = MODE == kInterleaved || (MODE == kByElement && a.rot.interleaved);
   const bool active = l * 8 < D;
   int ei[4], ej[4];
 #pragma unroll
@@ -217,21 +219,47 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 3) kv_append_kernel(AppendA
   }
 
   // The token's rows in steps of RPW: heads of q, then of k, then of v, each
-  // kind filled up to whole steps.
+  // kind filled up to whole steps.  Pointers run along; they are worked out
+  // anew only where the kind changes.
   const int HQ = a.num_heads, KV = a.c.num_kv_heads;
   const int sq = (HQ + RPW - 1) / RPW, sk = (KV + RPW - 1) / RPW;
   const int s0 = chunk * a.chunk_steps, s1 = min(sq + 2 * sk, s0 + a.chunk_steps);
-  auto kind_of = [&](int st) { return st < sq ? 0 : st < sq + sk ? 1 : 2; };
-  auto head_of = [&](int st, int kind) { return (st - (kind == 0 ? 0 : kind == 1 ? sq : sq + sk)) * RPW + sub; };
-  RawPairs<T, VEC> raw[kAhead];
-  auto fetch = [&](RawPairs<T, VEC> &r, int st) {
-    const int kind = kind_of(st), h = head_of(st, kind);
-    const nvfp4_head_rows &in = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-    r.load(static_cast<const T *>(in.data) + t * in.token_stride + h * in.head_stride, ei, ej, inter,
-           st < s1 && active && h < (kind ? KV : HQ) && (kind == 0 || cached));
+  struct Run {
+    int left, h, heads;  // steps of this kind left, this lane's head and their number
+    int kind;
+  };
+  auto run_at = [&](int st) {
+    Run r;
+    r.kind = st < sq ? 0 : st < sq + sk ? 1 : 2;
+    const int first = r.kind == 0 ? 0 : r.kind == 1 ? sq : sq + sk;
+    r.left = (r.kind == 0 ? sq : sk) - (st - first);
+    r.h = (st - first) * RPW + sub;
+    r.heads = r.kind == 2 || r.kind == 1 ? KV : HQ;
+    if (!active || (r.kind && !cached)) r.heads = 0;
+    return r;
+  };
+  RawPairs<T, MODE> raw[kAhead];
+  int fst = s0;  // the next step to fetch
+  Run fr;
+  fr.left = 0;
+  const T *src = nullptr;
+  int64_t sinc = 0;
+  auto fetch = [&](RawPairs<T, MODE> &r) {
+    if (fst >= s1) return;
+    if (fr.left == 0) {
+      fr = run_at(fst);
+      const nvfp4_head_rows &in = fr.kind == 0 ? a.q : fr.kind == 1 ? a.k : a.v;
+      src = static_cast<const T *>(in.data) + t * in.token_stride + fr.h * in.head_stride;
+      sinc = RPW * in.head_stride;
+    }
+    r.load(src, ei, ej, fr.h < fr.heads);
+    src += sinc;
+    fr.h += RPW;
+    --fr.left;
+    ++fst;
   };
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i) fetch(raw[i], s0 + i);
+  for (int i = 0; i < kAhead; ++i) fetch(raw[i]);
 
   float cs[4], sn[4];
 #pragma unroll
@@ -253,61 +281,67 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 3) kv_append_kernel(AppendA
 
   const float inv_d = 1.0f / (float)D;
   float A[4], B[4], C[4], E[4];  // x' = x A - y B, y' = y C + x E
-  int have = -1;                 // the kind that they are for
+  Run wr;
+  wr.left = 0;
+  wr.kind = 0;
   bool normed = false;
+  __nv_bfloat16 *dst = nullptr;
+  int64_t dinc = 0;
 #pragma unroll 1
   for (int sb = s0; sb < s1; sb += kAhead)
 #pragma unroll
-  for (int ring = 0; ring < kAhead; ++ring) {
-    const int st = sb + ring;
-    if (st >= s1) break;
-    const int kind = kind_of(st), h = head_of(st, kind);
-    if (kind != have) {
-      have = kind;
-      const __nv_bfloat16 *w = static_cast<const __nv_bfloat16 *>(kind == 0   ? a.norm.q_weight
-                                                                  : kind == 1 ? a.norm.k_weight
-                                                                              : nullptr);
-      normed = w != nullptr;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float wx = w && ei[i] >= 0 ? __bfloat162float(w[ei[i]]) + a.norm.weight_offset : 1.0f;
-        const float wy = w && ej[i] >= 0 ? __bfloat162float(w[ej[i]]) + a.norm.weight_offset : 1.0f;
-        const float c = kind == 2 ? 1.0f : cs[i], s = kind == 2 ? 0.0f : sn[i];
-        A[i] = wx * c, B[i] = wy * s, C[i] = wy * c, E[i] = wx * s;
-      }
-    }
-    float x[4], y[4];
-    raw[ring].get(inter, x, y);
-    fetch(raw[ring], st + kAhead);
-    float inv = 1.0f;
-    if (normed) {
-      float s = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s = fmaf(x[i], x[i], fmaf(y[i], y[i], s));
-#pragma unroll
-      for (int o = LPR / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      inv = rsqrtf(s * inv_d + a.norm.eps);
-    }
-    if (active && h < (kind ? KV : HQ) && (kind == 0 || cached)) {
-      if (kind < 2) {  // values pass as they are, whatever they are
+    for (int ring = 0; ring < kAhead; ++ring) {
+      const int st = sb + ring;
+      if (st >= s1) break;
+      if (wr.left == 0) {
+        wr = run_at(st);
+        const __nv_bfloat16 *w = static_cast<const __nv_bfloat16 *>(wr.kind == 0   ? a.norm.q_weight
+                                                                    : wr.kind == 1 ? a.norm.k_weight
+                                                                                   : nullptr);
+        normed = w != nullptr;
+        float wx[4], wy[4];
+        RawPairs<__nv_bfloat16, MODE> rw;
+        rw.load(w, ei, ej, normed && active);
+        rw.get(wx, wy);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float u = x[i] * A[i] - y[i] * B[i], w = y[i] * C[i] + x[i] * E[i];
-          x[i] = u * inv, y[i] = w * inv;
+          const float p = normed ? wx[i] + a.norm.weight_offset : 1.0f, q = normed ? wy[i] + a.norm.weight_offset : 1.0f;
+          A[i] = p * cs[i], B[i] = q * sn[i], C[i] = q * cs[i], E[i] = p * sn[i];
+        }
+        if (wr.kind == 0) {
+          dst = static_cast<__nv_bfloat16 *>(a.qo.data) + t * a.qo.token_stride + wr.h * a.qo.head_stride;
+          dinc = RPW * a.qo.head_stride;
+        } else {
+          const int64_t *cstr = wr.kind == 1 ? a.c.k_strides : a.c.v_strides;
+          dst = static_cast<__nv_bfloat16 *>(wr.kind == 1 ? a.c.k : a.c.v) + page * cstr[0] + slot * cstr[1] +
+                wr.h * cstr[2];
+          dinc = RPW * cstr[2];
         }
       }
-      __nv_bfloat16 *dst;
-      if (kind == 0)
-        dst = static_cast<__nv_bfloat16 *>(a.qo.data) + t * a.qo.token_stride + h * a.qo.head_stride;
-      else if (kind == 1)
-        dst = static_cast<__nv_bfloat16 *>(a.c.k) + page * a.c.k_strides[0] + slot * a.c.k_strides[1] +
-              h * a.c.k_strides[2];
-      else
-        dst = static_cast<__nv_bfloat16 *>(a.c.v) + page * a.c.v_strides[0] + slot * a.c.v_strides[1] +
-              h * a.c.v_strides[2];
-      store_pairs<VEC>(dst, ei, ej, inter, x, y);
+      float x[4], y[4];
+      raw[ring].get(x, y);
+      fetch(raw[ring]);
+      float inv = 1.0f;
+      if (normed) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s = fmaf(x[i], x[i], fmaf(y[i], y[i], s));
+#pragma unroll
+        for (int o = LPR / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        inv = rsqrtf(s * inv_d + a.norm.eps);
+      }
+      if (wr.kind < 2) {  // values pass as they are, whatever they are
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float u = x[i] * A[i] - y[i] * B[i], v = y[i] * C[i] + x[i] * E[i];
+          x[i] = u * inv, y[i] = v * inv;
+        }
+      }
+      if (wr.h < wr.heads) store_pairs<MODE>(dst, ei, ej, x, y);
+      dst += dinc;
+      wr.h += RPW;
+      --wr.left;
     }
-  }
 }
 
 template <typename T, int LPR>
@@ -331,8 +365,9 @@ cudaError_t launch_append(AppendArgs &a, bool vec, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return vec ? cudaLaunchKernelEx(&cfg, kv_append_kernel<T, LPR, true>, a)
-             : cudaLaunchKernelEx(&cfg, kv_append_kernel<T, LPR, false>, a);
+  return !vec                ? cudaLaunchKernelEx(&cfg, kv_append_kernel<T, LPR, kByElement>, a)
+         : a.rot.interleaved ? cudaLaunchKernelEx(&cfg, kv_append_kernel<T, LPR, kInterleaved>, a)
+                             : cudaLaunchKernelEx(&cfg, kv_append_kernel<T, LPR, kHalves>, a);
 }
 
 }  // namespace
@@ -388,6 +423,7 @@ extern "C" int nvfp4_kv_append(const nvfp4_kv_cache *cache, const nvfp4_attentio
     return aligned(r->data, 16) && (r->token_stride * es) % 16 == 0 && (r->head_stride * es) % 16 == 0;
   };
   const bool vec = fits(q, esize) && fits(k, esize) && fits(v, esize) && fits(q_out, 2) &&
+                   aligned(a.norm.q_weight, 16) && aligned(a.norm.k_weight, 16) &&
                    (a.rot.interleaved || (R % 8 == 0 && (D - R) % 8 == 0));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
