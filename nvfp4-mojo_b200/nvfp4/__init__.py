@@ -13,6 +13,7 @@ from .attention import (
     kv_append,
     paged_attention,
 )
+from .attention_layer import AttentionLayer, AttentionWeights
 from .config import (
     FP4_E2M1_LUT,
     NVFP4_GROUP_SIZE,
@@ -64,5 +65,6 @@ __all__ = [
     "Nvfp4Error", "LoadedWeight", "SafetensorsFile", "TensorInfo", "discover_safetensor_shards",
     "load_linear_safetensors", "load_moe_experts", "load_qwen35_layer", "open_model_shards",
     "open_safetensors", "AttentionBatch", "AttentionConfig", "PagedKVCache", "Rotary",
-    "attention_workspace", "kv_append", "paged_attention", "norm_residual",
+    "attention_workspace", "kv_append", "paged_attention", "norm_residual", "AttentionLayer",
+    "AttentionWeights",
 ]
