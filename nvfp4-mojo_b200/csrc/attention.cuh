@@ -244,14 +244,14 @@ __device__ __forceinline__ int attn_line_at(int c, int total, int parts) {
 struct AttnPlanSmem {
   int units[kPlanCache];  // per sequence and head
   int sum[32];
-  AttnCursor cur;
 };
 
 // Plans a worker's share; every thread of the block calls it.  Workers are the
-// blocks (WARPS 0: one result for all threads), or the first WARPS warps of
-// each.  parts: at most all workers and one per `min_units` units.
+// blocks (WARPS 0: the result is for warp `solo`, which lists the block's
+// items), or the first WARPS warps of each.  parts: at most all workers and one
+// per `min_units` units.
 template <int R, int KT, int E, int WARPS>
-__device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units, AttnPlanSmem *sm) {
+__device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units, AttnPlanSmem *sm, int solo) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
   const int NS = attn_num_seqs(a);
   // Units of the items start, start + step, ... of sequence b and one head.
@@ -263,17 +263,19 @@ __device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units
     for (int rb = start; rb < nb; rb += step) u += attn_item_units<R, KT, E>(a, s, rb);
     return u;
   };
-  // Sequences of few items: a thread each; of many: a warp each.  For up to
-  // 32 sequences of few items each warp that works alone plans alone.
+  // Sequences of few items: a thread each; of many: a warp each.  Of a few
+  // sequences the warps that want a plan make it without the others.
   const bool by_warp = a.max_blocks > 4;
-  const bool alone = WARPS && !by_warp && NS <= 32;
+  const bool alone = NS <= (by_warp ? 4 : 32);
+  if (alone && !WARPS && warp != solo) return AttnCursor{};
   int sum = 0;
 #pragma unroll 1
-  for (int b = alone ? lane : by_warp ? warp : tid; b < NS; b += alone ? 32 : by_warp ? nw : (int)blockDim.x) {
+  for (int b = by_warp ? (alone ? 0 : warp) : (alone ? lane : tid); b < NS;
+       b += by_warp ? (alone ? 1 : nw) : (alone ? 32 : (int)blockDim.x)) {
     int u = seq_units(b, by_warp ? lane : 0, by_warp ? 32 : 1);
     if (by_warp) u = __reduce_add_sync(0xffffffffu, u);
     if (!by_warp || lane == 0) {
-      if (!alone && b < kPlanCache) sm->units[b] = u;
+      if ((by_warp || !alone) && b < kPlanCache) sm->units[b] = u;  // (alone: each warp writes the same)
       sum += u;
     }
   }
@@ -285,7 +287,7 @@ __device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units
     sum = __reduce_add_sync(0xffffffffu, lane < nw ? sm->sum[lane] : 0);
   }
   AttnCursor c = {};
-  if (warp < (WARPS ? WARPS : 1)) {
+  if (WARPS ? warp < WARPS : warp == solo) {
     c.worker = WARPS ? blockIdx.x * WARPS + warp : blockIdx.x;
     c.total = a.Hkv * sum;
     c.parts = min(div_pos(c.total + min_units - 1, min_units), (int)gridDim.x * (WARPS ? WARPS : 1));
@@ -298,7 +300,7 @@ __device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units
 #pragma unroll 1
       for (int base = 0; base < NS; base += 32) {
         const int b = base + lane;
-        const int u = b >= NS ? 0 : !alone && b < kPlanCache ? sm->units[b] : seq_units(b, 0, 1);
+        const int u = b >= NS ? 0 : (by_warp || !alone) && b < kPlanCache ? sm->units[b] : seq_units(b, 0, 1);
         int inc = u * a.Hkv;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -338,11 +340,8 @@ __device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units
         o -= __shfl_sync(0xffffffffu, inc, 31);
       }
     }
-    if (!WARPS && lane == 0) sm->cur = c;
   }
-  if (WARPS) return c;
-  __syncthreads();
-  return sm->cur;
+  return c;
 }
 
 // One stretch of a worker's share: key units [off, off + take) of an item.
@@ -492,7 +491,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
     const int c0 = blockIdx.x * WPB + __ffs(lead) - 1;
     const AttnMeta w = a.meta[c0];
     const int np = w.last_part - c0 + 1;
-    const bool many = np > 6;  // parts enough to share a row
+    const bool many = RPB == 1 && np > 6;  // parts enough to share a row
 #pragma unroll 1
     for (int i = many ? 0 : warp; i < RPB; i += many ? 1 : 8) {
       const int r = blockIdx.y * RPB + i;

@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   {
-    const AttnCursor c = attn_plan<R, KT, kItemCost, kWarps>(a, 1 + kItemCost, &plan);
+    const AttnCursor c = attn_plan<R, KT, kItemCost, kWarps>(a, 1 + kItemCost, &plan, 0);
     if (lane == 0) {
       curs[warp] = c;
       a.meta[c.worker].last_part = -1;

@@ -163,6 +163,12 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // The largest of three.
 __device__ __forceinline__ float max3(float x, float y, float z) {
   float r;
@@ -230,9 +236,10 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
     tmem_relinquish();
   }
   tc_fence_before();
-  AttnCursor cur = attn_plan<R, KT, kItemCost, 0>(a, 2 + kItemCost, &plan);  // ends with __syncthreads
+  __syncthreads();
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;");
+  AttnCursor cur = attn_plan<R, KT, kItemCost, 0>(a, 2 + kItemCost, &plan, C::kSoftWarps + 2);
   const uint32_t tmem = tmem_slot;
   if (threadIdx.x == 0) a.meta[blockIdx.x].last_part = -1;
   volatile int *abort = &abort_flag;
@@ -316,6 +323,8 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
         const int lo_all = __reduce_max_sync(0xffffffffu, ar.lo), hi_all = __reduce_min_sync(0xffffffffu, ar.hi);
         const float slope = MOD && a.slopes ? a.slopes[ar.head] * kLog2e : 0.0f;
         const int pos = ar.pos - (a.prefix_pass ? 0 : a.prefix_len);
+        const float cap_in = MOD && a.softcap > 0.0f ? 2.0f * kLog2e / a.softcap * a.scale : 0.0f;
+        const float cap_out = -2.0f * kLog2e * a.softcap;
 #pragma unroll 1
         for (int u = 0; u < take; ++u, ++n) {
           const int j0 = j_first + u * KT;
@@ -334,16 +343,17 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
 #pragma unroll
           for (int c = 0; c < KT; ++c) s[c] = __uint_as_float(raw[c / 32][c % 32]);
           if constexpr (MOD) {
-            const float cap2 = 2.0f * kLog2e / a.softcap * a.scale;
-            const float dist = (float)(pos - j0);  // a conversion per element would be on the MUFU, too
+            if (a.softcap > 0.0f) {  // cap tanh(scale s / cap) = cap - 2 cap / (1 + e^(2 scale s / cap)), base 2
 #pragma unroll
-            for (int c = 0; c < KT; ++c) {
-              float v;
-              if (a.softcap > 0.0f)  // cap tanh(scale s / cap)
-                v = a.softcap - __fdividef(2.0f * a.softcap, 1.0f + ex2(s[c] * cap2));
-              else
-                v = s[c] * a.scale;
-              s[c] = fmaf(v, kLog2e, -slope * fabsf(dist - (float)c));
+              for (int c = 0; c < KT; ++c) s[c] = fmaf(rcp(1.0f + ex2(s[c] * cap_in)), cap_out, -0.5f * cap_out);
+            } else {
+#pragma unroll
+              for (int c = 0; c < KT; ++c) s[c] *= a.scale * kLog2e;
+            }
+            if (a.slopes) {
+              const float dist = (float)(pos - j0);  // a conversion per element would be on the MUFU, too
+#pragma unroll
+              for (int c = 0; c < KT; ++c) s[c] = fmaf(-slope, fabsf(dist - (float)c), s[c]);
             }
           }
           if (j0 < lo_all || j0 + KT > hi_all) {
@@ -728,7 +738,7 @@ cudaError_t launch_tc(const CUtensorMap &tk, const CUtensorMap &tv, const AttnAr
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if ((e = cudaLaunchKernelEx(&cfg, k, tk, tv, a)) != cudaSuccess) return e;
-  constexpr int RPB = 16;
+  constexpr int RPB = 8;
   cfg.gridDim = dim3((unsigned)grid, C::R / RPB, 1);
   cfg.blockDim = dim3(256, 1, 1);
   cfg.dynamicSmemBytes = 0;
