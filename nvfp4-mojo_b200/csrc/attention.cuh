@@ -474,26 +474,36 @@ __device__ __forceinline__ void attn_store4(const AttnArgs &a, const AttnRow &r,
 }
 
 // Joins the parts of the items that workers cut.  Block (x, y): the items led
-// by the workers WPB x .. WPB x + WPB - 1, rows RPB y .. RPB y + RPB - 1.  With
-// few parts a warp takes a row; with many all eight take every eighth part of
-// a row and join through shared memory.
+// by the workers WPB x .. WPB x + WPB - 1, rows RPB y .. RPB y + RPB - 1.  A warp
+// takes an item's row: of several rows (WPB 1), or of the item of the worker
+// that has its number (RPB 1).  There, items of seven parts and more come last:
+// all eight warps take every eighth part and join through shared memory.
 template <int R, int DP, int WPB, int RPB>
 __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnArgs a) {
+  static_assert((WPB == 1 || WPB == 8) && (RPB == 1 || WPB == 1), "a warp's rows");
   __shared__ float4 s_o[8][DP / 4];
   __shared__ float2 s_ml[8];
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int V = DP >= 128 ? DP / 128 : 1;  // float4 per lane
-  unsigned lead = __ballot_sync(0xffffffffu, lane < WPB && a.meta[blockIdx.x * WPB + min(lane, WPB - 1)].last_part >= 0);
+  const int last = a.meta[blockIdx.x * WPB + min(lane, WPB - 1)].last_part;
+  const bool leads = lane < WPB && last >= 0, wide = RPB == 1 && last - (int)(blockIdx.x * WPB + lane) >= 6;
+  const unsigned shared = __ballot_sync(0xffffffffu, leads && wide);
+  unsigned todo = __ballot_sync(0xffffffffu, leads && !wide && (WPB == 1 || lane == warp));
+  bool many = false;
 #pragma unroll 1
-  for (; lead; lead &= lead - 1) {
-    const int c0 = blockIdx.x * WPB + __ffs(lead) - 1;
+  for (;; todo &= todo - 1) {
+    if (!todo) {
+      if (many || !shared) break;
+      many = true;
+      todo = shared;
+    }
+    const int c0 = blockIdx.x * WPB + __ffs(todo) - 1;
     const AttnMeta w = a.meta[c0];
     const int np = w.last_part - c0 + 1;
-    const bool many = RPB == 1 && np > 6;  // parts enough to share a row
 #pragma unroll 1
-    for (int i = many ? 0 : warp; i < RPB; i += many ? 1 : 8) {
+    for (int i = RPB == 1 ? 0 : warp; i < RPB; i += 8) {
       const int r = blockIdx.y * RPB + i;
       if (r >= w.live) break;  // the same for all warps where they share rows
       float m = -INFINITY, l = 0.0f;
