@@ -4,24 +4,32 @@
 // An item is QT tiles of 128 query rows (attention.cuh: the heads of a group
 // share their keys, so 8 heads make a tile of 16 tokens); QT = 2, or 1 above
 // head size 128, where O takes half of TMEM.  Per tile of 64 keys and query
-// tile: S = Q K^T into one of two S buffers in TMEM, a softmax thread per row,
-// P as bf16 back over S, O += P V with P as the TMEM operand and V in its
-// natural token-major layout (MN-major operand).  The next S is issued before
-// the product that waits for P, so a softmax finds its next S ready and its
-// warps never stop; O stays in TMEM for all of an item.
-//   warps 0-3 (and 4-7, QT = 2)  softmax of tile 0 (1), Q into shared memory,
-//                                the rare rescaling of O, the epilogue;
-//   then one warp each           MMA issue for each query tile, TMA producer,
-//                                and the block's list of items with the
-//                                zeroing of values that no row sees.
+// tile: S = Q K^T into one of two S buffers in TMEM, two softmax threads per
+// row with 32 keys each, P as bf16 back over S, O += P V with P as the TMEM
+// operand and V in its natural token-major layout (MN-major operand).  The next
+// S is issued before the product that waits for P, so a softmax finds its next
+// S ready and its warps never stop; O stays in TMEM for all of an item.
+//   warps 0-7 (and 8-15, QT = 2)  softmax of tile 0 (1), Q into shared memory,
+//                                 the rare rescaling of O, the epilogue;
+//   then one warp each            MMA issue for each query tile, TMA producer,
+//                                 and the block's list of items with the
+//                                 zeroing of values that no row sees.
 // O is rescaled only when a row's maximum has grown by more than 2^8 since
 // the last time (weights then stay below 2^8, exact in the sums' fp32); the
 // reference is the same for sum and product, so the result is not changed.
-// Besides the tensor cores the exponentials bound it: 2 x 128 x 64 of them per
-// key tile take the MUFU 1024 cycles, as long as the products take the tensor
-// cores.  (A part of them on the FMA pipe, by a polynomial, measured slower:
-// 650 us with one in eight against 629 us, a prompt of 8192 at 32 / 4 heads of
-// 128: the issue slots are as scarce.)
+// A row's two threads meet once per tile, to learn whether either saw such a
+// growth.  (One thread per row: 297 against 278 us for four ragged prompts at
+// head size 256, where a tile's softmax is the one in flight; 572 against 570
+// for a prompt of 8192 at 32 / 4 heads of 128.)
+//
+// What bounds it: that prompt runs at 970 TFLOP/s and 990 W, where the power
+// limit takes the clock from 1965 to 1680 MHz.  Per pair of query tiles and key
+// tile it takes 1950 cycles: the exponentials 1024 of the MUFU, in a phase of
+// all warps that nothing else fills, and the products 1050 of the tensor cores.
+// Exponentials on the FMA pipe in part (a polynomial of degree 4) give 587 to
+// 620 us from 1/8 to 1/2 of them, the exponentials of the two query tiles taken
+// in turns 597: more instructions at the same power.  Head size 256 loads 64 KB
+// per tile of 128 rows and is bound by that, 6 TB/s from L2.
 #include <cuda_bf16.h>
 
 #include <type_traits>
@@ -43,6 +51,7 @@ constexpr int kItemCost = 5;  // of an item's beginning and end, in key tiles
 constexpr int kSegs = 4;      // items that the scheduling warp may be ahead
 
 constexpr int KT = 64;        // keys per tile
+constexpr int HK = KT / 2;    // of them a softmax thread's
 
 template <int DP>
 struct TcCfg {
@@ -51,7 +60,7 @@ struct TcCfg {
   static constexpr int kTile = KT * DP * 2;         // bytes of a key or value tile
   static constexpr int kQ = 128 * DP * 2;           // bytes of a query tile
   static constexpr int kSlots = DP == 64 ? 16 : DP == 128 ? 9 : 4;
-  static constexpr int kSoftWarps = 4 * QT;
+  static constexpr int kSoftWarps = 8 * QT;
   static constexpr int kThreads = (kSoftWarps + 4) * 32;
   static constexpr int offKV = QT * kQ;
   static constexpr int bytes = offKV + kSlots * kTile + 1024;
@@ -69,6 +78,14 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
       "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
       "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 // 16 lanes x 32 columns: lane l gets columns 8 k + 2 (l % 4) + {0, 1} of rows
@@ -188,6 +205,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
   __shared__ AttnPlanSmem plan;
   __shared__ uint64_t bars[3 * kSlots + 15 + 2 * kSegs];
   __shared__ AttnSegment segs[kSegs];
+  __shared__ float row_x[2][R];  // a row's value of each of its two threads
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   const uint32_t sbase = smem_u32(smem);
@@ -212,11 +230,11 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       mbar_init(empty + 8 * i, QT);  // a warp per query tile
       mbar_init(edge + 8 * i, 1);
     }
-    mbar_init(bar_q, 4);
-    mbar_init(bar_q + 8, 4);
+    mbar_init(bar_q, 8);
+    mbar_init(bar_q + 8, 8);
     for (int x = 0; x < 4; ++x) {
       mbar_init(bar_s + 8 * x, 1);
-      mbar_init(bar_p + 8 * x, 4);
+      mbar_init(bar_p + 8 * x, 8);
       mbar_init(bar_o + 8 * x, 1);
     }
     mbar_init(bar_end, QT);
@@ -262,8 +280,8 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
   auto tiles = [&](const AttnSegment &x) { return QT == 2 && x.s.ql * a.G - x.rb * R > 128 ? 2 : 1; };
 
   if (warp < C::kSoftWarps) {
-    if constexpr (QT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    const int t = warp >> 2, wq = warp & 3;            // tile, lane quarter
+    if constexpr (QT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    const int t = warp >> 3, half = warp >> 2 & 1, wq = warp & 3;  // tile, half of the keys, lane quarter
     const int my = t * 128 + wq * 32 + lane;           // row within the item
     const uint32_t lanes = static_cast<uint32_t>(32 * wq) << 16;
     const uint32_t tO = tmem + lanes + C::colO + t * DP;
@@ -271,7 +289,26 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
     const float c2 = MOD ? 1.0f : a.scale * kLog2e;
     const uint64_t c22 = pair(c2, c2);
 
-    // This warp's 32 rows of the next item's Q, 16-byte chunks swizzled as the
+    // The two warps of 32 rows.  Both always make the same calls: a warp whose
+    // wait ran out goes on with what there is until the next item.
+    const uint32_t bar_pair = 1 + 4 * t + wq;
+    auto pair_any = [&](bool x) -> bool {
+      uint32_t r;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+          "barrier.cta.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+          : "=r"(r)
+          : "r"((uint32_t)x), "r"(bar_pair)
+          : "memory");
+      return r != 0;
+    };
+    auto pair_other = [&](float x) -> float {  // the other thread's, of this row
+      row_x[half][my] = x;
+      asm volatile("barrier.cta.sync %0, 64;" ::"r"(bar_pair) : "memory");
+      return row_x[half ^ 1][my];
+    };
+
+    // This warp's 16 rows of the next item's Q, 16-byte chunks swizzled as the
     // MMA reads them; rows and columns beyond the item's or the head's are
     // zeros.  Started here, handed over in q_done().
     auto q_start = [&]() {
@@ -284,8 +321,8 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       constexpr int CH = DP / 8, RPI = 32 / CH;  // chunks per row, rows per warp step
       const int c = lane % CH;
 #pragma unroll 4
-      for (int r0 = 0; r0 < 32; r0 += RPI) {
-        const int r = r0 + lane / CH;
+      for (int r0 = 0; r0 < 16; r0 += RPI) {
+        const int r = 16 * half + r0 + lane / CH;
         const uint64_t p = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(src), r);
         const int rr = wq * 32 + r;
         const bool on = p != 0 && 8 * c < a.D;
@@ -303,13 +340,13 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
     };
 
     uint32_t n = 0;  // key tiles of this query tile so far
-    bool have = next_seg(), ok = true;
+    bool ok = true, have = !pair_any(!next_seg());
     bool fetch = have && g.take > 0 && t < tiles(g);
     if (fetch) {
       q_start();
       q_done();
     }
-    while (have && ok) {
+    while (have) {
       const bool mine = t < tiles(g);
       const int take = g.take, slot = g.slot, j_first = (g.it.u0 + g.off) * KT;
       const int row = g.rb * R + my;
@@ -327,63 +364,59 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
         const float cap_out = -2.0f * kLog2e * a.softcap;
 #pragma unroll 1
         for (int u = 0; u < take; ++u, ++n) {
-          const int j0 = j_first + u * KT;
+          const int j0 = j_first + u * KT + half * HK;
           const uint32_t x = 2 * t + (n & 1);
           const uint32_t tS = tmem + lanes + x * KT;
-          if (!__all_sync(0xffffffffu, attn_wait(bar_s + 8 * x, (n >> 1) & 1, status, kDevTimeoutAcc, abort))) {
-            ok = false;
-            break;
-          }
+          ok = attn_wait(bar_s + 8 * x, (n >> 1) & 1, status, kDevTimeoutAcc, abort) && ok;
+          __syncwarp();
           tc_fence_after();
-          uint32_t raw[2][32];
-          tmem_ld_32x32b_x32(tS, raw[0]);
-          tmem_ld_32x32b_x32(tS + 32, raw[1]);
+          uint32_t raw[HK];
+          tmem_ld_32x32b_x32(tS + half * HK, raw);
           tmem_ld_wait();
-          float s[KT];
+          float s[HK];
 #pragma unroll
-          for (int c = 0; c < KT; ++c) s[c] = __uint_as_float(raw[c / 32][c % 32]);
+          for (int c = 0; c < HK; ++c) s[c] = __uint_as_float(raw[c]);
           if constexpr (MOD) {
             if (a.softcap > 0.0f) {  // cap tanh(scale s / cap) = cap - 2 cap / (1 + e^(2 scale s / cap)), base 2
 #pragma unroll
-              for (int c = 0; c < KT; ++c) s[c] = fmaf(rcp(1.0f + ex2(s[c] * cap_in)), cap_out, -0.5f * cap_out);
+              for (int c = 0; c < HK; ++c) s[c] = fmaf(rcp(1.0f + ex2(s[c] * cap_in)), cap_out, -0.5f * cap_out);
             } else {
 #pragma unroll
-              for (int c = 0; c < KT; ++c) s[c] *= a.scale * kLog2e;
+              for (int c = 0; c < HK; ++c) s[c] *= a.scale * kLog2e;
             }
             if (a.slopes) {
               const float dist = (float)(pos - j0);  // a conversion per element would be on the MUFU, too
 #pragma unroll
-              for (int c = 0; c < KT; ++c) s[c] = fmaf(-slope, fabsf(dist - (float)c), s[c]);
+              for (int c = 0; c < HK; ++c) s[c] = fmaf(-slope, fabsf(dist - (float)c), s[c]);
             }
           }
-          if (j0 < lo_all || j0 + KT > hi_all) {
+          if (j0 < lo_all || j0 + HK > hi_all) {
             const int lo = ar.lo - j0, hi = ar.hi - j0;
 #pragma unroll
-            for (int c = 0; c < KT; ++c) s[c] = c >= lo && c < hi ? s[c] : -INFINITY;
+            for (int c = 0; c < HK; ++c) s[c] = c >= lo && c < hi ? s[c] : -INFINITY;
           }
           float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-          for (int c = 4; c < KT - 4; c += 8)
+          for (int c = 4; c < HK - 4; c += 8)
 #pragma unroll
             for (int i = 0; i < 4; ++i) top[i] = max3(top[i], s[c + i], s[c + 4 + i]);
-          top[0] = max3(top[0], s[KT - 4], s[KT - 3]);
-          top[1] = max3(top[1], s[KT - 2], s[KT - 1]);
-          const float mx = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * c2;
-          const bool grow = mx > m + 8.0f;
-          if (__any_sync(0xffffffffu, grow)) {
+          top[0] = max3(top[0], s[HK - 4], s[HK - 3]);
+          top[1] = max3(top[1], s[HK - 2], s[HK - 1]);
+          float mx = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * c2;
+          // (Behind this barrier both threads have read their S, and P may go over it.)
+          if (pair_any(mx > m + 8.0f)) {
+            mx = fmaxf(mx, pair_other(mx));
+            const bool grow = mx > m + 8.0f;
             const float mn = grow ? mx : m;
             if (u > 0) {  // O of the tiles before, once they are all in
               const uint32_t y = 2 * t + ((n - 1) & 1);
-              if (!__all_sync(0xffffffffu, attn_wait(bar_o + 8 * y, ((n - 1) >> 1) & 1, status, kDevTimeoutAcc,
-                                                     abort))) {
-                ok = false;
-                break;
-              }
+              ok = attn_wait(bar_o + 8 * y, ((n - 1) >> 1) & 1, status, kDevTimeoutAcc, abort) && ok;
+              __syncwarp();
               tc_fence_after();
               const float f = grow ? ex2(m - mn) : 1.0f;
               l *= f;
 #pragma unroll 1
-              for (int c = 0; c < DP; c += 32) {
+              for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
                 uint32_t o[32];
                 tmem_ld_32x32b_x32(tO + c, o);
                 tmem_ld_wait();
@@ -397,9 +430,9 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
           const float mu = m == -INFINITY ? 0.0f : m;
           const uint64_t nm2 = pair(-mu, -mu);
           uint64_t sum[2] = {0, 0};
-          uint32_t p[32];
+          uint32_t p[HK / 2];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
+          for (int i = 0; i < HK / 2; ++i) {
             const uint64_t e2 = fma2(pair(s[2 * i], s[2 * i + 1]), c22, nm2);
             float e0, e1;
             unpair(e2, e0, e1);
@@ -410,7 +443,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
             // unrounded weights.
             p[i] = pack_bf16(e0, e1);
           }
-          tmem_st_x32(tS, p);
+          tmem_st_x16(tS + half * (HK / 2), p);
           float l0, l1;
           unpair(add2(sum[0], sum[1]), l0, l1);
           l += l0 + l1;
@@ -419,20 +452,20 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_p + 8 * x);
         }
-        if (!ok) break;
         // Every S of the item is done: its Q may go.
-        have = next_seg();
+        have = !pair_any(!(next_seg() && ok));
         fetch = have && g.take > 0 && t < tiles(g);
         if (fetch) {
           q_start();
           q_done();
         }
         const uint32_t y = 2 * t + ((n - 1) & 1);
-        if (!__all_sync(0xffffffffu, attn_wait(bar_o + 8 * y, ((n - 1) >> 1) & 1, status, kDevTimeoutAcc, abort)))
-          break;
+        ok = attn_wait(bar_o + 8 * y, ((n - 1) >> 1) & 1, status, kDevTimeoutAcc, abort) && ok;
+        __syncwarp();
         tc_fence_after();
+        l += pair_other(l);
       } else {
-        have = next_seg();
+        have = !pair_any(!(next_seg() && ok));
         fetch = have && g.take > 0 && t < tiles(g);
         if (fetch) {
           q_start();
@@ -449,9 +482,9 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       if (in) {
         if (slot < 0) {
           f = attn_finish(a, ar, m, l);
-          attn_store_lse(a, f);
+          if (half == 0) attn_store_lse(a, f);
         } else {
-          a.part_ml[(int64_t)slot * R + my] = make_float2(m, l);
+          if (half == 0) a.part_ml[(int64_t)slot * R + my] = make_float2(m, l);
           f.so = 1.0f;
         }
       }
@@ -485,12 +518,11 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
               gate[i] = reinterpret_cast<const char *>(a.gate + tok * a.g_ts + head * a.g_hs + 2 * (lane & 3));
             }
           }
-          // 32 columns a step; with a gate or a prefix part 64, whose loads are
-          // in flight together.
-          constexpr int W = MODE == 2 ? 64 : 32;
-          const int cols = MODE == 0 ? DP : a.D;
+          // This warp's half of the columns, 32 a step.
+          constexpr int W = 32;
+          const int cols = min(MODE == 0 ? DP : a.D, (half + 1) * (DP / 2));
 #pragma unroll 1
-          for (int c0 = 0; c0 < cols; c0 += W) {
+          for (int c0 = half * (DP / 2); c0 < cols; c0 += W) {
             // Per row i: columns c0 + 8 k + 2 (lane % 4) + {0, 1}.
             uint32_t o[W / 32][16] = {}, w[2][W / 8] = {};
             float2 p[2][W / 8] = {};
@@ -539,7 +571,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       tc_fence_before();
     }
   } else {
-    if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     const int role = warp - C::kSoftWarps;
     if (role == 0 || (role == 3 && QT == 2)) {
       // ---------------- MMA issue, a warp per query tile ----------------
