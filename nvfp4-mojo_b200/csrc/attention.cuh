@@ -41,7 +41,8 @@ struct AttnArgs {
   int prefix_len;
   int prefix_pass;  // 1: all tokens against the shared prefix; 0: own keys
   int causal, window;
-  int max_blocks;   // bound on items per sequence and head (max_q_len)
+  int max_rows;     // of a sequence and key/value head, by max_q_len: sizes the
+  int max_blocks;   // grid of the join; and their items: who plans
   int wide;         // a copy brings all columns of its rows, not 64 of them
   float scale, softcap;
   const float *slopes;
@@ -473,108 +474,118 @@ __device__ __forceinline__ void attn_store4(const AttnArgs &a, const AttnRow &r,
       make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
 }
 
-// Joins the parts of the items that workers cut.  Block (x, y): the items led
-// by the workers WPB x .. WPB x + WPB - 1, rows RPB y .. RPB y + RPB - 1.  A warp
-// takes an item's row: of several rows (WPB 1), or of the item of the worker
-// that has its number (RPB 1).  There, items of seven parts and more come last:
-// all eight warps take every eighth part and join through shared memory.
+// N columns' weighted sum of a row's parts, with their maximum and sum.
+template <int V>
+struct AttnParts {
+  float m = -INFINITY, l = 0.0f;
+  float4 acc[V] = {};
+  __device__ __forceinline__ void add(float2 ml, const float4 (&x)[V]) {
+    const float top = fmaxf(m, ml.x), mu = top == -INFINITY ? 0.0f : top;
+    const float f = ex2(m - mu), g = ex2(ml.x - mu);
+    m = top;
+    l = l * f + ml.y * g;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      acc[v].x = acc[v].x * f + x[v].x * g;
+      acc[v].y = acc[v].y * f + x[v].y * g;
+      acc[v].z = acc[v].z * f + x[v].z * g;
+      acc[v].w = acc[v].w * f + x[v].w * g;
+    }
+  }
+  // Parts p, p + step, ... below np of row r of the item that worker c0 leads,
+  // columns col + 128 v: IN of them in flight.
+  template <int R, int DP, int IN>
+  __device__ __forceinline__ void read(const AttnArgs &a, int c0, int r, int p, int step, int np, int col) {
+#pragma unroll 1
+    for (; p < np; p += IN * step) {
+      float2 ml[IN];
+      float4 x[IN][V];
+#pragma unroll
+      for (int q = 0; q < IN; ++q) {
+        const int pp = min(p + q * step, np - 1);  // (a load that is not used, rather than a branch)
+        const int64_t at = (int64_t)(pp == 0 ? 2 * c0 + 1 : 2 * (c0 + pp)) * R + r;
+        ml[q] = a.part_ml[at];
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          x[q][v] = *reinterpret_cast<const float4 *>(a.part_o + at * DP + min(col, DP - 4) + 128 * v);
+      }
+#pragma unroll
+      for (int q = 0; q < IN; ++q)
+        if (p + q * step < np) add(ml[q], x[q]);
+    }
+  }
+};
+
+__device__ __forceinline__ AttnRow attn_meta_row(const AttnArgs &a, const AttnMeta &w, int r) {
+  AttnRow ar;
+  const int t = div_pos(w.row0 + r, a.G);
+  ar.token = w.tok0 + t;
+  ar.head = w.h * a.G + w.row0 + r - t * a.G;
+  return ar;
+}
+
+// Joins the parts of the items that workers cut.  A warp takes a row: with
+// several rows per block (RPB, WPB 1) block (x, y) those from RPB y on of the
+// item that worker x leads, else block (x, y) row y of the items that the
+// workers 8 x .. 8 x + 7 lead, an item per warp.  There, items of seven parts and
+// more come last: all eight warps take every eighth part, each block z 128
+// columns, and join through shared memory.
 template <int R, int DP, int WPB, int RPB>
 __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnArgs a) {
-  static_assert((WPB == 1 || WPB == 8) && (RPB == 1 || WPB == 1), "a warp's rows");
-  __shared__ float4 s_o[8][DP / 4];
-  __shared__ float2 s_ml[8];
+  static_assert((WPB == 1) != (RPB == 1) && (WPB == 1 || WPB == 8), "a warp's rows");
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int V = DP >= 128 ? DP / 128 : 1;  // float4 per lane
   const int last = a.meta[blockIdx.x * WPB + min(lane, WPB - 1)].last_part;
   const bool leads = lane < WPB && last >= 0, wide = RPB == 1 && last - (int)(blockIdx.x * WPB + lane) >= 6;
-  const unsigned shared = __ballot_sync(0xffffffffu, leads && wide);
-  unsigned todo = __ballot_sync(0xffffffffu, leads && !wide && (WPB == 1 || lane == warp));
-  bool many = false;
-#pragma unroll 1
-  for (;; todo &= todo - 1) {
-    if (!todo) {
-      if (many || !shared) break;
-      many = true;
-      todo = shared;
-    }
-    const int c0 = blockIdx.x * WPB + __ffs(todo) - 1;
+  if (blockIdx.z == 0 && __ballot_sync(0xffffffffu, leads && !wide && (WPB == 1 || lane == warp))) {
+    const int c0 = blockIdx.x * WPB + (WPB == 1 ? 0 : warp);
     const AttnMeta w = a.meta[c0];
-    const int np = w.last_part - c0 + 1;
+    const int r0 = RPB * blockIdx.y + (WPB == 1 ? warp : 0), r1 = RPB == 1 ? w.live : min(w.live, RPB * (int)blockIdx.y + RPB);
 #pragma unroll 1
-    for (int i = RPB == 1 ? 0 : warp; i < RPB; i += 8) {
-      const int r = blockIdx.y * RPB + i;
-      if (r >= w.live) break;  // the same for all warps where they share rows
-      float m = -INFINITY, l = 0.0f;
-      float4 acc[V];
+    for (int r = r0; r < r1; r += RPB == 1 ? gridDim.y : 8) {
+      AttnParts<V> t;
+      t.template read<R, DP, 4>(a, c0, r, 0, 1, w.last_part - c0 + 1, 4 * lane);
+      const AttnRow ar = attn_meta_row(a, w, r);
+      const AttnFinish f = attn_finish(a, ar, t.m, t.l);
 #pragma unroll
-      for (int v = 0; v < V; ++v) acc[v] = make_float4(0, 0, 0, 0);
-      auto add = [&](const float2 ml, const float4 (&x)[V]) {
-        const float top = fmaxf(m, ml.x), mu = top == -INFINITY ? 0.0f : top;
-        const float f = ex2(m - mu), g = ex2(ml.x - mu);
-        m = top;
-        l = l * f + ml.y * g;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          acc[v].x = acc[v].x * f + x[v].x * g;
-          acc[v].y = acc[v].y * f + x[v].y * g;
-          acc[v].z = acc[v].z * f + x[v].z * g;
-          acc[v].w = acc[v].w * f + x[v].w * g;
-        }
-      };
-      // Four parts' loads in flight.
-#pragma unroll 1
-      for (int p = many ? warp : 0; p < np; p += many ? 32 : 4) {
-        float2 ml[4];
-        float4 x[4][V];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int pp = p + (many ? 8 * q : q);
-          ml[q] = make_float2(-INFINITY, 0.0f);
-          const int64_t at = ((int64_t)(pp == 0 ? 2 * c0 + 1 : 2 * (c0 + pp))) * R + r;
-          if (pp < np) ml[q] = a.part_ml[at];
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            x[q][v] = make_float4(0, 0, 0, 0);
-            if (pp < np && 4 * lane + 128 * v < DP)
-              x[q][v] = *reinterpret_cast<const float4 *>(a.part_o + at * DP + 4 * lane + 128 * v);
-          }
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) add(ml[q], x[q]);
+      for (int v = 0; v < V; ++v) {
+        float x[4] = {t.acc[v].x, t.acc[v].y, t.acc[v].z, t.acc[v].w};
+        attn_store4(a, ar, f, 4 * lane + 128 * v, DP, x);
       }
-      if (many) {
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          if (4 * lane + 128 * v < DP) s_o[warp][lane + 32 * v] = acc[v];
-        if (lane == 0) s_ml[warp] = make_float2(m, l);
+      if (lane == 0) attn_store_lse(a, f);
+    }
+  }
+  if constexpr (RPB == 1) {
+    __shared__ float4 s_o[8][32];
+    __shared__ float2 s_ml[8];
+    const int col = 128 * blockIdx.z + 4 * lane;
+#pragma unroll 1
+    for (unsigned todo = __ballot_sync(0xffffffffu, leads && wide); todo; todo &= todo - 1) {
+      const int c0 = blockIdx.x * WPB + __ffs(todo) - 1;
+      const AttnMeta w = a.meta[c0];
+#pragma unroll 1
+      for (int r = blockIdx.y; r < w.live; r += gridDim.y) {
+        AttnParts<1> t;
+        t.template read<R, DP, 8>(a, c0, r, warp, 8, w.last_part - c0 + 1, col);
+        s_o[warp][lane] = t.acc[0];
+        if (lane == 0) s_ml[warp] = make_float2(t.m, t.l);
         __syncthreads();
         if (warp == 0) {
-#pragma unroll 1
+#pragma unroll
           for (int q = 1; q < 8; ++q) {
-            float4 x[V];
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-              x[v] = 4 * lane + 128 * v < DP ? s_o[q][lane + 32 * v] : make_float4(0, 0, 0, 0);
-            add(s_ml[q], x);
+            const float4 y[1] = {s_o[q][lane]};
+            t.add(s_ml[q], y);
           }
+          const AttnRow ar = attn_meta_row(a, w, r);
+          const AttnFinish f = attn_finish(a, ar, t.m, t.l);
+          float v[4] = {t.acc[0].x, t.acc[0].y, t.acc[0].z, t.acc[0].w};
+          if (col < DP) attn_store4(a, ar, f, col, DP, v);
+          if (col == 0) attn_store_lse(a, f);
         }
+        __syncthreads();
       }
-      if (!many || warp == 0) {
-        AttnRow ar;
-        const int t = div_pos(w.row0 + r, a.G);
-        ar.token = w.tok0 + t;
-        ar.head = w.h * a.G + w.row0 + r - t * a.G;
-        const AttnFinish f = attn_finish(a, ar, m, l);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          float x[4] = {acc[v].x, acc[v].y, acc[v].z, acc[v].w};
-          attn_store4(a, ar, f, 4 * lane + 128 * v, DP, x);
-        }
-        if (lane == 0) attn_store_lse(a, f);
-      }
-      if (many) __syncthreads();
     }
   }
 }

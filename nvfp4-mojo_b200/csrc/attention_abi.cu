@@ -214,7 +214,9 @@ extern "C" int nvfp4_paged_attention(const nvfp4_attention_desc *desc, const nvf
   a.part_ml = reinterpret_cast<float2 *>(w + L.part_ml);
   a.meta = reinterpret_cast<AttnMeta *>(w + L.meta);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto pass = [&](int R, const char *what) -> int {
+  auto pass = [&](int R, int64_t rows, const char *what) -> int {
+    a.max_rows = (int)(rows < 1 << 30 ? rows : 1 << 30);
+    a.max_blocks = (a.max_rows + R - 1) / R;
     // A box of the cache map: a page, or as much of it as a key tile takes.
     const int tile = R <= 32 ? attn_rows_tile(desc->head_dim) : 64;
     const int box = cache->page_size < tile ? cache->page_size : tile;
@@ -235,11 +237,9 @@ extern "C" int nvfp4_paged_attention(const nvfp4_attention_desc *desc, const nvf
     a.prev_lse = reinterpret_cast<float *>(w + L.prev_lse);
     a.prefix_pass = 1;
     a.page_table = batch->prefix_pages;
-    a.max_blocks = (int)(((int64_t)a.T * a.G + L.R0 - 1) / L.R0);
-    if ((rc = pass(L.R0, "attention launch (prefix)"))) return rc;
+    if ((rc = pass(L.R0, (int64_t)a.T * a.G, "attention launch (prefix)"))) return rc;
     a.prefix_pass = 0;
     a.page_table = batch->page_table;
   }
-  a.max_blocks = (int)(((int64_t)batch->max_q_len * a.G + L.R1 - 1) / L.R1);
-  return pass(L.R1, "attention launch");
+  return pass(L.R1, (int64_t)batch->max_q_len * a.G, "attention launch");
 }

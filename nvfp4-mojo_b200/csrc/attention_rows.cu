@@ -418,7 +418,7 @@ cudaError_t launch_rows(const CUtensorMap &tk, const CUtensorMap &tv, const Attn
   cfg.numAttrs = 1;
   if ((e = cudaLaunchKernelEx(&cfg, k, tk, tv, a)) != cudaSuccess) return e;
   constexpr int RPB = 1;
-  cfg.gridDim = dim3((unsigned)grid, C::R / RPB, 1);
+  cfg.gridDim = dim3((unsigned)grid, (unsigned)(a.max_rows < C::R ? a.max_rows : C::R), (DP + 127) / 128);
   cfg.blockDim = dim3(256, 1, 1);
   cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, attn_join_kernel<C::R, DP, kWarps, RPB>, a);
