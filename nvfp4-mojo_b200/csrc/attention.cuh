@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
 #pragma unroll 1
     for (int r = r0; r < r1; r += RPB == 1 ? gridDim.y : 8) {
       AttnParts<V> t;
-      t.template read<R, DP, 4>(a, c0, r, 0, 1, w.last_part - c0 + 1, 4 * lane);
+      t.template read<R, DP, RPB == 1 ? 4 : 2>(a, c0, r, 0, 1, w.last_part - c0 + 1, 4 * lane);
       const AttnRow ar = attn_meta_row(a, w, r);
       const AttnFinish f = attn_finish(a, ar, t.m, t.l);
 #pragma unroll
