@@ -1,0 +1,71 @@
+"""How paged_attention divides a call's work: items cut into few and into many
+parts side by side, the ways of planning (few, many and very many sequences,
+with few and with many items), bounds that are larger than the lengths, and
+two calls at once."""
+import pytest
+import torch
+
+from test_gpu_attention import batch_of, make, run_and_check
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("H,KV,D", [(8, 1, 64), (8, 2, 128), (16, 2, 256), (6, 2, 80), (4, 4, 136)])
+@pytest.mark.parametrize("tokens", [1, 2])
+def test_long_contexts_beside_short_ones(H, KV, D, tokens):
+    lens = [20011, 2, 40, 700, 3, 65, 31, 1300, 2]
+    run_and_check(make(71, lens, [tokens] * len(lens), KV, D, H, 64))
+
+
+def test_long_contexts_behind_a_prefix():
+    s = make(72, [9000, 2, 300], [1, 1, 1], 1, 256, 8, 16, prefix=5000)
+    gate = torch.randn(s["T"], s["H"], s["D"], generator=s["g"]).to(torch.bfloat16)
+    run_and_check(s, gate=gate)
+
+
+@pytest.mark.parametrize("qlens", [
+    [700], [300, 1, 0, 170], [200, 1, 1, 3, 0, 171],            # items of a sequence: many
+    [1] * 33, [20] * 33,                                        # more sequences than a warp
+    [1] * 1100, [1] * 1050 + [200], [33] + [1] * 1050,          # than the plan keeps
+])
+def test_plans(qlens):
+    g = torch.Generator().manual_seed(len(qlens))
+    lens = [n + int(torch.randint(0, 40, (1,), generator=g)) if n else 0 for n in qlens]
+    run_and_check(make(73, lens, qlens, 1, 64, 8, 16))
+
+
+@pytest.mark.parametrize("H,KV,D,qlens", [(128, 1, 64, [1, 2, 5]), (128, 1, 256, [1, 3]), (127, 1, 128, [1, 4])])
+def test_as_many_heads_per_key_as_allowed(H, KV, D, qlens):
+    run_and_check(make(74, [200 + 31 * n for n in qlens], qlens, KV, D, H, 64))
+
+
+@pytest.mark.parametrize("qlens,bound", [([1, 1, 1], 2), ([1, 2, 1], 4), ([1, 2, 3], 700), ([30, 2], 5000)])
+def test_bounds_above_the_lengths(qlens, bound):
+    lens = [400 + 97 * i for i in range(len(qlens))]
+    run_and_check(make(75, lens, qlens, 2, 128, 8, 16), single=False, max_q=bound)
+
+
+def test_two_calls_at_once_and_a_workspace_used_again():
+    """Calls on two streams with a workspace each, in turns of different shapes."""
+    import nvfp4
+
+    sets = [make(76, [3000, 17], [1, 1], 2, 128, 8, 16), make(77, [900, 500], [300, 260], 2, 128, 8, 64),
+            make(78, [700] * 6, [1] * 6, 2, 128, 8, 16, prefix=900)]
+    cfg = nvfp4.AttentionConfig(8, 2, 128, causal=True)
+    batches = [batch_of(s) for s in sets]
+    queries = [s["q"].cuda() for s in sets]
+    alone = [nvfp4.paged_attention(q, s["cache"], b, cfg) for s, b, q in zip(sets, batches, queries)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    sizes = [nvfp4.attention_workspace(cfg, b).numel() for b in batches]
+    spaces = [torch.full((max(sizes),), 0xff, dtype=torch.uint8, device="cuda") for _ in streams]
+    torch.cuda.synchronize()
+    got = []
+    for turn in range(6):
+        for i, (st, ws) in enumerate(zip(streams, spaces)):
+            with torch.cuda.stream(st):
+                k = (turn + i) % 3
+                got.append((k, nvfp4.paged_attention(queries[k], sets[k]["cache"], batches[k], cfg, workspace=ws)))
+    torch.cuda.synchronize()
+    for k, o in got:
+        assert torch.equal(o, alone[k])
