@@ -82,13 +82,17 @@ int check_desc(const nvfp4_attention_desc *d) {
   return NVFP4_OK;
 }
 
-// Query rows of an item, which also names the kernel: 16 or 32 rows on
-// attention_rows.cu while a sequence's rows per key/value head fit one item
-// (keys are read once), else attention_tc.cu.
+// Query rows of an item, which also names the kernel: 16, or 32 at head sizes up
+// to 64, on attention_rows.cu while a sequence's rows per key/value head fit one
+// item, else attention_tc.cu.  Measured on the one and on the other, 64 sequences
+// of 200 to 12000 keys, 4 key/value heads: 8 rows of 128 133 and 174 us (256
+// sequences of up to 400 keys 41 and 81), 24 to 32 rows of 128 211 and 166 us, of
+// 64 114 and 157 us; 33 rows and more, whose keys attention_rows.cu would read
+// twice, 394 and 175 us.
 int rows_of(const nvfp4_attention_desc &d, int64_t rows) {
   if (rows <= 16) return 16;
   if (d.head_dim > 128) return 128;
-  return rows <= 32 ? 32 : 256;
+  return rows <= 32 && d.head_dim <= 64 ? 32 : 256;
 }
 
 struct AttnLayout {

@@ -11,7 +11,7 @@ namespace nvfp4 {
 // `devices` remembers where that has been done.
 cudaError_t attn_allow_smem(const void *kernel, int bytes, std::atomic<uint64_t> &devices);
 
-// attention_rows.cu: items of R = 16 or 32 rows (16 above head size 128), and
+// attention_rows.cu: items of R = 16 or 32 rows (16 above head size 64), and
 // the launch that joins what its workers (warps) cut.  Key tiles of
 // attn_rows_tile tokens.
 constexpr int kAttnRowsWorkers = 8;  // per block

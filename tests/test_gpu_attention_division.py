@@ -39,6 +39,14 @@ def test_as_many_heads_per_key_as_allowed(H, KV, D, qlens):
     run_and_check(make(74, [200 + 31 * n for n in qlens], qlens, KV, D, H, 64))
 
 
+@pytest.mark.parametrize("H,KV,D", [(8, 1, 64), (10, 2, 40), (8, 1, 128), (8, 1, 136)])
+@pytest.mark.parametrize("opts", [{}, dict(window=50, softcap=8.0)])
+def test_rows_between_the_kernels(H, KV, D, opts):
+    """17 to 32 rows of a key/value head, and the first count beyond."""
+    run_and_check(make(79, [500, 3, 33, 2100], [4, 3, 0, 4], KV, D, H, 16), **opts)
+    run_and_check(make(80, [500, 5, 2100], [5, 5, 1], KV, D, H, 16, prefix=40), **opts)
+
+
 @pytest.mark.parametrize("qlens,bound", [([1, 1, 1], 2), ([1, 2, 1], 4), ([1, 2, 3], 700), ([30, 2], 5000)])
 def test_bounds_above_the_lengths(qlens, bound):
     lens = [400 + 97 * i for i in range(len(qlens))]
