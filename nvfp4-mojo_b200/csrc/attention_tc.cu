@@ -47,14 +47,18 @@ static __device__ int g_attn_tc_status;
 
 namespace {
 
-// Of an item's beginning and end, in key tiles.  (Four ragged prompts at head size
-// 256: 288 us with 2, 279 with 5, 287 with 9; three with a window of 1024: 147,
-// 153, 165.)
-constexpr int kItemCost = 5;
 constexpr int kSegs = 4;      // items that the scheduling warp may be ahead
 
 constexpr int KT = 64;        // keys per tile
 constexpr int HK = KT / 2;    // of them a softmax thread's
+
+// Of an item's beginning and end, in key tiles, which two query tiles with capped
+// or biased scores take longer for.  (A prompt of 8192, 32 / 4 heads of 128: 622 us
+// with 2, 594 with 3, 547 with 5, 570 with 7.  Four ragged ones at head size 256:
+// 288 with 2, 279 with 5, 287 with 9.  Three with cap and bias, 28 / 4 heads of 128:
+// 150 with 1, 147 with 2, 148 with 3, 153 with 5.)
+template <int DP, bool MOD>
+constexpr int kItemCost = MOD && DP <= 128 ? 2 : 5;
 
 template <int DP>
 struct TcCfg {
@@ -201,7 +205,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
     attn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const __grid_constant__ AttnArgs a) {
   using C = TcCfg<DP>;
-  constexpr int QT = C::QT, R = C::R, kSlots = C::kSlots;
+  constexpr int QT = C::QT, R = C::R, kSlots = C::kSlots, E = kItemCost<DP, MOD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                               ~static_cast<uintptr_t>(1023));
@@ -260,7 +264,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;");
-  AttnCursor cur = attn_plan<R, KT, kItemCost, 0>(a, 2 + kItemCost, &plan, C::kSoftWarps + 2);
+  AttnCursor cur = attn_plan<R, KT, E, 0>(a, 2 + E, &plan, C::kSoftWarps + 2);
   const uint32_t tmem = tmem_slot;
   if (threadIdx.x == 0) a.meta[blockIdx.x].last_part = -1;
   volatile int *abort = &abort_flag;
@@ -713,7 +717,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
             if (listed >= kSegs &&
                 !attn_wait(seg_empty + 8 * i, (listed / kSegs - 1) & 1, status, kDevTimeoutEmpty, abort))
               break;
-            more = attn_segment<R, KT, kItemCost>(a, cur, g);
+            more = attn_segment<R, KT, E>(a, cur, g);
             if (!more) g.take = -1;
             segs[i] = g;
             mbar_arrive(seg_full + 8 * i);
