@@ -529,7 +529,12 @@ __device__ __forceinline__ AttnRow attn_meta_row(const AttnArgs &a, const AttnMe
 // item that worker x leads, else block (x, y) row y of the items that the
 // workers 8 x .. 8 x + 7 lead, an item per warp.  There, items of seven parts and
 // more come last: all eight warps take every eighth part, each block z 128
-// columns, and join through shared memory.
+// columns, and join through shared memory.  Bound by latency: a part's loads
+// depend on nothing but its place, so two, four or eight parts are in flight.
+// (One context of 60000 keys, 592 parts a row: 53 us with four in flight per warp
+// and one block per row, 43 so, attention included; prompts' items of 2 to 3 parts
+// 276 us with two in flight, 287 with eight.  256 contexts of up to 400 keys: 55 us
+// with one warp per block's items, 41 with one each.)
 template <int R, int DP, int WPB, int RPB>
 __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnArgs a) {
   static_assert((WPB == 1) != (RPB == 1) && (WPB == 1 || WPB == 8), "a warp's rows");
