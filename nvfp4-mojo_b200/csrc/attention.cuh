@@ -43,7 +43,7 @@ struct AttnArgs {
   int causal, window;
   int max_rows;     // of a sequence and key/value head, by max_q_len: sizes the
   int max_blocks;   // grid of the join; and their items: who plans
-  int wide;         // a copy brings all columns of its rows, not 64 of them
+  int wide, wide_v; // a copy of keys (of values) brings all columns of its rows, not 64 of them
   float scale, softcap;
   const float *slopes;
   const __nv_bfloat16 *q, *gate;

@@ -224,12 +224,13 @@ extern "C" int nvfp4_paged_attention(const nvfp4_attention_desc *desc, const nvf
     // A box of the cache map: a page, or as much of it as a key tile takes.
     const int tile = R <= 32 ? attn_rows_tile(desc->head_dim) : 64;
     const int box = cache->page_size < tile ? cache->page_size : tile;
-    // One copy for all columns where they fill the kernel's tile; the MMA's
-    // operands also need the tile's rows in one piece.
-    a.wide = desc->head_dim == L.dp && (R <= 32 || box == tile);
+    // One copy for all columns where they fill the kernel's tile; the MMA on keys
+    // also needs the tile's rows in one piece.
+    a.wide_v = desc->head_dim == L.dp;
+    a.wide = a.wide_v && (R <= 32 || box == tile);
     CUtensorMap tk, tv;
     if (!make_cache_map(&tk, cache->k, cache->k_strides, *cache, box, a.wide) ||
-        !make_cache_map(&tv, cache->v, cache->v_strides, *cache, box, a.wide))
+        !make_cache_map(&tv, cache->v, cache->v_strides, *cache, box, a.wide_v))
       return fail(NVFP4_ERR_CUDA, "tensor map of the cache");
     return check_launch(R <= 32 ? launch_attn_rows(tk, tv, a, R, grid, st) : launch_attn_tc(tk, tv, a, grid, st),
                         what);

@@ -131,18 +131,20 @@ __device__ __forceinline__ void mma_ss4(uint32_t d, uint32_t alo, uint32_t blo, 
       : "memory");
 #undef NVFP4_SS_STEP
 }
-// D[tmem] (+)= A[tmem] B[smem] over 64 tokens: 8 columns of A and 2048 bytes
-// of B a k-step.
-__device__ __forceinline__ void mma_ts4(uint32_t d, uint32_t a, uint32_t blo, uint32_t idesc, uint32_t acc) {
+// D[tmem] (+)= A[tmem] B[smem] over 64 tokens: 8 columns of A a k-step, and of B
+// b1 (an odd step) and b2 (two steps) 16-byte units.
+__device__ __forceinline__ void mma_ts4(uint32_t d, uint32_t a, uint32_t blo, uint32_t idesc, uint32_t acc, uint32_t b1,
+                                        uint32_t b2) {
 #define NVFP4_TS_STEP(aoff, boff, pred)                                  \
-  "add.u32 x, %1, " aoff ";\n\tadd.u32 y, %2, " boff ";\n\tmov.b64 bd, {y, %5};\n\t" \
+  "add.u32 x, %1, " aoff ";\n\t" boff "mov.b64 bd, {y, %5};\n\t" \
   "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [x], bd, %3, " pred ";\n\t"
   asm volatile(
       "{\n\t.reg .pred p, q, one;\n\t.reg .b32 x, y;\n\t.reg .b64 bd;\n\t"
       "elect.sync _|q, 0xffffffff;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.u32 one, 0, 0;\n\t" NVFP4_TS_STEP("0", "0", "p")
-          NVFP4_TS_STEP("8", "128", "one") NVFP4_TS_STEP("16", "256", "one") NVFP4_TS_STEP("24", "384", "one") "}" ::"r"(d),
-      "r"(a), "r"(blo), "r"(idesc), "r"(acc), "r"(kDescHi)
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.u32 one, 0, 0;\n\t" NVFP4_TS_STEP("0", "mov.b32 y, %2;\n\t", "p")
+          NVFP4_TS_STEP("8", "add.u32 y, %2, %6;\n\t", "one") NVFP4_TS_STEP("16", "add.u32 y, %2, %7;\n\t", "one")
+              NVFP4_TS_STEP("24", "add.u32 y, y, %6;\n\t", "one") "}" ::"r"(d),
+      "r"(a), "r"(blo), "r"(idesc), "r"(acc), "r"(kDescHi), "r"(b1), "r"(b2)
       : "memory");
 #undef NVFP4_TS_STEP
 }
@@ -155,8 +157,10 @@ __device__ __forceinline__ void commit_to(uint32_t bar) {
 
 // Low word of a descriptor.  Keys and queries are K-major (the leading offset
 // is not used, 16 bytes); values [token][d], 64 columns of 128 swizzled bytes
-// per token, are an MN-major B operand: 64-column blocks KT * 128 bytes apart
-// (leading offset), groups of 8 tokens 1024 bytes apart (stride offset).
+// per token, are an MN-major B operand: 64-column blocks (leading offset) and
+// groups of 8 tokens 1024 bytes apart (stride offset).  A value tile lies box by
+// box, each with its columns' blocks one after the other, as one copy of a box
+// writes them; a key tile, block by block over all boxes, as one MMA reads it.
 __device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lead) {
   return ((saddr & 0x3FFFFu) >> 4) | (lead >> 4) << 16;
 }
@@ -586,8 +590,9 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       constexpr uint32_t idS = idesc_bf16_f32(128, KT);
       constexpr uint32_t idO = idesc_bf16_f32(128, DP) | kTransposeB;
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), sb = __shfl_sync(0xffffffffu, sbase, 0);
+      const uint32_t box = min(a.page_size, KT), b1 = box == 16 ? DP * 2 : 128, b2 = box == KT ? 256 : DP * 4;
       const uint32_t qd = desc_lo(sb + t * C::kQ, 16), kd = desc_lo(sb + C::offKV, 16),
-                     vd = desc_lo(sb + C::offKV, KT * 128);
+                     vd = desc_lo(sb + C::offKV, box * 128);
       bool ok = true;
       // The slot of the next key tile's K (its V is in the slot after) and of
       // the pending tile's V, with the parities of their rounds.
@@ -606,7 +611,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
           ++np;
           if (ok) {
             tc_fence_after();
-            mma_ts4(tm + C::colO + t * DP, tm + x * KT, vd + vslot * (C::kTile >> 4), idO, !pfirst);
+            mma_ts4(tm + C::colO + t * DP, tm + x * KT, vd + vslot * (C::kTile >> 4), idO, !pfirst, b1, b2);
             commit_to(bar_o + 8 * x);
           }
         }
@@ -657,9 +662,8 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       // ---------------- TMA producer ----------------
       const int box = a.page_size < KT ? a.page_size : KT;
       const int per = KT / box;
-      // This lane's box of a tile and its columns (wide: all of them).
+      // This lane's box of a tile and its block of columns (wide: all of them).
       const int bi = lane % per, bx = lane / per;
-      const bool used = bx < (a.wide ? 1 : DP / 64);
       const uint64_t policy = l2_evict_normal_policy();
       uint32_t at = 0;
       bool ok = true;
@@ -677,11 +681,13 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
           }
           const bool ragged = j0 < lo || j0 + KT > hi;
           const int tok = j0 + bi * box;
-          const bool mine = used && tok < hi && tok + box > lo;  // holds a key that some row sees
+          const bool seen = tok < hi && tok + box > lo;  // holds a key that some row sees
           const int page = __shfl_sync(0xffffffffu, ids, ((tok >> a.page_shift) - ids_at) & 31);
           const int row = tok & (a.page_size - 1);
-          const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * box * (a.wide ? DP * 2 : 128);
           for (int kv = 0; kv < 2; ++kv, ++at) {
+            const bool all = kv ? a.wide_v : a.wide;
+            const bool mine = seen && bx < (all ? 1 : DP / 64);
+            const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * box * (all ? DP * 2 : 128);
             const uint32_t slot = at % kSlots, round = at / kSlots;
             if (round > 0 && !__all_sync(0xffffffffu, attn_wait(empty + 8 * slot, (round - 1) & 1, status,
                                                                 kDevTimeoutEmpty, abort))) {
@@ -692,7 +698,7 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
             if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
             __syncwarp();
             if (mine)
-              attn_load_box(sbase + C::offKV + slot * C::kTile + bx * (KT * 128) + bi * box * 128, kv ? &tmV : &tmK,
+              attn_load_box(sbase + C::offKV + slot * C::kTile + (kv ? bi * (DP / 64) + bx : bx * per + bi) * box * 128, kv ? &tmV : &tmK,
                             64 * bx, row, h, page, bar, policy);
           }
         }
@@ -736,11 +742,12 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
           }
           phase ^= 1u << slot;
           uint8_t *V = smem + C::offKV + slot * C::kTile;
+          const int box = a.page_size < KT ? a.page_size : KT;
           for (int x = lane; x < KT * (DP / 8); x += 32) {
-            const int r = x / (DP / 8), c = x % (DP / 8), j = j0 + r;
+            const int r = x / (DP / 8), c = x % (DP / 8), j = j0 + r, in = r & (box - 1);
             if (j < g.it.lo || j >= g.it.hi)
-              *reinterpret_cast<uint4 *>(V + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
-                  make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4 *>(V + ((r - in) * (DP / 64) + (c >> 3) * box + in) * 128 +
+                                         (((c & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
           __syncwarp();
