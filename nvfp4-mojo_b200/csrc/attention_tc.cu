@@ -18,9 +18,9 @@
 // the last time (weights then stay below 2^8, exact in the sums' fp32); the
 // reference is the same for sum and product, so the result is not changed.
 // A row's two threads meet once per tile, to learn whether either saw such a
-// growth.  (One thread per row: 297 against 278 us for four ragged prompts at
-// head size 256, where a tile's softmax is the one in flight; 572 against 570
-// for a prompt of 8192 at 32 / 4 heads of 128.)
+// growth.  (One thread per row: 19 us more of 278, four ragged prompts at head
+// size 256, where a tile's softmax is the one in flight; 572 against 570 us for a
+// prompt of 8192 at 32 / 4 heads of 128.)
 //
 // What bounds it: that prompt runs at 970 TFLOP/s and 990 W, where the power
 // limit takes the clock from 1965 to 1680 MHz.  Per pair of query tiles and key
@@ -29,7 +29,9 @@
 // Exponentials on the FMA pipe in part (a polynomial of degree 4) give 587 to
 // 620 us from 1/8 to 1/2 of them, the exponentials of the two query tiles taken
 // in turns 597: more instructions at the same power.  Head size 256 loads 64 KB
-// per tile of 128 rows and is bound by that, 6 TB/s from L2.
+// per tile of 128 rows and is bound by that: those ragged prompts, in pages of 16,
+// take 235 us, 720 TFLOP/s (277 while a copy brought 64 of a value's columns; 213
+// without the output gate).
 #include <cuda_bf16.h>
 
 #include <type_traits>
@@ -53,10 +55,10 @@ constexpr int KT = 64;        // keys per tile
 constexpr int HK = KT / 2;    // of them a softmax thread's
 
 // Of an item's beginning and end, in key tiles, which two query tiles with capped
-// or biased scores take longer for.  (A prompt of 8192, 32 / 4 heads of 128: 622 us
-// with 2, 594 with 3, 547 with 5, 570 with 7.  Four ragged ones at head size 256:
-// 288 with 2, 279 with 5, 287 with 9.  Three with cap and bias, 28 / 4 heads of 128:
-// 150 with 1, 147 with 2, 148 with 3, 153 with 5.)
+// or biased scores take longer for.  (A prompt of 8192, 32 / 4 heads of 128: 618 us
+// with 2, 569 with 5, 569 with 8.  Four ragged ones at head size 256: 245 with 2,
+// 235 with 5, 236 with 8.  Three with cap and bias, 28 / 4 heads of 128: 150 with 1,
+// 147 with 2, 148 with 3, 153 with 5.)
 template <int DP, bool MOD>
 constexpr int kItemCost = MOD && DP <= 128 ? 2 : 5;
 
@@ -365,6 +367,11 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
       if (g.last_part >= 0 && threadIdx.x == 0) a.meta[blockIdx.x] = attn_meta<R>(a, g);
       AttnRow ar = attn_row(a, g.s, g.h, in ? row : 0);
       if (!in) ar.lo = ar.hi = 0;
+      // The gate comes from HBM: into L2 under the item's tiles.
+      if (a.gate && in && slot < 0 && !a.prefix_pass) {
+        const __nv_bfloat16 *p = a.gate + ar.token * a.g_ts + ar.head * a.g_hs;
+        for (int c = 64 * half; c < a.D; c += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + c));
+      }
       float m = -INFINITY, l = 0.0f;
       if (mine && take > 0) {
         // Keys that all rows of the warp see need no mask.
@@ -529,8 +536,9 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
               gate[i] = reinterpret_cast<const char *>(a.gate + tok * a.g_ts + head * a.g_hs + 2 * (lane & 3));
             }
           }
-          // This warp's half of the columns, 32 a step.
-          constexpr int W = 32;
+          // This warp's half of the columns, 32 a step; 64 where there are registers
+          // for the gate's and the prefix's loads of as many.
+          constexpr int W = MODE == 2 && QT == 1 ? 64 : 32;
           const int cols = min(MODE == 0 ? DP : a.D, (half + 1) * (DP / 2));
 #pragma unroll 1
           for (int c0 = half * (DP / 2); c0 < cols; c0 += W) {
