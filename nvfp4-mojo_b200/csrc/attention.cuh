@@ -547,9 +547,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
   if (blockIdx.z == 0 && __ballot_sync(0xffffffffu, leads && !wide && (WPB == 1 || lane == warp))) {
     const int c0 = blockIdx.x * WPB + (WPB == 1 ? 0 : warp);
     const AttnMeta w = a.meta[c0];
-    const int r0 = RPB * blockIdx.y + (WPB == 1 ? warp : 0), r1 = RPB == 1 ? w.live : min(w.live, RPB * (int)blockIdx.y + RPB);
 #pragma unroll 1
-    for (int r = r0; r < r1; r += RPB == 1 ? gridDim.y : 8) {
+    for (int r = RPB * blockIdx.y + (WPB == 1 ? warp : 0); r < w.live; r += RPB * gridDim.y) {
       AttnParts<V> t;
       t.template read<R, DP, RPB == 1 ? 4 : 2>(a, c0, r, 0, 1, w.last_part - c0 + 1, 4 * lane);
       const AttnRow ar = attn_meta_row(a, w, r);

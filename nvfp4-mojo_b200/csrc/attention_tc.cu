@@ -793,7 +793,8 @@ cudaError_t launch_tc(const CUtensorMap &tk, const CUtensorMap &tv, const AttnAr
   cfg.numAttrs = 1;
   if ((e = cudaLaunchKernelEx(&cfg, k, tk, tv, a)) != cudaSuccess) return e;
   constexpr int RPB = 8;
-  cfg.gridDim = dim3((unsigned)grid, C::R / RPB, 1);
+  const int rows = a.max_rows < C::R ? a.max_rows : C::R;
+  cfg.gridDim = dim3((unsigned)grid, (unsigned)((rows + RPB - 1) / RPB), 1);
   cfg.blockDim = dim3(256, 1, 1);
   cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, attn_join_kernel<C::R, DP, 1, RPB>, a);
