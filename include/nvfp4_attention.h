@@ -144,7 +144,7 @@ size_t nvfp4_attention_workspace_size(const nvfp4_attention_desc *desc,
  * q, out and gate 16-byte aligned with strides that are multiples of 8
  * elements; out may be q.  The workspace (256-byte aligned, any contents) is
  * the call's own until it has finished: calls that may run at the same time
- * need one each.  Nothing is read beyond a sequence's keys, so what the rest
+ * need one each.  Nothing beyond a sequence's keys is used, so what the rest
  * of its last page holds does not matter.  A key or value that is not finite
  * makes the outputs of the queries of the same call that read it, and may
  * make those of queries of the same sequence that do not, not finite.
