@@ -77,3 +77,37 @@ def test_two_calls_at_once_and_a_workspace_used_again():
     torch.cuda.synchronize()
     for k, o in got:
         assert torch.equal(o, alone[k])
+
+
+@pytest.mark.parametrize("qlens", [[1, 1, 1], [2, 1, 40]])
+def test_offsets_beyond_32_bits(qlens):
+    """The last pages of a cache of 2.3 G elements, rows 2^30 elements apart in
+    q: the results of a small cache and packed rows, bit for bit."""
+    import nvfp4
+
+    H, KV, D, page, far = 8, 4, 128, 64, 70000
+    T, lens = sum(qlens), [n + 130 for n in qlens]
+    g = torch.Generator().manual_seed(81)
+    rows = lambda heads: torch.randn(T, heads, D, generator=g).to(torch.bfloat16).cuda()
+    q, k, v = rows(H), rows(KV), rows(KV)
+    small = [torch.randn(12, page, KV, D, generator=g).to(torch.bfloat16).cuda() for _ in range(2)]
+    big = [torch.empty(far, page, KV, D, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    for s, b in zip(small, big):
+        b[-12:] = s
+    table = torch.randperm(12, generator=g)[:9].reshape(3, 3).to(torch.int32).cuda()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    starts = i32([0, qlens[0], qlens[0] + qlens[1], T])
+    apart = torch.empty(min(T, 3) * 2 ** 30, dtype=torch.bfloat16, device="cuda")
+    q_far = apart.as_strided((T, H, D), (2 ** 30 if T <= 3 else 2 ** 26, D, 1))
+    q_far.copy_(q)
+    cfg = nvfp4.AttentionConfig(H, KV, D, causal=True)
+    got = []
+    for cache, pages, queries in ((small, table, q), (big, table + (far - 12), q_far)):
+        cache = nvfp4.PagedKVCache(*cache)
+        batch = nvfp4.AttentionBatch(i32(lens), pages, q_start=starts, num_tokens=T, max_q_len=max(qlens))
+        turned = nvfp4.kv_append(queries, k, v, cache, batch, q_out=queries)
+        got.append((turned.clone(), nvfp4.paged_attention(turned, cache, batch, cfg)))
+    torch.cuda.synchronize()
+    for s, b in zip(small, big):
+        assert torch.equal(s, b[-12:])
+    assert torch.equal(*(x[0] for x in got)) and torch.equal(*(x[1] for x in got))
