@@ -12,9 +12,9 @@
 // heads of 256 take 36 us, 3.65 TB/s, at 160 instructions a row and 60 % of the
 // issue slots.  (Three blocks per SM with four rows in flight per lane; two blocks,
 // without spills, 41 us, four with two rows 47; products two at a time 35, but 40
-// against 35 for 32 + 2 x 4 heads of 128.)  Latency-bound for a few tokens (64 of 32 + 2 x 4 heads of 128: 4.5
-// us): then a token's heads are spread over more warps, and the first rows' loads
-// run under the angles.
+// against 35 for 32 + 2 x 4 heads of 128.)  Latency-bound for a few tokens (64 of
+// 32 + 2 x 4 heads of 128: 4.5 us): then a token's heads are spread over more warps,
+// and the first rows' loads run under the angles.
 #include <cuda_bf16.h>
 
 #include "../../include/nvfp4.h"
