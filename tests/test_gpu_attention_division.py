@@ -111,3 +111,13 @@ def test_offsets_beyond_32_bits(qlens):
     for s, b in zip(small, big):
         assert torch.equal(s, b[-12:])
     assert torch.equal(*(x[0] for x in got)) and torch.equal(*(x[1] for x in got))
+
+
+@pytest.mark.parametrize("D", [8, 24, 72, 120, 200, 248])
+@pytest.mark.parametrize("qlens", [[1, 1, 1], [1, 70, 6]])
+def test_head_sizes_that_fill_no_tile(D, qlens):
+    for prefix in (0, 33):
+        s = make(82, [n + 150 for n in qlens], qlens, 2, D, 6, 16, prefix=prefix)
+        gate = torch.randn(s["T"], s["H"], D, generator=s["g"]).to(torch.bfloat16)
+        run_and_check(s, gate=gate, window=100)
+        run_and_check(s, causal=False)
