@@ -298,6 +298,7 @@ __device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units
       // The sequence that holds unit c.at, 32 sequences at a time; then, with
       // its units per head, the item in the same way.
       int o = c.at, ub = 0;
+      bool found = false;
 #pragma unroll 1
       for (int base = 0; base < NS; base += 32) {
         const int b = base + lane;
@@ -314,14 +315,20 @@ __device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units
           c.b = base + f;
           ub = __shfl_sync(0xffffffffu, u, f);
           o -= __shfl_sync(0xffffffffu, inc, f) - ub * a.Hkv;
+          found = true;
           break;
         }
         o -= __shfl_sync(0xffffffffu, inc, 31);
       }
-      c.h = div_pos(o, ub);
+      // Token ranges that overlap can make a longer line than the caller's bounds
+      // allow for, and its length wrap: a place that is not on it is no work.
+      found = found && o >= 0 && ub > 0;
+      c.h = found ? div_pos(o, ub) : 0;
+      found = found && c.h < a.Hkv;
       o -= c.h * ub;
       const AttnSeq s = attn_seq(a, c.b);
-      const int nb = attn_blocks<R>(a, s);
+      const int nb = found ? attn_blocks<R>(a, s) : 0;
+      found = false;
 #pragma unroll 1
       for (int base = 0; base < nb; base += 32) {
         const int u = base + lane < nb ? attn_item_units<R, KT, E>(a, s, base + lane) : 0;
@@ -336,10 +343,12 @@ __device__ __forceinline__ AttnCursor attn_plan(const AttnArgs &a, int min_units
           const int f = __ffs(hit) - 1;
           c.rb = base + f;
           c.off = o - (__shfl_sync(0xffffffffu, inc, f) - __shfl_sync(0xffffffffu, u, f));
+          found = true;
           break;
         }
         o -= __shfl_sync(0xffffffffu, inc, 31);
       }
+      if (!found || c.off < 0) c.at = c.end;
     }
   }
   return c;
@@ -358,6 +367,7 @@ template <int R, int KT, int E>
 __device__ __forceinline__ bool attn_segment(const AttnArgs &a, AttnCursor &c, AttnSegment &g) {
 #pragma unroll 1
   while (c.at < c.end) {
+    if (c.b >= attn_num_seqs(a)) return false;  // (the line's end, see attn_plan)
     g.s = attn_seq(a, c.b);
     const int nb = attn_blocks<R>(a, g.s);
     if (c.rb >= nb) {  // on to the next head or sequence

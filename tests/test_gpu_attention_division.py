@@ -121,3 +121,22 @@ def test_head_sizes_that_fill_no_tile(D, qlens):
         gate = torch.randn(s["T"], s["H"], D, generator=s["g"]).to(torch.bfloat16)
         run_and_check(s, gate=gate, window=100)
         run_and_check(s, causal=False)
+
+
+def test_overlapping_token_ranges_beyond_the_bounds():
+    """Every other sequence claims all tokens: more work than the counts allow
+    for.  Nothing is followed out of range, and the next call is right."""
+    import nvfp4
+    from nvfp4 import _lib
+
+    B, T, H, KV, D = 2300, 16384, 32, 4, 64
+    k, v = (torch.zeros(8, 64, KV, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    table = torch.zeros(1, dtype=torch.int32, device="cuda").expand(B, 940).contiguous()
+    starts = torch.tensor([0, T] * (B // 2) + [0], dtype=torch.int32, device="cuda")
+    batch = nvfp4.AttentionBatch(torch.full((B,), 60000, dtype=torch.int32, device="cuda"), table, q_start=starts,
+                                 num_tokens=T, max_q_len=16)
+    q = torch.zeros(T, H, D, dtype=torch.bfloat16, device="cuda")
+    nvfp4.paged_attention(q, nvfp4.PagedKVCache(k, v), batch, nvfp4.AttentionConfig(H, KV, D, causal=False))
+    torch.cuda.synchronize()
+    assert _lib.load().nvfp4_device_status() == 0
+    run_and_check(make(83, [300, 20], [1, 20], 2, 64, 8, 16))
