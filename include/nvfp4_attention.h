@@ -67,7 +67,7 @@ typedef struct nvfp4_attention_batch {
   const int32_t *q_start;       /* [num_seqs + 1], or NULL: num_seqs == num_tokens */
   const int32_t *kv_len;        /* [num_seqs], this call's tokens included */
   const int32_t *page_table;    /* [num_seqs, max_pages] */
-  int64_t page_table_stride;
+  int64_t page_table_stride;    /* at least max_pages, or 0: one row for all sequences */
   int32_t max_pages;
   int32_t prefix_len;           /* 0: none */
   const int32_t *prefix_pages;  /* [ceil(prefix_len / page_size)] */

@@ -59,7 +59,9 @@ int check_attention_batch(const nvfp4_attention_batch *b, int page_size) {
     return fail(NVFP4_ERR_INVALID_ARG, "bad lengths: max_pages %d, prefix_len %d", b->max_pages, b->prefix_len);
   if (b->prefix_len > 0 && !b->prefix_pages) return fail(NVFP4_ERR_INVALID_ARG, "null prefix_pages");
   if (b->num_seqs > 0 && !b->kv_len) return fail(NVFP4_ERR_INVALID_ARG, "null kv_len");
-  if (b->num_seqs > 0 && b->max_pages > 0 && (!b->page_table || b->page_table_stride < b->max_pages))
+  // (One row for all sequences is a stride of 0; of one sequence it means nothing.)
+  if (b->num_seqs > 0 && b->max_pages > 0 &&
+      (!b->page_table || (b->num_seqs > 1 && b->page_table_stride != 0 && b->page_table_stride < b->max_pages)))
     return fail(NVFP4_ERR_INVALID_ARG, "null page_table or stride below max_pages");
   return NVFP4_OK;
 }

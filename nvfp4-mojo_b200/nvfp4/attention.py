@@ -101,7 +101,8 @@ class PagedKVCache:
 
 class AttentionBatch:
     """One step's sequences.  kv_len int32 [B]: each sequence's keys, this
-    step's tokens included; page_table int32 [B, max_pages]; q_start int32
+    step's tokens included; page_table int32 [B, max_pages] (one row expanded to
+    B where all sequences have the same pages); q_start int32
     [B + 1]: the tokens of sequence b are rows q_start[b] : q_start[b + 1] of
     the call (None: one token per sequence), at most max_q_len each, num_tokens
     in all.  prefix_pages int32 and prefix_len: a prefix that every sequence
@@ -119,6 +120,10 @@ class AttentionBatch:
         _i32(page_table, "page_table", 2)
         if page_table.shape[0] != B or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
             raise ValueError("page_table must be [num_seqs, max_pages] with contiguous rows")
+        # The rows' distance means nothing for one row; 0 is one row expanded to all sequences.
+        table_stride = page_table.stride(0) if B > 1 else page_table.shape[1]
+        if 0 < table_stride < page_table.shape[1]:
+            raise ValueError("page_table rows must not overlap")
         if q_start is None:
             if max_q_len != 1 or num_tokens not in (None, B):
                 raise ValueError("without q_start every sequence has one token")
@@ -140,8 +145,8 @@ class AttentionBatch:
         self.prefix_len, self.device = int(prefix_len), kv_len.get_device()
         p = lambda t: None if t is None else t.data_ptr()
         self._c = _lib.AttnBatch(B, self.max_q_len, self.num_tokens, p(q_start), kv_len.data_ptr(),
-                                 page_table.data_ptr(), max(page_table.stride(0), page_table.shape[1]),
-                                 page_table.shape[1], self.prefix_len, p(prefix_pages),
+                                 page_table.data_ptr(), table_stride, page_table.shape[1],
+                                 self.prefix_len, p(prefix_pages),
                                  p(visible_len))
         self._ref = ctypes.byref(self._c)
 
