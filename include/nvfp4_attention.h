@@ -98,7 +98,8 @@ typedef struct nvfp4_qk_norm {
 /*
  * For every token of the batch: q normed and rotated into q_out (may be q
  * itself), k normed and rotated into the cache, v into the cache.  q, k, v
- * are rows of in_dtype (bf16 or f32), q_out and the cache bf16.  positions
+ * are rows of in_dtype (bf16 or f32), q_out and the cache bf16; other overlaps
+ * of q_out's rows, with each other or with q, k and v, are refused.  positions
  * [num_axes, num_tokens] with row stride position_stride, or NULL: the
  * token's position on every axis.  rotary or norm NULL: none.  The angle is
  * exact to fp32 for every int32 position.  A token whose key lies outside the
@@ -142,7 +143,8 @@ size_t nvfp4_attention_workspace_size(const nvfp4_attention_desc *desc,
  * scores.  A query that sees no key gets 0 and -inf; a token outside every
  * sequence leaves out and lse as they were.  slopes fp32 [num_heads] or NULL.
  * q, out and gate 16-byte aligned with strides that are multiples of 8
- * elements; out may be q.  The workspace (256-byte aligned, any contents) is
+ * elements; out may be q or gate (the same rows in the same places), and is
+ * refused where its rows overlap theirs or each other otherwise.  The workspace (256-byte aligned, any contents) is
  * the call's own until it has finished: calls that may run at the same time
  * need one each.  Nothing beyond a sequence's keys is used, so what the rest
  * of its last page holds does not matter.  A key or value that is not finite

@@ -49,7 +49,8 @@ typedef struct nvfp4_norm_desc {
 /*
  * residual, post_weight and gate may be NULL; one of residual_out and y may
  * be NULL, and y is written where pre_weight is not NULL.  residual_out may
- * be residual or x (same dtype and stride); y may be x in the same way.
+ * be residual or x (same dtype and stride); y may be x in the same way.  Other
+ * overlaps of an output with x, residual, gate or the other output are refused.
  */
 int nvfp4_norm_residual(const nvfp4_norm_desc *desc, const void *x, const void *residual,
                         const void *post_weight, const void *gate, const void *pre_weight,

@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include "../../include/nvfp4_attention.h"
+#include "abi_util.h"
 
 namespace nvfp4 {
 
@@ -14,5 +15,10 @@ namespace nvfp4 {
 // with its message recorded.
 int check_kv_cache(const nvfp4_kv_cache *c);
 int check_attention_batch(const nvfp4_attention_batch *b, int page_size);
+
+// What a call reads or writes of `tokens` x `heads` rows of `dim` values.
+inline RowSpan head_span(const nvfp4_head_rows &r, int64_t tokens, int64_t heads, int dim, int esize) {
+  return RowSpan{r.data, (int64_t)dim * esize, {tokens, heads}, {r.token_stride * esize, r.head_stride * esize}};
+}
 
 }  // namespace nvfp4

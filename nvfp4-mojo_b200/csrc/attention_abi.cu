@@ -176,6 +176,19 @@ extern "C" int nvfp4_paged_attention(const nvfp4_attention_desc *desc, const nvf
                 "q, out and gate: not null, 16-byte aligned, strides multiples of 8 elements");
   if (q->data == out->data && (q->token_stride != out->token_stride || q->head_stride != out->head_stride))
     return fail(NVFP4_ERR_INVALID_ARG, "out is q with another stride");
+  // Rows are written while others are still read: in their own places only.
+  auto span = [&](const nvfp4_head_rows *r) {
+    return head_span(*r, batch->num_tokens, desc->num_heads, desc->head_dim, 2);
+  };
+  const RowSpan so = span(out), sq = span(q);
+  if (rows_overlap(so)) return fail(NVFP4_ERR_INVALID_ARG, "rows of out overlap");
+  if ((!same_rows(so, sq) && rows_overlap(so, sq)) || (gate && !same_rows(so, span(gate)) && rows_overlap(so, span(gate))))
+    return fail(NVFP4_ERR_INVALID_ARG, "out overlaps q or gate in other places than its own");
+  if (lse) {
+    const RowSpan sl = {lse, (int64_t)batch->num_tokens * desc->num_heads * 4, {1, 1}, {0, 0}};
+    if (rows_overlap(sl, so) || rows_overlap(sl, sq) || (gate && rows_overlap(sl, span(gate))))
+      return fail(NVFP4_ERR_INVALID_ARG, "lse overlaps q, gate or out");
+  }
   const int grid = attn_sms();
   const AttnLayout L = attn_layout(*desc, *batch, grid);
   if (!ws || !aligned(ws, 256)) return fail(NVFP4_ERR_INVALID_ARG, "null workspace or not 256-byte aligned");

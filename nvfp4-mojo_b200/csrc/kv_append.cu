@@ -406,10 +406,20 @@ extern "C" int nvfp4_kv_append(const nvfp4_kv_cache *cache, const nvfp4_attentio
   if (batch->num_tokens == 0 || batch->num_seqs == 0) return NVFP4_OK;
   if (!q->data || !k->data || !v->data || !q_out->data) return fail(NVFP4_ERR_INVALID_ARG, "null row pointer");
   const int esize = in_dtype == NVFP4_DTYPE_BF16 ? 2 : 4;
-  auto overlaps = [](const nvfp4_head_rows *a, const nvfp4_head_rows *b) { return a->data == b->data; };
-  if (overlaps(q, q_out) && (esize != 2 || q->token_stride != q_out->token_stride ||
-                             q->head_stride != q_out->head_stride))
+  if (q->data == q_out->data &&
+      (esize != 2 || q->token_stride != q_out->token_stride || q->head_stride != q_out->head_stride))
     return fail(NVFP4_ERR_INVALID_ARG, "q_out is q with another dtype or stride");
+  // Rows are written while others are still read: in their own places only.
+  auto span = [&](const nvfp4_head_rows *r, int heads, int es) {
+    return head_span(*r, batch->num_tokens, heads, cache->head_dim, es);
+  };
+  const RowSpan so = span(q_out, num_heads, 2), sq = span(q, num_heads, esize);
+  if (rows_overlap(so)) return fail(NVFP4_ERR_INVALID_ARG, "rows of q_out overlap");
+  if ((!same_rows(so, sq) && rows_overlap(so, sq)) || rows_overlap(so, span(k, cache->num_kv_heads, esize)) ||
+      rows_overlap(so, span(v, cache->num_kv_heads, esize)))
+    return fail(NVFP4_ERR_INVALID_ARG, "q_out overlaps k, v, or q in other places than its own");
+  if (cache->num_pages > 0 && cache->k == cache->v)
+    return fail(NVFP4_ERR_INVALID_ARG, "keys and values share their places in the cache");
   AppendArgs a = {};
   a.c = *cache;
   a.b = *batch;

@@ -264,6 +264,18 @@ extern "C" int nvfp4_norm_residual(const nvfp4_norm_desc *d, const void *x, cons
     return fail(NVFP4_ERR_INVALID_ARG, "y is residual with another stride or dtype");
   if (y && y == r_out) return fail(NVFP4_ERR_INVALID_ARG, "y and residual_out are the same buffer");
   if (!x) return fail(NVFP4_ERR_INVALID_ARG, "null x");
+  auto span = [&](const void *p, int dt, int64_t stride, int64_t cols) {
+    const int es = dt == kBF16 ? 2 : 4;
+    return RowSpan{p, cols * es, {d->rows, 1}, {stride * es, 0}};
+  };
+  const RowSpan outs[2] = {span(r_out, d->residual_dtype, d->residual_out_stride, H), span(y, d->y_dtype, d->y_stride, H)};
+  const RowSpan ins[3] = {span(x, d->x_dtype, d->x_stride, H), span(residual, d->residual_dtype, d->residual_stride, H),
+                          span(gate, kBF16, d->gate_row_stride, d->gate_col_stride ? H : 1)};
+  for (const RowSpan &o : outs)
+    for (const RowSpan &i : ins)
+      if (o.base && i.base && !same_rows(o, i) && rows_overlap(o, i))
+        return fail(NVFP4_ERR_INVALID_ARG, "an output overlaps x, residual or gate in other places than its own");
+  if (r_out && y && rows_overlap(outs[0], outs[1])) return fail(NVFP4_ERR_INVALID_ARG, "y and residual_out overlap");
   NormArgs a;
   a.d = *d;
   a.x = x;

@@ -32,6 +32,88 @@ int check_launch(cudaError_t e, const char *what) {
 
 bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
+namespace {
+
+typedef __int128 Wide;  // strides are the caller's, and may be anything
+
+// A row of `lb` bytes at x + i * s, for some i in [lo, hi], meets one of `la` bytes at 0.
+bool row_meets(Wide x, Wide s, Wide lo, Wide hi, Wide la, Wide lb) {
+  if (lo > hi) return false;
+  if (s < 0) {
+    const Wide t = lo;
+    lo = -hi, hi = -t, s = -s;
+  }
+  if (s == 0) return x > -lb && x < la;
+  // The first i with x + i * s > -lb.
+  const Wide need = -lb + 1 - x;
+  Wide i = need > 0 ? (need + s - 1) / s : -(-need / s);
+  if (i < lo) i = lo;
+  return i <= hi && x + i * s < la;
+}
+
+// The span's memory from its base on: [first, second).
+void extent(const RowSpan &a, Wide &lo, Wide &hi) {
+  lo = 0, hi = a.bytes;
+  for (int d = 0; d < 2; ++d) {
+    const Wide reach = (Wide)(a.n[d] - 1) * a.stride[d];
+    (reach < 0 ? lo : hi) += reach;
+  }
+}
+
+// Strides of dimensions that have one place mean nothing: as 0.
+RowSpan plain(RowSpan a) {
+  for (int d = 0; d < 2; ++d)
+    if (a.n[d] == 1) a.stride[d] = 0;
+  return a;
+}
+
+}  // namespace
+
+bool rows_overlap(const RowSpan &x) {
+  const RowSpan a = plain(x);
+  auto size = [](int64_t s) { return s < 0 ? -(Wide)s : (Wide)s; };
+  for (int d = 0; d < 2; ++d) {  // one dimension's rows side by side within a step of the other
+    const int e = 1 - d;
+    if ((a.n[d] <= 1 || size(a.stride[d]) >= a.bytes) &&
+        (a.n[e] <= 1 || size(a.stride[e]) >= (a.n[d] - 1) * size(a.stride[d]) + a.bytes))
+      return false;
+  }
+  for (int64_t j = 0; j < a.n[1]; ++j)
+    if (row_meets((Wide)j * a.stride[1], a.stride[0], j ? -(Wide)(a.n[0] - 1) : 1, a.n[0] - 1, a.bytes, a.bytes))
+      return true;
+  return false;
+}
+
+bool rows_overlap(const RowSpan &x, const RowSpan &y) {
+  RowSpan a = plain(x), b = plain(y);
+  if (a.n[0] <= 0 || a.n[1] <= 0 || b.n[0] <= 0 || b.n[1] <= 0) return false;
+  const Wide far = (Wide) reinterpret_cast<uintptr_t>(b.base) - (Wide) reinterpret_cast<uintptr_t>(a.base);
+  Wide al, ah, bl, bh;
+  extent(a, al, ah);
+  extent(b, bl, bh);
+  if (far + bl >= ah || far + bh <= al) return false;
+  for (int d = 0; d < 2; ++d) {
+    if (a.n[d] == 1) a.stride[d] = b.stride[d];
+    if (b.n[d] == 1) b.stride[d] = a.stride[d];
+  }
+  if (a.stride[0] != b.stride[0]) return true;
+  // All of a token as one piece of memory first, then row by row.
+  const Wide ra = (Wide)(a.n[1] - 1) * a.stride[1], rb = (Wide)(b.n[1] - 1) * b.stride[1];
+  if (!row_meets(far + (rb < 0 ? rb : 0) - (ra < 0 ? ra : 0), a.stride[0], 1 - a.n[0], b.n[0] - 1,
+                 a.bytes + (ra < 0 ? -ra : ra), b.bytes + (rb < 0 ? -rb : rb)))
+    return false;
+  if (a.stride[1] != b.stride[1]) return true;
+  for (int64_t j = 1 - a.n[1]; j < b.n[1]; ++j)
+    if (row_meets(far + (Wide)j * a.stride[1], a.stride[0], 1 - a.n[0], b.n[0] - 1, a.bytes, b.bytes)) return true;
+  return false;
+}
+
+bool same_rows(const RowSpan &x, const RowSpan &y) {
+  const RowSpan a = plain(x), b = plain(y);
+  return a.base == b.base && a.bytes == b.bytes && a.n[0] == b.n[0] && a.n[1] == b.n[1] &&
+         a.stride[0] == b.stride[0] && a.stride[1] == b.stride[1];
+}
+
 }  // namespace nvfp4
 
 using namespace nvfp4;
