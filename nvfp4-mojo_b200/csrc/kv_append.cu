@@ -9,7 +9,7 @@
 // Norm weight and rotation are one 2 x 2 matrix per pair, inv (x A - y B, y C +
 // x E), and the rows ahead are loaded before the present ones are turned.  Bound
 // by the issue of its instructions more than by HBM: 6424 tokens of 16 + 2 x 2
-// heads of 256 take 36 us, 3.65 TB/s, at 160 instructions a row and 60 % of the
+// heads of 256 take 37 us, 3.60 TB/s, at 160 instructions a row and 60 % of the
 // issue slots.  (Three blocks per SM with four rows in flight per lane; two blocks,
 // without spills, 41 us, four with two rows 47; products two at a time 35, but 40
 // against 35 for 32 + 2 x 4 heads of 128.)  Latency-bound for a few tokens (64 of
@@ -339,7 +339,12 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 3) kv_append_kernel(AppendA
       if (wr.kind < 2) {  // values pass as they are, whatever they are
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float u = x[i] * A[i] - y[i] * B[i], v = y[i] * C[i] + x[i] * E[i];
+          // (A pair that is not turned has no product with its partner, which may be infinite.)
+          float u = x[i] * A[i], v = y[i] * C[i];
+          if (4 * l + (MODE == kHalves ? 0 : i) < half) {  // (halves: four pairs alike)
+            u = fmaf(-y[i], B[i], u);
+            v = fmaf(x[i], E[i], v);
+          }
           x[i] = u * inv, y[i] = v * inv;
         }
       }

@@ -37,3 +37,38 @@ def test_one_page_table_row_for_all_sequences(qlens):
     for a, b in zip(*got):
         assert torch.equal(a, b)
     assert not (got[0][1] == 0.5).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rotary,inter", [(0, False), (64, False), (64, True), (6, False), (128, False)])
+@pytest.mark.parametrize("norm", [False, True])
+def test_append_of_values_that_are_not_finite(dtype, rotary, inter, norm):
+    """What is not turned passes by itself: an infinity or a NaN stays in its
+    place, and in its pair where that is turned."""
+    import nvfp4
+
+    H, KV, D, qlens = 4, 2, 128, [3, 5]
+    s = make(90, [n + 9 for n in qlens], qlens, KV, D, H, 16, poison=False)
+    T = s["T"]
+    x = torch.randn(T, H + 2 * KV, D, generator=s["g"]).to(dtype)
+    x[0, 0, 3], x[1, 1, 70], x[2, 2, 127], x[3, 3, 100] = math.inf, -math.inf, math.nan, math.inf
+    x[4, H, 65], x[5, H + 1, 126], x[6, H + KV, 9], x[7, H + KV + 1, 64] = -math.inf, math.nan, math.inf, -math.inf
+    inv = (1e4 ** (-torch.arange(rotary // 2, dtype=torch.float64) / max(rotary // 2, 1))).float()
+    w = (1 + 0.3 * torch.randn(D, generator=s["g"])).to(torch.bfloat16) if norm else None
+    cu = lambda t: None if t is None else t.cuda()
+    q, k, v = x.cuda().split([H, KV, KV], 1)
+    got = nvfp4.kv_append(q, k, v, s["cache"], batch_of(s), q_norm=cu(w), k_norm=cu(w),
+                          rotary=nvfp4.Rotary(inv.cuda(), interleaved=inter) if rotary else None)
+    rows = x.double()
+    if norm:
+        rows = torch.cat([ref.head_norm(rows[:, :H + KV], w, 1e-6, 0.0), rows[:, H + KV:]], 1)
+    own = torch.cat([torch.arange(n - m, n) for n, m in zip(s["kv_len"].tolist(), qlens)])
+    if rotary:
+        rows = torch.cat([ref.rotate(rows[:, :H + KV], own[:, None].double() * inv.double(), inter),
+                          rows[:, H + KV:]], 1)
+    seq = torch.repeat_interleave(torch.arange(2), torch.tensor(qlens))
+    at = (s["table"][seq, own // 16].long(), own % 16)
+    got = torch.cat([got.cpu(), s["cache"].k.cpu()[at], s["cache"].v.cpu()[at]], 1)
+    # As for the finite rows: one rounding to bf16 and fp32 before it.
+    size = torch.where(torch.isfinite(rows), rows, 0.0).abs().amax(-1, keepdim=True)
+    ref.check(got, rows, ref.BF16 * rows.abs() + 1.01 * size * (ref.F32 * (D + 40) + 2.0 ** -20), "rows")
