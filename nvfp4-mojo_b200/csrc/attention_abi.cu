@@ -1,6 +1,7 @@
 // attention_abi.cu -- nvfp4_paged_attention: checks, the workspace's layout
 // and the passes (include/nvfp4_attention.h).
 #include <atomic>
+#include <cfloat>
 #include <cmath>
 
 #include "../../include/nvfp4.h"
@@ -215,6 +216,7 @@ extern "C" int nvfp4_paged_attention(const nvfp4_attention_desc *desc, const nvf
   a.window = desc->window;
   a.scale = desc->scale;
   a.softcap = desc->softcap;
+  a.inv_cap = desc->softcap > 0.0f ? fminf(1.0f / desc->softcap, FLT_MAX) : 0.0f;  // (of a cap that is not normal)
   a.slopes = slopes;
   a.q = static_cast<const __nv_bfloat16 *>(q->data);
   a.q_ts = q->token_stride;

@@ -264,9 +264,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
               float v = s[mt][n][2 * e + x];
               if constexpr (MOD) {
                 v *= a.scale;
-                if (a.softcap > 0.0f)  // cap tanh(v / cap)
-                  v = a.softcap - __fdividef(2.0f * a.softcap, 1.0f + ex2(v * (2.0f * kLog2e / a.softcap)));
-                v = fmaf(v, kLog2e, -slope[mt][e] * fabsf(dist[mt][e] - (float)j));
+                v = a.softcap > 0.0f ? a.softcap * tanh_log2e(v * a.inv_cap) : v * kLog2e;
+                v = fmaf(-slope[mt][e], fabsf(dist[mt][e] - (float)j), v);
               } else {
                 v *= sl2;
               }

@@ -193,10 +193,10 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 // The largest of three.
@@ -378,8 +378,6 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
         const int lo_all = __reduce_max_sync(0xffffffffu, ar.lo), hi_all = __reduce_min_sync(0xffffffffu, ar.hi);
         const float slope = MOD && a.slopes ? a.slopes[ar.head] * kLog2e : 0.0f;
         const int pos = ar.pos - (a.prefix_pass ? 0 : a.prefix_len);
-        const float cap_in = MOD && a.softcap > 0.0f ? 2.0f * kLog2e / a.softcap * a.scale : 0.0f;
-        const float cap_out = -2.0f * kLog2e * a.softcap;
 #pragma unroll 1
         for (int u = 0; u < take; ++u, ++n) {
           const int j0 = j_first + u * KT + half * HK;
@@ -395,9 +393,22 @@ __global__ void __launch_bounds__(TcCfg<DP>::kThreads, 1)
 #pragma unroll
           for (int c = 0; c < HK; ++c) s[c] = __uint_as_float(raw[c]);
           if constexpr (MOD) {
-            if (a.softcap > 0.0f) {  // cap tanh(scale s / cap) = cap - 2 cap / (1 + e^(2 scale s / cap)), base 2
+            if (a.softcap > 0.0f) {  // cap tanh(scale s / cap), base 2 (tanh_log2e, two at a time)
 #pragma unroll
-              for (int c = 0; c < HK; ++c) s[c] = fmaf(rcp(1.0f + ex2(s[c] * cap_in)), cap_out, -0.5f * cap_out);
+              for (int c = 0; c < HK; c += 2) {
+                float x0, x1, q0, q1;
+                unpair(mul2(mul2(pair(s[c], s[c + 1]), pair(a.scale, a.scale)), pair(a.inv_cap, a.inv_cap)), x0, x1);
+                const uint64_t t = pair(hold(x0, kTanhMax), hold(x1, kTanhMax)), u = mul2(t, t);
+                uint64_t p = pair(tanh_p(4), tanh_p(4)), q = pair(tanh_q(4), tanh_q(4));
+#pragma unroll
+                for (int k = 3; k >= 0; --k) {
+                  p = fma2(p, u, pair(tanh_p(k), tanh_p(k)));
+                  q = fma2(q, u, pair(tanh_q(k), tanh_q(k)));
+                }
+                unpair(q, q0, q1);
+                p = mul2(mul2(mul2(t, p), pair(rcp(q0), rcp(q1))), pair(a.softcap, a.softcap));
+                unpair(p, s[c], s[c + 1]);
+              }
             } else {
 #pragma unroll
               for (int c = 0; c < HK; ++c) s[c] *= a.scale * kLog2e;

@@ -72,3 +72,29 @@ def test_append_of_values_that_are_not_finite(dtype, rotary, inter, norm):
     # As for the finite rows: one rounding to bf16 and fp32 before it.
     size = torch.where(torch.isfinite(rows), rows, 0.0).abs().amax(-1, keepdim=True)
     ref.check(got, rows, ref.BF16 * rows.abs() + 1.01 * size * (ref.F32 * (D + 40) + 2.0 ** -20), "rows")
+
+
+@pytest.mark.parametrize("cap", [0.5, 3.0, 50.0, 1e3, 1e4, 1e6, 1e20, 3e38])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("tokens", [1, 3, 90])
+def test_caps_of_every_size(cap, D, tokens):
+    """One key per query (window 1), so that the log-sum-exp is the capped
+    score itself: its error goes with the score and not with the cap."""
+    import nvfp4
+
+    H, KV, qlens = 4, 1, [tokens, tokens, tokens]
+    s = make(91, [tokens + 40, tokens, tokens + 3], qlens, KV, D, H, 16)
+    _, lse = nvfp4.paged_attention(s["q"].cuda(), s["cache"], batch_of(s),
+                                   nvfp4.AttentionConfig(H, KV, D, window=1, softcap=cap), return_lse=True)
+    own = torch.cat([torch.arange(n - tokens, n) for n in s["kv_len"].tolist()])
+    seq = torch.repeat_interleave(torch.arange(3), tokens)
+    key = s["k"][s["table"][seq, own // 16].long(), own % 16, 0].double()
+    x = s["q"].double()
+    want = torch.einsum("thd,td->th", x, key) / math.sqrt(D)
+    size = torch.einsum("thd,td->th", x.abs(), key.abs()) / math.sqrt(D)
+    c64 = float(torch.tensor(cap, dtype=torch.float32))
+    want = c64 * torch.tanh(want / c64)
+    # The product's sum and the scale: D + 4 roundings of its terms' size, which
+    # the cap never enlarges; then the cap in fp32 (16 roundings of the result)
+    # and the way to base 2 and back (4).
+    ref.check(lse, want, ref.F32 * ((D + 4) * size + 20 * want.abs()), "lse")
