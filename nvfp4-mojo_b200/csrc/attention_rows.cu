@@ -133,8 +133,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   const int qr = lane >> 2, qc = lane & 3;
   const float sl2 = a.scale * kLog2e;
   uint32_t qf[MT][DP / 16][4];
-  int lo[MT][2], hi[MT][2];
-  float slope[MT][2], dist[MT][2], m[MT][2], l[MT][2], o[MT][DP / 8][4];
+  int lo[MT][2], hi[MT][2], pos[MT][2];
+  float slope[MT][2], m[MT][2], l[MT][2], o[MT][DP / 8][4];
 
   while (true) {
     // ---- loads
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
           const AttnRow r = attn_row(a, g.s, g.h, in ? row : 0);
           lo[mt][e] = in ? r.lo : 0;
           hi[mt][e] = in ? r.hi : 0;
-          dist[mt][e] = (float)(r.pos - (a.prefix_pass ? 0 : a.prefix_len));
+          pos[mt][e] = r.pos - (a.prefix_pass ? 0 : a.prefix_len);
           slope[mt][e] = MOD && a.slopes ? a.slopes[r.head] * kLog2e : 0.0f;
           src[e] = in ? reinterpret_cast<const uint32_t *>(a.q + r.token * a.q_ts + r.head * a.q_hs) : nullptr;
           m[mt][e] = -INFINITY;
@@ -256,6 +256,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float top = -INFINITY;
+          // Subtracted as integers: a position beyond 2^24 is no fp32 number.
+          const float dist = (float)(pos[mt][e] - j0 - 2 * qc);
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -265,7 +267,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
               if constexpr (MOD) {
                 v *= a.scale;
                 v = a.softcap > 0.0f ? a.softcap * tanh_log2e(v * a.inv_cap) : v * kLog2e;
-                v = fmaf(-slope[mt][e], fabsf(dist[mt][e] - (float)j), v);
+                v = fmaf(-slope[mt][e], fabsf(dist - (float)(8 * n + x)), v);
               } else {
                 v *= sl2;
               }

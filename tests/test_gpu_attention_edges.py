@@ -98,3 +98,30 @@ def test_caps_of_every_size(cap, D, tokens):
     # the cap never enlarges; then the cap in fp32 (16 roundings of the result)
     # and the way to base 2 and back (4).
     ref.check(lse, want, ref.F32 * ((D + 4) * size + 20 * want.abs()), "lse")
+
+
+@pytest.mark.parametrize("n", [2 ** 24 + 2, 2 ** 25 + 77])
+@pytest.mark.parametrize("tokens", [1, 4, 70])
+@pytest.mark.parametrize("D", [64, 128])
+def test_distances_at_far_positions(n, tokens, D):
+    """The bias goes by whole distances, also where fp32 no longer holds the
+    positions.  A window keeps the keys few; the table names eight pages in turn."""
+    import nvfp4
+
+    H, KV, page, window = 4, 1, 256, 50
+    g = torch.Generator().manual_seed(92)
+    k, v = (torch.randn(8, page, KV, D, generator=g).to(torch.bfloat16) for _ in range(2))
+    q = torch.randn(tokens, H, D, generator=g).to(torch.bfloat16)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    table = (torch.arange(-(-n // page), device="cuda") % 8).to(torch.int32)[None]
+    batch = nvfp4.AttentionBatch(i32([n]), table, q_start=i32([0, tokens]), num_tokens=tokens, max_q_len=tokens)
+    slopes = torch.tensor([1.0, 0.5, 0.25, 2.0])
+    out, lse = nvfp4.paged_attention(q.cuda(), nvfp4.PagedKVCache(k.cuda(), v.cuda()), batch,
+                                     nvfp4.AttentionConfig(H, KV, D, window=window), slopes=slopes.cuda(),
+                                     return_lse=True)
+    # The same as a short sequence: the last keys alone, behind a multiple of the eight pages.
+    first = (n - tokens - window) // (8 * page) * (8 * page)
+    o, l, o_tol, l_tol = ref.attention(q, k, v, [n - first], (torch.arange(-(-(n - first) // page)) % 8)[None],
+                                       [0, tokens], window=window, slopes=slopes)
+    ref.check(out, o, o_tol, "out")
+    ref.check(lse, l, l_tol, "lse")
