@@ -213,7 +213,9 @@ extern "C" int nvfp4_paged_attention(const nvfp4_attention_desc *desc, const nvf
   a.visible = batch->visible_len;
   a.prefix_len = batch->prefix_len;
   a.causal = desc->causal != 0;
-  a.window = desc->window;
+  // Positions stay below 2^30 (check_attention_batch), so a longer window masks
+  // nothing either; below the first key, a position less a longer one would wrap.
+  a.window = desc->window < 1 << 30 ? desc->window : 1 << 30;
   a.scale = desc->scale;
   a.softcap = desc->softcap;
   a.inv_cap = desc->softcap > 0.0f ? fminf(1.0f / desc->softcap, FLT_MAX) : 0.0f;  // (of a cap that is not normal)

@@ -10,6 +10,7 @@ import attention_ref as ref
 from test_gpu_attention import append_case, batch_of, make, run_and_check, test_norm_residual as norm_case
 
 pytestmark = pytest.mark.gpu
+I32_MAX = 2 ** 31 - 1
 
 
 @pytest.mark.parametrize("qlens", [[1, 1, 1, 1], [2, 40, 1, 9]])
@@ -125,3 +126,13 @@ def test_distances_at_far_positions(n, tokens, D):
                                        [0, tokens], window=window, slopes=slopes)
     ref.check(out, o, o_tol, "out")
     ref.check(lse, l, l_tol, "lse")
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("window", [I32_MAX, I32_MAX - 3, 2 ** 30, 2 ** 30 + 1])
+def test_windows_as_long_as_the_type(causal, window):
+    """A window beyond every sequence masks nothing, also for the tokens that
+    stand before the first key."""
+    run_and_check(make(8, [3, 40], [7, 2], width=4), causal=causal, window=window)
+    run_and_check(make(93, [30, 9], [200, 9], 1, 128, 8, 16), causal=causal, window=window)
+    run_and_check(make(94, [3, 0, 40], [70, 1, 2], 2, 64, 8, 16, prefix=20), causal=causal, window=window)
