@@ -70,6 +70,14 @@ def _i32(t: torch.Tensor, name: str, dim: int) -> torch.Tensor:
     return t
 
 
+def _int32(x, name: str) -> int:
+    """x for an int32 field: ctypes would drop the bits beyond it."""
+    x = int(x)
+    if not -2 ** 31 <= x < 2 ** 31:
+        raise ValueError(f"{name} {x} is out of range")
+    return x
+
+
 class PagedKVCache:
     """Keys and values in pages: k and v bf16 [num_pages, page_size,
     num_kv_heads, head_dim], any strides with contiguous heads (a permuted
@@ -141,13 +149,12 @@ class AttentionBatch:
         _check_device(kv_len, page_table=page_table, q_start=q_start, prefix_pages=prefix_pages,
                       visible_len=visible_len)
         self.tensors = (kv_len, page_table, q_start, prefix_pages, visible_len)
-        self.num_seqs, self.num_tokens, self.max_q_len = B, int(num_tokens), int(max_q_len)
-        self.prefix_len, self.device = int(prefix_len), kv_len.get_device()
+        self.num_seqs, self.num_tokens, self.max_q_len = B, int(num_tokens), _int32(max_q_len, "max_q_len")
+        self.prefix_len, self.device = _int32(prefix_len, "prefix_len"), kv_len.get_device()
         p = lambda t: None if t is None else t.data_ptr()
         self._c = _lib.AttnBatch(B, self.max_q_len, self.num_tokens, p(q_start), kv_len.data_ptr(),
                                  page_table.data_ptr(), table_stride, page_table.shape[1],
-                                 self.prefix_len, p(prefix_pages),
-                                 p(visible_len))
+                                 self.prefix_len, p(prefix_pages), p(visible_len))
         self._ref = ctypes.byref(self._c)
 
     def _check_pages(self, page_size: int) -> None:
@@ -164,8 +171,10 @@ class AttentionConfig:
     def __init__(self, num_heads: int, num_kv_heads: int, head_dim: int,
                  scale: Optional[float] = None, causal: bool = True, window: int = 0,
                  softcap: float = 0.0):
-        self.num_heads, self.num_kv_heads, self.head_dim = num_heads, num_kv_heads, head_dim
-        self._c = _lib.AttnDesc(num_heads, num_kv_heads, head_dim, int(causal), int(window),
+        self.num_heads, self.num_kv_heads = _int32(num_heads, "num_heads"), _int32(num_kv_heads, "num_kv_heads")
+        self.head_dim = _int32(head_dim, "head_dim")
+        self._c = _lib.AttnDesc(self.num_heads, self.num_kv_heads, self.head_dim, int(bool(causal)),
+                                _int32(window, "window"),
                                 1.0 / math.sqrt(head_dim) if scale is None else scale, softcap)
         self._ref = ctypes.byref(self._c)
 

@@ -56,10 +56,10 @@ def norm_residual(x: torch.Tensor, residual: Optional[torch.Tensor] = None,
     `residual_out` may be `residual` (update in place)."""
     L = _lib.load()
     shape, dev = x.shape, x.get_device()
+    if len(shape) != 2 or shape[1] > 32768:
+        raise ValueError("x must be [rows, hidden], hidden at most 32768")
     if dev < 0:
         raise ValueError("x must be a CUDA tensor (there is no CPU path)")
-    if len(shape) != 2:
-        raise ValueError("x must be [rows, hidden]")
     rows, hidden = shape
     xs = _rows(x, "x", shape, dev)
     rs = 0 if residual is None else _rows(residual, "residual", shape, dev)

@@ -132,3 +132,34 @@ def test_norm_outputs_that_overlap_are_refused():
                dict(gate=far, ro=(far[0] + 128, 64)), dict(gate=(far[0], 0), ro=far), dict(gate=(far[0] + 2, 64), ro=far, gc=0),
                dict(ro=far, y=(far[0] + 128, 64)), dict(ro=far, rd=0, y=(far[0] + 64, 64))):
         assert "overlap" in norm_word(8, 64, (A, 64), **kw), kw
+
+
+@pytest.mark.parametrize("name", ["num_heads", "num_kv_heads", "head_dim", "window"])
+@pytest.mark.parametrize("by", [2 ** 31, 2 ** 32, -2 ** 32])
+def test_whole_numbers_that_do_not_fit_are_refused(name, by):
+    """ctypes would pass on their low 32 bits, which may be an ordinary number."""
+    import nvfp4
+
+    good = dict(num_heads=8, num_kv_heads=2, head_dim=128, window=16)
+    nvfp4.AttentionConfig(**good)
+    with pytest.raises(ValueError, match=name):
+        nvfp4.AttentionConfig(**{**good, name: good[name] + by})
+
+
+def test_lengths_that_do_not_fit_are_refused(on_cpu):
+    i = lambda *x: torch.tensor(x, dtype=torch.int32)
+    make = lambda **kw: on_cpu.AttentionBatch(i(9, 9), torch.zeros(2, 4, dtype=torch.int32), q_start=i(0, 4, 9),
+                                              num_tokens=9, **kw)
+    make(max_q_len=5, prefix_len=3, prefix_pages=i(1))
+    with pytest.raises(ValueError, match="max_q_len"):
+        make(max_q_len=2 ** 32 + 5)
+    with pytest.raises(ValueError, match="prefix_len"):
+        make(max_q_len=5, prefix_len=2 ** 32 + 3, prefix_pages=i(1))
+
+
+def test_norm_rows_that_do_not_fit_are_refused():
+    import nvfp4
+
+    for hidden in (32769, 2 ** 32 + 8):
+        with pytest.raises(ValueError, match="hidden"):
+            nvfp4.norm_residual(torch.empty(1, hidden, dtype=torch.bfloat16, device="meta"))
