@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 3) kv_append_kernel(AppendA
 
   // The token's sequence: token t itself in a step of single tokens (checked
   // first), else by bisection of q_start.
-  int b = (int)t, qs = (int)t, qe = (int)t + 1;
+  int b = (int)t, qe = (int)t + 1;
   if (a.b.q_start) {
     const int B = a.b.num_seqs;
     b = min(b, B - 1);
@@ -197,8 +197,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 3) kv_append_kernel(AppendA
       b = lo;
       if (b >= B || a.b.q_start[b] > t) return;  // in no sequence
     }
-    qs = a.b.q_start[b];
-    qe = a.b.q_start[b + 1];
+    qe = min(a.b.q_start[b + 1], (int)a.b.num_tokens);
   }
   const int64_t key = (int64_t)a.b.kv_len[b] - qe + t;  // own key index
   const int64_t at = key >> a.page_shift;

@@ -136,3 +136,24 @@ def test_windows_as_long_as_the_type(causal, window):
     run_and_check(make(8, [3, 40], [7, 2], width=4), causal=causal, window=window)
     run_and_check(make(93, [30, 9], [200, 9], 1, 128, 8, 16), causal=causal, window=window)
     run_and_check(make(94, [3, 0, 40], [70, 1, 2], 2, 64, 8, 16, prefix=20), causal=causal, window=window)
+
+
+@pytest.mark.parametrize("last", [8, 9, I32_MAX])
+def test_append_holds_token_ranges_to_the_calls_rows(last):
+    """Tokens beyond the call's rows do not exist: those that do are the last
+    ones of their sequence's keys, for the append as for the attention."""
+    import nvfp4
+
+    s = make(95, [12, 20], [3, 4], 2, 128, 4, 16, poison=False)
+    x = torch.randn(7, 8, 128, generator=s["g"]).to(torch.bfloat16).cuda()
+    q, k, v = x.split([4, 2, 2], 1)
+    starts = s["q_start"].clone()
+    starts[2] = last
+    b = nvfp4.AttentionBatch(s["kv_len"].cuda(), s["table"].cuda(), q_start=starts.cuda(), num_tokens=7, max_q_len=4)
+    want = [c.clone() for c in (s["cache"].k, s["cache"].v)]
+    for c, rows in zip(want, (k, v)):
+        for t, (seq, key) in enumerate([(0, 9), (0, 10), (0, 11), (1, 16), (1, 17), (1, 18), (1, 19)]):
+            c[s["table"][seq, key // 16], key % 16] = rows[t]
+    got = nvfp4.kv_append(q, k, v, s["cache"], b)
+    assert torch.equal(got, q)
+    assert torch.equal(s["cache"].k, want[0]) and torch.equal(s["cache"].v, want[1])
