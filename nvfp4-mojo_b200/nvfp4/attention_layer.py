@@ -43,7 +43,8 @@ class AttentionWeights:
     def from_layer(cls, layer, q_norm=None, k_norm=None, stream=None) -> "AttentionWeights":
         """From a layer of `load_qwen35_layer`: q, k and v stacked into one
         matrix (one launch instead of three), each one's input_scale folded
-        into its rows' weight_scale_2 (the product is the same)."""
+        into its rows' weight_scale_2 (the product is the same).  q_norm and
+        k_norm None: the layer's own, where it has them."""
         parts = (layer.q_proj, layer.k_proj, layer.v_proj)
         device = parts[0].packed_weights.device
         w = stack_rows([p.packed_weights for p in parts], stream=stream)
@@ -51,6 +52,8 @@ class AttentionWeights:
         rows = [_row_scales(p.weight_scale_2 if p.weight_scale_2_rows is None else p.weight_scale_2_rows,
                             p.out_features, p.input_scale).to(device) for p in parts]
         lin = NvFp4Linear(parts[0].in_features, w.shape[0], weight_scale_2_rows=torch.cat(rows))
+        q_norm, k_norm = (getattr(layer, n, None) if w is None else w
+                          for n, w in (("q_norm", q_norm), ("k_norm", k_norm)))
         o = layer.o_proj
         vec = lambda x: None if x is None else _bf16_vector(x, device)
         return cls((lin, w, sf), (o.to_linear(), o.packed_weights, o.blockscales),

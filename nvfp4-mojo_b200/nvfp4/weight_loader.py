@@ -245,6 +245,18 @@ def _find_load_raw(shards, name: str) -> np.ndarray:
     return model.shards[s].read_tensor_bytes(i)
 
 
+def _find_load_vector(shards, name: str) -> Optional[torch.Tensor]:
+    """A host tensor of the first shard holding name; None where none does."""
+    for shard in _model_of(shards).shards:
+        i = shard.find_tensor(name)
+        if i >= 0:
+            dtype = {"BF16": torch.bfloat16, "F16": torch.float16, "F32": torch.float32}.get(shard.tensors[i].dtype)
+            if dtype is None:
+                raise ValueError(f"{name}: {shard.tensors[i].dtype} is not a float type")
+            return torch.from_numpy(shard.read_tensor_bytes(i)).view(dtype)
+    return None
+
+
 def load_moe_experts(model, layer, num_experts: Optional[int] = None, first: int = 0,
                      shared: bool = False, router: bool = True, device="cuda", stream=None):
     """Experts [first, first + num_experts) of a layer as stacked nvfp4.moe
@@ -298,7 +310,9 @@ class Qwen35LayerWeights:
     """struct Qwen35LayerWeights (nvfp4/weight_loader.mojo:776-825) on the
     device: attention projections as LoadedWeight, the routed experts and
     the shared expert as stacked MoEWeights, the router as fp32 [H, E] (in
-    the routed MoEWeights), the layer norms as raw host bytes."""
+    the routed MoEWeights), the layer norms as raw host bytes; q_norm and
+    k_norm, the norms of the query and key heads, as host tensors where the
+    checkpoint has them (the reference does not load them)."""
 
     q_proj: LoadedWeight
     k_proj: LoadedWeight
@@ -309,6 +323,8 @@ class Qwen35LayerWeights:
     input_layernorm: np.ndarray
     post_attn_layernorm: np.ndarray
     extra: Dict[str, object] = field(default_factory=dict)
+    q_norm: Optional[torch.Tensor] = None
+    k_norm: Optional[torch.Tensor] = None
 
 
 def load_qwen35_layer(shards, layer_idx: int, num_experts: int) -> Qwen35LayerWeights:
@@ -323,4 +339,6 @@ def load_qwen35_layer(shards, layer_idx: int, num_experts: int) -> Qwen35LayerWe
     return Qwen35LayerWeights(att["q_proj"], att["k_proj"], att["v_proj"], att["o_proj"],
                               experts, shared,
                               _find_load_raw(model, f"{lp}.input_layernorm.weight"),
-                              _find_load_raw(model, f"{lp}.post_attention_layernorm.weight"))
+                              _find_load_raw(model, f"{lp}.post_attention_layernorm.weight"),
+                              q_norm=_find_load_vector(model, f"{lp}.self_attn.q_norm.weight"),
+                              k_norm=_find_load_vector(model, f"{lp}.self_attn.k_norm.weight"))
