@@ -45,10 +45,29 @@ class AttentionWeights:
         matrix (one launch instead of three), each one's input_scale folded
         into its rows' weight_scale_2 (the product is the same).  q_norm and
         k_norm None: the layer's own, where it has them."""
+        device = layer.q_proj.packed_weights.device
+        with torch.cuda.device(device):
+            here = torch.cuda.current_stream()
+            if stream is None:
+                stream = here
+            elif not isinstance(stream, torch.cuda.Stream):
+                stream = torch.cuda.ExternalStream(int(stream), device=device)
+            # Everything is made on `stream`, after what the caller has under way,
+            # and before what comes on the caller's own stream, where the layer runs.
+            stream.wait_stream(here)
+            with torch.cuda.stream(stream):
+                w = cls._stack(layer, device, q_norm, k_norm)
+            here.wait_stream(stream)
+            for t in (w.in_proj[0].weight_scale_2_rows, *w.in_proj[1:], w.input_norm, w.post_norm, w.q_norm, w.k_norm):
+                if t is not None:
+                    t.record_stream(here)
+        return w
+
+    @classmethod
+    def _stack(cls, layer, device, q_norm, k_norm) -> "AttentionWeights":
         parts = (layer.q_proj, layer.k_proj, layer.v_proj)
-        device = parts[0].packed_weights.device
-        w = stack_rows([p.packed_weights for p in parts], stream=stream)
-        sf = stack_rows([_u8(p.blockscales) for p in parts], stream=stream)
+        w = stack_rows([p.packed_weights for p in parts])
+        sf = stack_rows([_u8(p.blockscales) for p in parts])
         rows = [_row_scales(p.weight_scale_2 if p.weight_scale_2_rows is None else p.weight_scale_2_rows,
                             p.out_features, p.input_scale).to(device) for p in parts]
         lin = NvFp4Linear(parts[0].in_features, w.shape[0], weight_scale_2_rows=torch.cat(rows))

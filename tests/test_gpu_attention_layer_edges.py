@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import st_fixtures as F
-from test_gpu_attention_layer import build, close, reference
+from test_gpu_attention_layer import build, close, loaded, reference
 from test_gpu_loader import moe_checkpoint
 from nvfp4.weight_loader import SafetensorsModel
 
@@ -46,3 +46,39 @@ def test_the_heads_norms_of_a_loaded_layer_are_used(tmp_path, normed):
     assert torch.equal(weights.q_norm.cpu(), qn) and torch.equal(weights.k_norm.cpu(), kn.to(torch.bfloat16))
     other = nvfp4.AttentionWeights.from_layer(layer, k_norm=qn)  # the caller's come first
     assert torch.equal(other.q_norm.cpu(), qn) and torch.equal(other.k_norm.cpu(), qn)
+
+
+def test_weights_stacked_on_another_stream_are_ready(O):
+    """from_layer on a stream that is busy: what the caller's stream reads next
+    is the stacked weights, and nothing that it still uses is overwritten."""
+    import nvfp4
+
+    H, KV, D, d_model = 8, 2, 128, 512
+    layer, m = {}, {}
+    rng = np.random.default_rng(41)
+    for p, (n, k) in {"q_proj": (H * D, d_model), "k_proj": (KV * D, d_model), "v_proj": (KV * D, d_model),
+                      "o_proj": (d_model, H * D)}.items():
+        layer[p], m[p] = loaded(O, rng, n, k, p != "k_proj")
+    one = torch.ones(d_model, dtype=torch.bfloat16).view(torch.uint8).numpy()
+    layer = SimpleNamespace(**layer, input_layernorm=one, post_attn_layernorm=one, q_norm=torch.full((D,), 2.0),
+                            k_norm=None)
+    parts = lambda w: (*w.in_proj[1:], w.in_proj[0].weight_scale_2_rows, w.q_norm, w.input_norm)
+    want = [t.cpu() for t in parts(nvfp4.AttentionWeights.from_layer(layer))]
+    assert torch.equal(want[0], torch.cat([p.packed_weights.cpu() for p in (layer.q_proj, layer.k_proj, layer.v_proj)]))
+    for side in (torch.cuda.Stream(), torch.cuda.Stream()):
+        for stream in (side, side.cuda_stream):
+            source = torch.arange(want[0].numel(), device="cuda") % 251
+            torch.cuda.synchronize()
+            spare = torch.empty_like(source, dtype=torch.uint8)
+            torch.cuda._sleep(20_000_000)  # the caller's stream is busy,
+            spare.copy_(source)
+            kept = spare.clone()           # with memory of the weights' size
+            del spare
+            with torch.cuda.stream(side):
+                torch.cuda._sleep(20_000_000)  # and so is the other one
+            weights = nvfp4.AttentionWeights.from_layer(layer, stream=stream)
+            got = [t.clone() for t in parts(weights)]
+            torch.cuda.synchronize()
+            for a, b in zip(got, want):
+                assert torch.equal(a.cpu(), b)
+            assert torch.equal(kept.cpu(), source.cpu().to(torch.uint8))
