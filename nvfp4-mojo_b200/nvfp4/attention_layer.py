@@ -99,7 +99,8 @@ class AttentionLayer:
     def attention(self, h: torch.Tensor, cache: PagedKVCache, batch: AttentionBatch,
                   positions: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
         """h bf16 [T, d_model], normed -> o_proj(attention) bf16 [T, d_model];
-        this step's keys and values go into the cache."""
+        this step's keys and values go into the cache.  Rows in no sequence
+        (a padded batch) have an attention of 0."""
         c = self.config
         H, KV, D, T = c.num_heads, c.num_kv_heads, c.head_dim, h.shape[0]
         x = nvfp4_linear(*self.w.in_proj, h)
@@ -109,8 +110,10 @@ class AttentionLayer:
         if self.gated:
             heads = x[:, :nq * D].view(T, H, 2, D)
             q, gate = heads[:, :, 0], heads[:, :, 1]
+        # (Append and attention leave rows in no sequence as they are.)
+        q_out = None if batch.tensors[2] is None else torch.zeros(T, H, D, dtype=torch.bfloat16, device=x.device)
         q = kv_append(q, k, v, cache, batch, rotary=self.rotary, positions=positions, q_norm=self.w.q_norm,
-                      k_norm=self.w.k_norm, norm_eps=self.eps, norm_offset=self.offset)
+                      k_norm=self.w.k_norm, norm_eps=self.eps, norm_offset=self.offset, q_out=q_out)
         a = paged_attention(q, cache, batch, c, gate=gate, out=q, workspace=workspace)
         return nvfp4_linear(*self.w.out, a.view(T, H * D))
 

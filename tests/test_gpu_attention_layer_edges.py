@@ -15,6 +15,35 @@ from nvfp4.weight_loader import SafetensorsModel
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize("D,gated,res", [(128, False, torch.bfloat16), (256, True, torch.float32)])
+def test_rows_in_no_sequence_get_no_attention(O, D, gated, res):
+    """A batch padded behind its last sequence: its rows' residual is what it
+    would be without the layer, whatever the memory held before."""
+    import nvfp4
+
+    H, KV, d_model, lens, pad = 4, 1, 512, [20, 33], 11
+    att, m = build(O, 17, H, KV, D, d_model, gated, 64)
+    g = torch.Generator().manual_seed(5)
+    T = sum(lens)
+    cache = nvfp4.PagedKVCache.empty(8, 16, KV, D)
+    cache.k.fill_(math.nan)
+    cache.v.fill_(math.nan)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    batch = nvfp4.AttentionBatch(i32(lens), i32([[5, 2, 0], [1, 7, 3]]), q_start=i32([0, lens[0], T]),
+                                 num_tokens=T + pad, max_q_len=max(lens))
+    x = torch.randn(T + pad, d_model, generator=g).to(res)
+    ws = nvfp4.attention_workspace(att.config, batch)
+    for _ in range(2):
+        spoilt = torch.full((T + pad, H, D), math.nan, dtype=torch.bfloat16, device="cuda")
+        del spoilt  # its memory is the next of that size
+        r, y = att.step(None, x.cuda(), cache, batch, workspace=ws)
+        assert torch.equal(r[T:].cpu(), x[T:]) and torch.isfinite(y[T:]).all()
+        past = [[torch.zeros(0, KV, D, dtype=torch.float64) for _ in range(2)] for _ in lens]
+        want = [reference(m, z, p) for z, p in zip(x[:T].double().split(lens), past)]
+        close(r[:T], torch.cat([w[0] for w in want]))
+        close(y[:T], torch.cat([w[1] for w in want]))
+
+
 @pytest.mark.parametrize("normed", [True, False])
 def test_the_heads_norms_of_a_loaded_layer_are_used(tmp_path, normed):
     """self_attn.q_norm and k_norm of a checkpoint that has them reach the
