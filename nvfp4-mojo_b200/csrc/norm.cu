@@ -200,11 +200,12 @@ cudaError_t launch_norm_as(const NormArgs &a, int nt, cudaStream_t st) {
 
 template <int VPT, bool VEC>
 cudaError_t launch_norm_vpt(const NormArgs &a, int nt, cudaStream_t st) {
-  if constexpr (VPT == 4) return launch_norm_as<VPT, VEC, 1024>(a, nt, st);  // rows beyond 16384
-  if (nt <= 32) return launch_norm_as<VPT, VEC, 256>(a, nt, st);
-  if (nt <= 128) return launch_norm_as<VPT, VEC, 128>(a, nt, st);
-  if (nt <= 256) return launch_norm_as<VPT, VEC, 256>(a, nt, st);
-  if (nt <= 512) return launch_norm_as<VPT, VEC, 512>(a, nt, st);
+  if constexpr (VPT < 4) {  // (four: rows beyond 16384)
+    if (nt <= 32) return launch_norm_as<VPT, VEC, 256>(a, nt, st);
+    if (nt <= 128) return launch_norm_as<VPT, VEC, 128>(a, nt, st);
+    if (nt <= 256) return launch_norm_as<VPT, VEC, 256>(a, nt, st);
+    if (nt <= 512) return launch_norm_as<VPT, VEC, 512>(a, nt, st);
+  }
   return launch_norm_as<VPT, VEC, 1024>(a, nt, st);
 }
 
