@@ -46,7 +46,7 @@ static bool make_cache_map(CUtensorMap *m, void *base, const int64_t (&st)[3], c
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-static int attn_sms() {
+int attn_sms() {
   static std::atomic<int> count[64];  // per device
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;

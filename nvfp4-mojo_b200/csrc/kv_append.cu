@@ -362,7 +362,7 @@ cudaError_t launch_append(AppendArgs &a, bool vec, cudaStream_t st) {
   // every SM; fewer tokens are split over up to one warp per step of rows.
   // (400 tokens of 32 + 2 x 4 heads of 128: 7.9 us for 4 warps, 6.2 for 16, 7.9 for
   // 48; 1500 tokens 14.1, 10.3, 14.1; 64 tokens 4.2, 4.5, 4.5.)
-  const int64_t want = 148 * 16;
+  const int64_t want = (int64_t)attn_sms() * 16;
   int64_t chunks = a.b.num_tokens >= want ? 1 : (want + a.b.num_tokens - 1) / a.b.num_tokens;
   if (chunks > steps) chunks = steps;
   a.chunk_steps = (int)((steps + chunks - 1) / chunks);
