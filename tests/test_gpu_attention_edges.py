@@ -157,3 +157,48 @@ def test_append_holds_token_ranges_to_the_calls_rows(last):
     got = nvfp4.kv_append(q, k, v, s["cache"], b)
     assert torch.equal(got, q)
     assert torch.equal(s["cache"].k, want[0]) and torch.equal(s["cache"].v, want[1])
+
+
+LONG = [([2300, 1, 149], [0, 40, 17]), ([2500], [3])]
+
+
+@pytest.mark.parametrize("H,KV,D", [(32, 6, 64), (14, 3, 128), (7, 2, 256), (11, 3, 136)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("form", ["halves", "interleaved", "by element", "plain"])
+def test_append_of_long_prompts(H, KV, D, dtype, form):
+    """A warp takes a whole token: every ring slot is filled more than twice, and
+    the heads' kind changes inside the ring."""
+    rotary = {"halves": D // 2 if D % 16 == 0 else 64, "interleaved": D, "by element": 12, "plain": 0}[form]
+    for i, (qlens, ctx) in enumerate(LONG):
+        append_case(96 + i, qlens, ctx, H, KV, D, 32, rotary, 3 if i else 1, form == "interleaved", form != "plain",
+                    dtype)
+
+
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_append_of_long_prompts_in_place_and_off_alignment(inter, dtype):
+    """q_out over q, and rows that start off 16 bytes, against packed rows."""
+    import nvfp4
+
+    H, KV, D, T = 14, 3, 128, 2400
+    s = make(98, [T + 5], [T], KV, D, H, 32, poison=False)
+    x = torch.randn(T, H + 2 * KV, D, generator=s["g"]).to(dtype).cuda()
+    rot = nvfp4.Rotary(torch.rand(32, generator=s["g"]).cuda(), interleaved=inter)
+    w = (1 + 0.2 * torch.randn(D, generator=s["g"])).to(torch.bfloat16).cuda()
+
+    def run(x, **kw):
+        q, k, v = x.split([H, KV, KV], 1)
+        s["cache"].k.zero_(), s["cache"].v.zero_()
+        got = nvfp4.kv_append(q, k, v, s["cache"], batch_of(s), rotary=rot, q_norm=w, k_norm=w,
+                              **{n: q for n in kw})
+        return got.clone(), s["cache"].k.clone(), s["cache"].v.clone()
+
+    want = run(x)
+    odd = torch.empty(T, H + 2 * KV, D + 1, dtype=dtype, device="cuda")[..., 1:]
+    odd.copy_(x)
+    for a, b in zip(run(odd), want):
+        # Each within half a step of the exact value, and its fp32 error.
+        assert ((a.double() - b.double()).abs() <= 2 * ref.BF16 * b.double().abs() + 2.0 ** -18 * 8).all()
+    if dtype is torch.bfloat16:
+        for a, b in zip(run(x, q_out=1), want):
+            assert torch.equal(a, b)
