@@ -202,3 +202,33 @@ def test_append_of_long_prompts_in_place_and_off_alignment(inter, dtype):
     if dtype is torch.bfloat16:
         for a, b in zip(run(x, q_out=1), want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows", [591, 592, 2003])
+@pytest.mark.parametrize("hidden", [8, 100, 264, 512, 520, 1024, 2048, 5000])
+@pytest.mark.parametrize("x_dtype,r_dtype,post,gate,act", [
+    (torch.bfloat16, torch.bfloat16, False, None, "sigmoid"), (torch.bfloat16, torch.float32, True, "token", "sigmoid"),
+    (torch.float32, torch.float32, True, "full", "linear"), (torch.bfloat16, torch.float32, False, "channel", "sigmoid")])
+def test_norm_of_many_rows(rows, hidden, x_dtype, r_dtype, post, gate, act):
+    norm_case(rows, hidden, x_dtype, r_dtype, post, gate, act)
+
+
+@pytest.mark.parametrize("rows,hidden", [(600, 8192), (593, 16384), (593, 9000), (40, 32768)])
+def test_norm_of_many_long_rows(rows, hidden):
+    norm_case(rows, hidden, torch.bfloat16, torch.float32, True, "full", "sigmoid")
+
+
+@pytest.mark.parametrize("rows,hidden", [(593, 8), (593, 512), (700, 520), (700, 2048), (600, 8200)])
+def test_norm_of_many_rows_off_alignment(rows, hidden):
+    import nvfp4
+
+    g = torch.Generator().manual_seed(hidden)
+    n = lambda *s: torch.randn(*s, generator=g).to(torch.bfloat16).cuda()
+    w, p, gate = n(hidden), n(hidden), n(rows, 1)
+    odd, res = n(rows, hidden + 1)[:, 1:], n(rows, hidden + 3)[:, 3:]
+    got = nvfp4.norm_residual(odd, res, pre_weight=w, post_weight=p, gate=gate)
+    r, y = nvfp4.norm_residual(odd.contiguous(), res.contiguous(), pre_weight=w, post_weight=p, gate=gate)
+    for a, b, scale in ((got[0], r, 1.0), (got[1], y, 1.0)):
+        # The sums' order differs: both within half a step and 48 fp32 roundings of the exact value.
+        tol = 2 * (ref.BF16 + 48 * ref.F32) * b.double().abs() + 2 * 48 * ref.F32 * b.double().abs().amax(1, keepdim=True)
+        assert ((a.double() - b.double()).abs() <= tol).all()
