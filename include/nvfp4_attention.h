@@ -100,8 +100,8 @@ typedef struct nvfp4_qk_norm {
  * itself), k normed and rotated into the cache, v into the cache.  q, k, v
  * are rows of in_dtype (bf16 or f32), q_out and the cache bf16; other overlaps
  * of q_out's rows, with each other or with q, k and v, are refused.  positions
- * [num_axes, num_tokens] with row stride position_stride, or NULL: the
- * token's position on every axis.  rotary or norm NULL: none.  The angle is
+ * [num_axes, num_tokens] with row stride position_stride (0: one row for all
+ * axes), or NULL: the token's position on every axis.  rotary or norm NULL: none.  The angle is
  * exact to fp32 for every int32 position.  A token whose key lies outside the
  * page table, or in a page outside the cache, gets its q_out but no key.  A
  * token outside every sequence leaves cache and q_out as they were.

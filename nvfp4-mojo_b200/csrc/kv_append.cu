@@ -404,7 +404,8 @@ extern "C" int nvfp4_kv_append(const nvfp4_kv_cache *cache, const nvfp4_attentio
   const int R = rotary ? rotary->rotary_dim : 0;
   if (rotary && (R <= 0 || R % 2 || R > cache->head_dim || !rotary->inv_freq))
     return fail(NVFP4_ERR_INVALID_ARG, "rotary_dim %d: even, 2 .. head_dim, with inv_freq", R);
-  if (positions && (num_axes < 1 || (num_axes > 1 && position_stride < batch->num_tokens)))
+  if (positions &&
+      (num_axes < 1 || (num_axes > 1 && position_stride != 0 && position_stride < batch->num_tokens)))
     return fail(NVFP4_ERR_INVALID_ARG, "positions need num_axes >= 1 rows of num_tokens");
   if (norm && !(norm->eps >= 0.0f)) return fail(NVFP4_ERR_INVALID_ARG, "eps must not be negative");
   if (batch->num_tokens == 0 || batch->num_seqs == 0) return NVFP4_OK;

@@ -219,8 +219,8 @@ def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: PagedKVC
     q [T, num_heads, D], k and v [T, num_kv_heads, D]: bf16 or fp32, any token
     and head strides (slices of one projection).  q and k are RMS-normed per
     head where q_norm / k_norm (bf16 [D]) are given, then rotated.  positions
-    int32 [T] or [axes, T] (None: the token's place in its sequence).  q_out
-    bf16 [T, num_heads, D]; it may be q."""
+    int32 [T] or [axes, T] (one row expanded where the axes agree; None: the
+    token's place in its sequence).  q_out bf16 [T, num_heads, D]; it may be q."""
     L = _lib.load()
     T, D = batch.num_tokens, cache.head_dim
     dtype = q.dtype
@@ -249,8 +249,8 @@ def kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: PagedKVC
             raise ValueError("positions must be on the tensors' device")
         pos = positions.data_ptr()
         if positions.dim() == 2:
-            axes, stride = positions.shape[0], max(positions.stride(0), T)
-            if axes > 1 and positions.stride(0) < T:
+            axes, stride = positions.shape[0], positions.stride(0)
+            if axes > 1 and 0 < stride < T:
                 raise ValueError("positions must not overlap from axis to axis")
     norm = None
     if q_norm is not None or k_norm is not None:

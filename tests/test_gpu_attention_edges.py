@@ -159,6 +159,25 @@ def test_append_holds_token_ranges_to_the_calls_rows(last):
     assert torch.equal(s["cache"].k, want[0]) and torch.equal(s["cache"].v, want[1])
 
 
+def test_one_row_of_positions_for_all_axes():
+    """Text under a rotation by time, height and width: [T] expanded to the axes."""
+    import nvfp4
+
+    s = make(88, [40, 9], [30, 9], 2, 128, 4, 16, poison=False)
+    T = s["T"]
+    q, k, v = torch.randn(T, 8, 128, generator=s["g"]).to(torch.bfloat16).cuda().split([4, 2, 2], 1)
+    pos = torch.randint(0, 5000, (T,), generator=s["g"], dtype=torch.int32).cuda()
+    rot = nvfp4.Rotary(torch.rand(64, generator=s["g"]).cuda(), axes=(torch.arange(64) % 3).to(torch.int32).cuda())
+    got = []
+    for positions in (pos.expand(3, -1), pos.repeat(3, 1)):
+        turned = nvfp4.kv_append(q, k, v, s["cache"], batch_of(s), rotary=rot, positions=positions)
+        got.append((turned, s["cache"].k.clone()))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    with pytest.raises(ValueError, match="overlap"):
+        nvfp4.kv_append(q, k, v, s["cache"], batch_of(s), rotary=rot,
+                        positions=torch.zeros(T + 4, dtype=torch.int32, device="cuda").as_strided((3, T), (2, 1)))
+
+
 LONG = [([2300, 1, 149], [0, 40, 17]), ([2500], [3])]
 
 
