@@ -40,6 +40,24 @@ def test_one_page_table_row_for_all_sequences(qlens):
     assert not (got[0][1] == 0.5).all()
 
 
+@pytest.mark.parametrize("H,KV,D", [(8, 2, 128), (8, 1, 256), (4, 4, 64)])
+@pytest.mark.parametrize("prefix", [0, 70])
+def test_out_over_the_gate(H, KV, D, prefix):
+    """Each value of the gate is read before the output takes its place: in the
+    item's own end, in the join of cut items and behind a prefix."""
+    import nvfp4
+
+    for lens, qlens in (([9000, 3, 40], [1, 1, 1]), ([3000, 300, 70], [260, 300, 1])):
+        s = make(87, lens, qlens, KV, D, H, 16, prefix=prefix)
+        gate = torch.randn(s["T"], H, D, generator=s["g"]).to(torch.bfloat16).cuda()
+        cfg, b, q = nvfp4.AttentionConfig(H, KV, D), batch_of(s), s["q"].cuda()
+        want = nvfp4.paged_attention(q, s["cache"], b, cfg, gate=gate)
+        got = nvfp4.paged_attention(q, s["cache"], b, cfg, gate=gate, out=gate)
+        assert got.data_ptr() == gate.data_ptr() and torch.equal(got, want)
+        in_place = nvfp4.paged_attention(q, s["cache"], b, cfg, gate=want.clone(), out=q)
+        assert in_place.data_ptr() == q.data_ptr() and torch.isfinite(in_place).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rotary,inter", [(0, False), (64, False), (64, True), (6, False), (128, False)])
 @pytest.mark.parametrize("norm", [False, True])
