@@ -119,6 +119,34 @@ def test_caps_of_every_size(cap, D, tokens):
     ref.check(lse, want, ref.F32 * ((D + 4) * size + 20 * want.abs()), "lse")
 
 
+@pytest.mark.parametrize("qlens", [[1, 1, 1], [3, 60, 200]])
+@pytest.mark.parametrize("D,H,KV", [(128, 8, 2), (256, 8, 1), (64, 8, 2)])
+def test_capped_scores_that_are_not_finite(qlens, D, H, KV):
+    """A cap holds an infinite score and keeps one that is not a number."""
+    import nvfp4
+
+    s = make(86, [q + 70 for q in qlens], qlens, KV, D, H, 16)
+    bad, big = s["q"].clone(), s["q"].clone()
+    bad[1, 2, 5] = math.nan
+    # Scores beyond fp32: one column of q and of every key decides their sign.
+    big[0, 4] = 0
+    big[0, 4, 1] = 3e38
+    k = s["cache"].k.clone()
+    used = torch.isfinite(k).all(-1)
+    k[..., 1] = torch.where(used, torch.where(k[..., 1] > 0, 2.0, -2.0).to(torch.bfloat16), k[..., 1])
+    cache = nvfp4.PagedKVCache(k, s["cache"].v)
+    cfg = nvfp4.AttentionConfig(H, KV, D, scale=1.0, softcap=4.0)
+    b = batch_of(s)
+    out = nvfp4.paged_attention(bad.cuda(), s["cache"], b, nvfp4.AttentionConfig(H, KV, D, softcap=4.0))
+    assert torch.isnan(out[1, 2]).all()
+    out[1, 2] = 0
+    assert torch.isfinite(out).all()
+    out, lse = nvfp4.paged_attention(big.cuda(), cache, b, cfg, return_lse=True)
+    big[0, 4, 1] = 1e6  # far beyond the cap, within fp32: the same capped scores
+    want, want_lse = nvfp4.paged_attention(big.cuda(), cache, b, cfg, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse) and torch.isfinite(lse).all()
+
+
 @pytest.mark.parametrize("n", [2 ** 24 + 2, 2 ** 25 + 77])
 @pytest.mark.parametrize("tokens", [1, 4, 70])
 @pytest.mark.parametrize("D", [64, 128])
