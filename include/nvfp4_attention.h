@@ -8,8 +8,11 @@
  *
  * Conventions as in nvfp4.h: device pointers owned by the caller, 0 or a
  * negative nvfp4_status, work enqueued on `stream`.  Data is bf16 unless a
- * comment says otherwise; sums, softmax statistics and partial results are
- * fp32.  Lengths, page tables and positions are int32 in device memory, so
+ * comment says otherwise; scores, softmax statistics, sums and partial results
+ * are fp32.  The softmax's weights are rounded to bf16 for their product with
+ * the values (the sum keeps them unrounded), which moves an output by at most
+ * 2^-8 of the weighted mean of its |values|; exponentials and the gate's sigmoid
+ * are within a few units of 2^-22.  Lengths, page tables and positions are int32 in device memory, so
  * that a captured graph can be replayed with new ones.  Device values that
  * contradict the descriptors are clamped, never followed out of range: a page
  * id outside [0, num_pages) reads as zeros and is not written, a length is
@@ -72,7 +75,8 @@ typedef struct nvfp4_attention_batch {
   int32_t prefix_len;           /* 0: none */
   const int32_t *prefix_pages;  /* [ceil(prefix_len / page_size)] */
   const int32_t *visible_len;   /* [num_seqs] or NULL: the first visible_len[b]
-                                   positions are seen by every query of b */
+                                   positions are seen by every query of b (that
+                                   a window lets see so far back) */
 } nvfp4_attention_batch;
 
 /* Rotation of the first rotary_dim values of a head in pairs (i, i +

@@ -22,8 +22,8 @@
 // size 256, where a tile's softmax is the one in flight; 572 against 570 us for a
 // prompt of 8192 at 32 / 4 heads of 128.)
 //
-// What bounds it: that prompt runs at 970 TFLOP/s and 990 W, where the power
-// limit takes the clock from 1965 to 1680 MHz.  Per pair of query tiles and key
+// What bounds it: that prompt takes 548 to 574 us, 960 to 1000 TFLOP/s, at 990 W,
+// where the power limit takes the clock from 1965 to 1680 MHz.  Per pair of query tiles and key
 // tile it takes 1950 cycles: the exponentials 1024 of the MUFU, in a phase of
 // all warps that nothing else fills, and the products 1050 of the tensor cores.
 // Exponentials on the FMA pipe in part (a polynomial of degree 4) give 587 to
@@ -57,8 +57,11 @@ constexpr int HK = KT / 2;    // of them a softmax thread's
 // Of an item's beginning and end, in key tiles, which two query tiles with capped
 // or biased scores take longer for.  (A prompt of 8192, 32 / 4 heads of 128: 618 us
 // with 2, 569 with 5, 569 with 8.  Four ragged ones at head size 256: 245 with 2,
-// 235 with 5, 236 with 8.  Three with cap and bias, 28 / 4 heads of 128: 150 with 1,
-// 147 with 2, 148 with 3, 153 with 5.)
+// 235 with 5, 236 with 8.  Capped or biased, with 2, 3 and 5: three prompts of 28 / 4
+// heads of 128 146, 147 and 153 us, without bias and window 137, 135 and 142, of 8 / 8
+// heads of 64 64, 66 and 69, the prompt of 8192 942, 946 and 960, the four with bias at
+// head size 128 298, 290 and 285; at head size 256 the three 123, 123 and 126, the
+// four 268, 262 and 258.)
 template <int DP, bool MOD>
 constexpr int kItemCost = MOD && DP <= 128 ? 2 : 5;
 

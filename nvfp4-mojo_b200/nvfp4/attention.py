@@ -115,7 +115,8 @@ class AttentionBatch:
     the call (None: one token per sequence), at most max_q_len each, num_tokens
     in all.  prefix_pages int32 and prefix_len: a prefix that every sequence
     shares and kv_len does not count.  visible_len int32 [B]: positions below
-    it are seen by every query of the sequence, later ones or not.
+    it are seen by every query of the sequence, also by those before them (but
+    no further back than a window reaches).
 
     Lengths and tables stay on the device and are read when the call runs, so
     a captured call can be replayed after they were rewritten in place."""
