@@ -109,7 +109,8 @@ typedef struct nvfp4_qk_norm {
  * exact to fp32 for every int32 position.  A token whose key lies outside the
  * page table, or in a page outside the cache, gets its q_out but no key.  A
  * token outside every sequence leaves cache and q_out as they were.
- * Two tokens of one call must not share a key.
+ * Two tokens of one call must not share a key, and the cache's keys and values
+ * must not share their places (the same pointer for both is refused).
  */
 int nvfp4_kv_append(const nvfp4_kv_cache *cache, const nvfp4_attention_batch *batch,
                     const nvfp4_rotary *rotary, const nvfp4_qk_norm *norm,
